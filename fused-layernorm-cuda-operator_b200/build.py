@@ -25,7 +25,8 @@ OBJ = HERE / "build"
 LIB = HERE / "libfln_b200.so"
 
 CU_SOURCES = ["fln_pipeline_bwd_tail_bf16.cu", "fln_pipeline_bwd_tail_f16.cu", "fln_pipeline_bwd_tail_f32.cu", "fln_pipeline_bwd_odd.cu", "fln_pipeline_bwd.cu", "fln_pipeline_bwd_pair.cu", "fln_pipeline_bwd_wide.cu", "fln_pipeline_fwd.cu", "fln_pipeline_fwd_tail_bf16.cu", "fln_pipeline_fwd_tail_f16.cu", "fln_pipeline_fwd_tail_f32.cu", "fln_pipeline_fwd_fp8.cu", "fln_pipeline_fwd_drop.cu", "fln_forward.cu", "fln_backward.cu", "fln_fp8.cu", "fln_host.cu",
-              "fln_pipeline.cu", "fln_static.cu", "fln_dropout.cu"]
+              "fln_pipeline.cu", "fln_static.cu", "fln_dropout.cu",
+              "fln_nga.cu", "fln_rotary.cu", "fln_rotary_f32.cu", "fln_rotary_bf16.cu", "fln_rotary_f16.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC",
@@ -87,22 +88,33 @@ def build_shim(force=False, verbose=False) -> Path:
     import torch
     from torch.utils import cpp_extension as ce
 
-    src = CSRC / "fln_torch_shim.cpp"
+    sources = [CSRC / "fln_torch_shim.cpp", CSRC / "fln_torch_blocks.cpp"]
     out = shim_path()
-    if not force and _newer(out, [src, LIB, *INCLUDE.glob("*.h")]):
+    if not force and _newer(out, [*sources, *CSRC.glob("*.h"), LIB, *INCLUDE.glob("*.h"), HERE / "build.py"]):
         return out
     torch_lib = Path(torch.__file__).parent / "lib"
     cuda_home = Path(ce.CUDA_HOME or "/usr/local/cuda")
     inc = []
     for p in ce.include_paths() + [sysconfig.get_paths()["include"], str(INCLUDE), str(cuda_home / "include")]:
         inc += ["-isystem" if "torch" in p or "python" in p else "-I", p]
-    cmd = [
-        os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+    cxx = [
+        os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC",
         "-DTORCH_EXTENSION_NAME=fused_layernorm_cuda", "-DTORCH_API_INCLUDE_EXTENSION_H",
         "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch.compiled_with_cxx11_abi()),
-        *inc, src, "-o", out,
+        *inc,
+    ]
+    objs = [OBJ / (src.name + ".o") for src in sources]
+    stale = [(src, obj) for src, obj in zip(sources, objs)
+             if force or not _newer(obj, [src, *CSRC.glob("*.h"), *INCLUDE.glob("*.h")])]
+    with cf.ThreadPoolExecutor(max_workers=2) as ex:
+        list(ex.map(lambda so: _run([*cxx, "-c", so[0], "-o", so[1]], verbose), stale))
+    cmd = [
+        os.environ.get("CXX", "g++"), "-shared", *objs, "-o", out,
         "-L", torch_lib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python",
         "-L", HERE, "-lfln_b200",
+        # the C++ runtime that torch has loaded, also where the compiler driver is set up to link its
+        # own statically: with two of them, formatting a number into an error message crashes
+        "-l:libstdc++.so.6",
         "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + str(torch_lib),
     ]
     _run(cmd, verbose)
