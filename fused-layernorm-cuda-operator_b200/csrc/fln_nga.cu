@@ -1,0 +1,548 @@
+// fln_norm_gate_add_norm: entry points, and the kernels that serve every row length, alignment
+// and type (element loads, the row read once per pass).  The formulas stand in fln_nga.cuh.
+#include "fln_nga.cuh"
+
+namespace fln {
+
+constexpr int kLoopThreads = 256;
+
+// ----------------------------------------------------------------------------------------
+// forward, any shape: one CTA per row, which is read three times at most (statistics of N1;
+// the sum; its spread and y) and mostly found in L1 / L2 after the first.
+// ----------------------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ float nga_sum(const NgaParams& p, float v, int c, const T* w1, const T* b1, const T* gate,
+                                         const T* res) {
+  if (w1 != nullptr) v *= p.woff + Cvt<T>::to_f(w1[c]);
+  if (b1 != nullptr) v += Cvt<T>::to_f(b1[c]);
+  if (p.gate_mode != FLN_GATE_NONE) v *= gate_act<sizeof(T) == 4>(Cvt<T>::to_f(gate[c]), p.act);
+  v *= p.ba;
+  if (res != nullptr) v = fmaf(p.ra, Cvt<T>::to_f(res[c]), v);
+  return v;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kLoopThreads) nga_fwd_loop_kernel(const NgaParams p) {
+  __shared__ float red[2 * 32];
+  int flip = 0;
+  const int cols = p.cols;
+  const float inv_n = 1.0f / (float)cols;
+  const T* w1 = reinterpret_cast<const T*>(p.w1);
+  const T* b1 = reinterpret_cast<const T*>(p.b1);
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    const int64_t base = row * (int64_t)cols;
+    const int64_t group = row / p.group_rows;
+    const T* x = reinterpret_cast<const T*>(p.x) + base;
+    const T* res = p.res != nullptr ? reinterpret_cast<const T*>(p.res) + base : nullptr;
+    const T* gate = reinterpret_cast<const T*>(p.gate);
+    if (p.gate_mode == FLN_GATE_GROUP) gate += group * (int64_t)cols;
+    if (p.gate_mode == FLN_GATE_ELEMENT) gate += base;
+    const T* w2 = reinterpret_cast<const T*>(p.w2);
+    const T* b2 = reinterpret_cast<const T*>(p.b2);
+    if (p.affine_grouped) {
+      if (w2 != nullptr) w2 += group * (int64_t)cols;
+      if (b2 != nullptr) b2 += group * (int64_t)cols;
+    }
+    float mean1 = 0.f, rstd1 = 1.f;
+    if (p.post_kind != FLN_NO_NORM) {
+      float v[1] = {0.f};
+      if (p.post_kind == FLN_LAYERNORM) {
+        for (int c = threadIdx.x; c < cols; c += kLoopThreads) v[0] += Cvt<T>::to_f(x[c]);
+        cta_sum<1>(v, red, flip);
+        mean1 = v[0] * inv_n;
+        v[0] = 0.f;
+      }
+      for (int c = threadIdx.x; c < cols; c += kLoopThreads) {
+        const float d = Cvt<T>::to_f(x[c]) - mean1;
+        v[0] = fmaf(d, d, v[0]);
+      }
+      cta_sum<1>(v, red, flip);
+      rstd1 = rsqrtf(fmaf(v[0], inv_n, p.eps1));
+    }
+    auto s_of = [&](int c) { return nga_sum<T>(p, (Cvt<T>::to_f(x[c]) - mean1) * rstd1, c, w1, b1, gate, res); };
+    float mean2 = 0.f, rstd2 = 1.f;
+    if (p.kind != FLN_NO_NORM) {
+      float v[1] = {0.f};
+      if (p.kind == FLN_LAYERNORM) {
+        for (int c = threadIdx.x; c < cols; c += kLoopThreads) v[0] += s_of(c);
+        cta_sum<1>(v, red, flip);
+        mean2 = v[0] * inv_n;
+        v[0] = 0.f;
+      }
+      for (int c = threadIdx.x; c < cols; c += kLoopThreads) {
+        const float d = s_of(c) - mean2;
+        v[0] = fmaf(d, d, v[0]);
+      }
+      cta_sum<1>(v, red, flip);
+      rstd2 = rsqrtf(fmaf(v[0], inv_n, p.eps2));
+    }
+    for (int c = threadIdx.x; c < cols; c += kLoopThreads) {
+      const float s = s_of(c);
+      reinterpret_cast<T*>(p.sum)[base + c] = Cvt<T>::from_f(s);
+      if (p.kind != FLN_NO_NORM) {
+        float v = (s - mean2) * rstd2;
+        if (w2 != nullptr) v *= p.woff + Cvt<T>::to_f(w2[c]);
+        if (b2 != nullptr) v += Cvt<T>::to_f(b2[c]);
+        reinterpret_cast<T*>(p.y)[base + c] = Cvt<T>::from_f(v);
+      }
+    }
+    if (threadIdx.x == 0) {
+      if (p.mean1 != nullptr && p.post_kind == FLN_LAYERNORM) p.mean1[row] = mean1;
+      if (p.rstd1 != nullptr && p.post_kind != FLN_NO_NORM) p.rstd1[row] = rstd1;
+      if (p.mean2 != nullptr && p.kind == FLN_LAYERNORM) p.mean2[row] = mean2;
+      if (p.rstd2 != nullptr && p.kind != FLN_NO_NORM) p.rstd2[row] = rstd2;
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------------------
+// backward, any shape
+// ----------------------------------------------------------------------------------------
+// what one element of one row needs, given the row's scalars
+template <typename T>
+struct NgaBwdRow {
+  const T *x, *res, *dy, *dsum, *gate, *w1, *b1, *w2;
+  float mean1, rstd1, mean2, rstd2, c1, c2;
+  __device__ __forceinline__ void open(const NgaParams& p, int64_t row) {
+    const int64_t base = row * (int64_t)p.cols;
+    const int64_t group = row / p.group_rows;
+    x = reinterpret_cast<const T*>(p.x) + base;
+    res = p.res != nullptr ? reinterpret_cast<const T*>(p.res) + base : nullptr;
+    dy = p.dy != nullptr ? reinterpret_cast<const T*>(p.dy) + base : nullptr;
+    dsum = p.ds != nullptr ? reinterpret_cast<const T*>(p.ds) + base : nullptr;
+    gate = reinterpret_cast<const T*>(p.gate);
+    if (p.gate_mode == FLN_GATE_GROUP) gate += group * (int64_t)p.cols;
+    if (p.gate_mode == FLN_GATE_ELEMENT) gate += base;
+    w1 = reinterpret_cast<const T*>(p.w1);
+    b1 = reinterpret_cast<const T*>(p.b1);
+    w2 = reinterpret_cast<const T*>(p.w2);
+    if (p.affine_grouped && w2 != nullptr) w2 += group * (int64_t)p.cols;
+    mean1 = p.post_kind == FLN_LAYERNORM ? p.mean1[row] : 0.f;
+    rstd1 = p.post_kind != FLN_NO_NORM ? p.rstd1[row] : 1.f;
+    mean2 = p.kind == FLN_LAYERNORM && dy != nullptr ? p.mean2[row] : 0.f;
+    rstd2 = p.kind != FLN_NO_NORM && dy != nullptr ? p.rstd2[row] : 1.f;
+    c1 = c2 = 0.f;
+  }
+  __device__ __forceinline__ float g2(const NgaParams& p, int c) const {
+    float v = Cvt<T>::to_f(dy[c]);
+    if (w2 != nullptr) v *= p.woff + Cvt<T>::to_f(w2[c]);
+    return v;
+  }
+  __device__ __forceinline__ float xh(int c) const { return (Cvt<T>::to_f(x[c]) - mean1) * rstd1; }
+  // the forward's 32-bit sum, made again, normalized
+  __device__ __forceinline__ float sh(const NgaParams& p, int c) const {
+    return (nga_sum<T>(p, xh(c), c, w1, b1, gate, res) - mean2) * rstd2;
+  }
+  __device__ __forceinline__ float dsv(const NgaParams& p, int c) const {
+    float v = dsum != nullptr ? Cvt<T>::to_f(dsum[c]) : 0.f;
+    if (dy != nullptr) v += rstd2 * ((g2(p, c) - c2) - sh(p, c) * c1);
+    return v;
+  }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kLoopThreads) nga_bwd_loop_kernel(const NgaParams p) {
+  constexpr bool EXACT = sizeof(T) == 4;
+  __shared__ float red[2 * 2 * 32];
+  int flip = 0;
+  const int cols = p.cols;
+  const float inv_n = 1.0f / (float)cols;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    const int64_t base = row * (int64_t)cols;
+    NgaBwdRow<T> r;
+    r.open(p, row);
+    if (r.dy != nullptr) {
+      float v[2] = {0.f, 0.f};
+      for (int c = threadIdx.x; c < cols; c += kLoopThreads) {
+        const float g = r.g2(p, c);
+        v[0] = fmaf(g, r.sh(p, c), v[0]);
+        v[1] += g;
+      }
+      cta_sum<2>(v, red, flip);
+      r.c1 = v[0] * inv_n;
+      r.c2 = p.kind == FLN_LAYERNORM ? v[1] * inv_n : 0.f;
+      if (p.row_c != nullptr && threadIdx.x == 0) {
+        p.row_c[2 * row] = r.c1;
+        p.row_c[2 * row + 1] = r.c2;
+      }
+    }
+    auto g1_of = [&](int c, float e) {
+      if (p.gate_mode != FLN_GATE_NONE) e *= gate_act<EXACT>(Cvt<T>::to_f(r.gate[c]), p.act);
+      if (r.w1 != nullptr) e *= p.woff + Cvt<T>::to_f(r.w1[c]);
+      return e;
+    };
+    float v[2] = {0.f, 0.f};
+    for (int c = threadIdx.x; c < cols; c += kLoopThreads) {
+      const float ds = r.dsv(p, c);
+      if (p.dres != nullptr) reinterpret_cast<T*>(p.dres)[base + c] = Cvt<T>::from_f(p.ra * ds);
+      const float e = p.ba * ds;
+      if (p.dgate != nullptr && p.gate_mode == FLN_GATE_ELEMENT) {
+        float n = r.xh(c);
+        if (r.w1 != nullptr) n *= p.woff + Cvt<T>::to_f(r.w1[c]);
+        if (r.b1 != nullptr) n += Cvt<T>::to_f(r.b1[c]);
+        float a, da;
+        gate_act_grad<EXACT>(Cvt<T>::to_f(r.gate[c]), p.act, &a, &da);
+        reinterpret_cast<T*>(p.dgate)[base + c] = Cvt<T>::from_f(e * n * da);
+      }
+      if (p.dx != nullptr && p.post_kind != FLN_NO_NORM) {
+        const float g1 = g1_of(c, e);
+        v[0] = fmaf(g1, r.xh(c), v[0]);
+        v[1] += g1;
+      }
+    }
+    if (p.dx != nullptr) {
+      float d1 = 0.f, d2 = 0.f;
+      if (p.post_kind != FLN_NO_NORM) {
+        cta_sum<2>(v, red, flip);
+        d1 = v[0] * inv_n;
+        d2 = p.post_kind == FLN_LAYERNORM ? v[1] * inv_n : 0.f;
+      }
+      for (int c = threadIdx.x; c < cols; c += kLoopThreads) {
+        const float g1 = g1_of(c, p.ba * r.dsv(p, c));
+        // without a norm xh * d1 would be inf * 0 where x is infinite
+        const float d = p.post_kind != FLN_NO_NORM ? r.rstd1 * ((g1 - d2) - r.xh(c) * d1) : g1;
+        reinterpret_cast<T*>(p.dx)[base + c] = Cvt<T>::from_f(d);
+      }
+    }
+  }
+}
+
+// Column sums of a slot: 32 columns x 8 row lanes per CTA, every term recomputed from the row's
+// scalars (c1, c2 as the row kernel left them).
+template <typename T>
+__global__ void __launch_bounds__(256) nga_bwd_columns_kernel(const NgaParams p) {
+  constexpr bool EXACT = sizeof(T) == 4;
+  __shared__ float tile[8][33];
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31);
+  const int lane = threadIdx.x >> 5;
+  const bool col_ok = c < p.cols;
+  for (int64_t slot = blockIdx.y; slot < p.slots; slot += gridDim.y) {
+    const SlotRows sr = slot_rows(p, slot);
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    if (col_ok) {
+      for (int64_t row = sr.first + lane; row < sr.last; row += 8) {
+        NgaBwdRow<T> r;
+        r.open(p, row);
+        if (r.dy != nullptr) {
+          r.c1 = p.row_c[2 * row];
+          r.c2 = p.row_c[2 * row + 1];
+          const float d = Cvt<T>::to_f(r.dy[c]);
+          if (p.acc & kAccU) acc[2] = fmaf(d, r.sh(p, c), acc[2]);
+          acc[3] += d;
+        }
+        if (p.acc & (kAccP | kAccQ)) {
+          float h = p.ba * r.dsv(p, c);
+          if (p.gate_mode == FLN_GATE_ELEMENT) h *= gate_act<EXACT>(Cvt<T>::to_f(r.gate[c]), p.act);
+          if (p.acc & kAccP) acc[0] = fmaf(h, r.xh(c), acc[0]);
+          acc[1] += h;
+        }
+      }
+    }
+    int k = 0;
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      if (!(p.acc & (1 << a))) continue;
+      __syncthreads();
+      tile[lane][threadIdx.x & 31] = acc[a];
+      __syncthreads();
+      if (lane == 0 && col_ok) {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t += tile[i][threadIdx.x & 31];
+        p.partials[(slot * p.nacc + k) * (int64_t)p.cols + c] = t;
+      }
+      ++k;
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------------------
+// Sums of the partial rows.  blockIdx.y < groups: the gradients that belong to one group each
+// (dgate of a gate per group, dweight / dbias per group); blockIdx.y == groups: those of the
+// vectors shared by all rows.  32 columns x 16 lanes; lane l adds partial rows l, l + 16, ... and
+// the lanes are added in order.  `rep` partial rows per slot.
+// ----------------------------------------------------------------------------------------
+constexpr int kFinalLanes = 16;
+template <typename T>
+__global__ void __launch_bounds__(32 * kFinalLanes) nga_finalize_kernel(const NgaParams p, const NgaGrads g, int rep, int groups) {
+  constexpr bool EXACT = sizeof(T) == 4;
+  __shared__ float tile[kFinalLanes][33];
+  const int tx = threadIdx.x & 31, lane = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + tx;
+  const bool ok = c < p.cols;
+  const int64_t per_group = p.slots_per_group * rep;
+  const bool gate_grouped = p.gate_mode == FLN_GATE_GROUP, gate_vec = p.gate_mode == FLN_GATE_VECTOR;
+  // the sum of one accumulator over partial rows [from, to); with `scaled` each partial row is
+  // multiplied by act(gate) of its group first
+  auto total = [&](int which, int64_t from, int64_t to, bool scaled) {
+    const int k = __popc(p.acc & (which - 1));
+    float t = 0.f;
+    if (ok) {
+      const float* src = p.partials + (int64_t)k * p.cols + c;
+      const int64_t pitch = (int64_t)p.nacc * p.cols;
+      if (scaled) {
+        for (int64_t r = from + lane; r < to; r += kFinalLanes) {
+          const float gv = Cvt<T>::to_f(reinterpret_cast<const T*>(p.gate)[(r / per_group) * p.cols + c]);
+          t = fmaf(gate_act<EXACT>(gv, p.act), src[r * pitch], t);
+        }
+      } else {
+        int64_t r = from + lane;
+        for (; r + 7 * kFinalLanes < to; r += 8 * kFinalLanes) {
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = __ldcg(src + (r + j * kFinalLanes) * pitch);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) t += v[j];
+        }
+        for (; r < to; r += kFinalLanes) t += __ldcg(src + r * pitch);
+      }
+    }
+    __syncthreads();
+    tile[lane][tx] = t;
+    __syncthreads();
+    t = 0.f;
+#pragma unroll
+    for (int i = 0; i < kFinalLanes; ++i) t += tile[i][tx];
+    return t;
+  };
+  const bool writer = ok && lane == 0;
+  auto dgate_of = [&](float P, float Q, int64_t at) {
+    float a, da;
+    gate_act_grad<EXACT>(Cvt<T>::to_f(reinterpret_cast<const T*>(p.gate)[at]), p.act, &a, &da);
+    float w = 1.f;
+    if (p.w1 != nullptr) w = p.woff + Cvt<T>::to_f(reinterpret_cast<const T*>(p.w1)[c]);
+    float n = w * P;
+    if (p.b1 != nullptr) n = fmaf(Cvt<T>::to_f(reinterpret_cast<const T*>(p.b1)[c]), Q, n);
+    reinterpret_cast<T*>(g.dgate)[at] = Cvt<T>::from_f(n * da);
+  };
+  for (int64_t y = blockIdx.y; y <= groups; y += gridDim.y) {
+    if (y < groups) {  // one group
+      const int64_t from = y * per_group, to = from + per_group;
+      const int64_t at = y * p.cols + c;
+      if (gate_grouped && g.dgate != nullptr) {
+        const float P = total(kAccP, from, to, false);
+        const float Q = p.b1 != nullptr ? total(kAccQ, from, to, false) : 0.f;
+        if (writer) dgate_of(P, Q, at);
+      }
+      if (p.affine_grouped) {
+        if (g.dw2 != nullptr) {
+          const float v = total(kAccU, from, to, false);
+          if (writer) reinterpret_cast<T*>(g.dw2)[at] = Cvt<T>::from_f(v);
+        }
+        if (g.db2 != nullptr) {
+          const float v = total(kAccV, from, to, false);
+          if (writer) reinterpret_cast<T*>(g.db2)[at] = Cvt<T>::from_f(v);
+        }
+      }
+    } else {  // vectors shared by all rows
+      const int64_t to = p.slots * rep;
+      const float a = gate_vec && ok ? gate_act<EXACT>(Cvt<T>::to_f(reinterpret_cast<const T*>(p.gate)[c]), p.act) : 1.f;
+      float P = 0.f, Q = 0.f;
+      if (g.dw1 != nullptr || (gate_vec && g.dgate != nullptr)) P = total(kAccP, 0, to, gate_grouped);
+      if (g.db1 != nullptr || (gate_vec && g.dgate != nullptr && p.b1 != nullptr)) Q = total(kAccQ, 0, to, gate_grouped);
+      if (writer) {
+        if (g.dw1 != nullptr) reinterpret_cast<T*>(g.dw1)[c] = Cvt<T>::from_f(a * P);
+        if (g.db1 != nullptr) reinterpret_cast<T*>(g.db1)[c] = Cvt<T>::from_f(a * Q);
+        if (gate_vec && g.dgate != nullptr) dgate_of(P, Q, c);
+      }
+      if (!p.affine_grouped) {
+        if (g.dw2 != nullptr) {
+          const float v = total(kAccU, 0, to, false);
+          if (writer) reinterpret_cast<T*>(g.dw2)[c] = Cvt<T>::from_f(v);
+        }
+        if (g.db2 != nullptr) {
+          const float v = total(kAccV, 0, to, false);
+          if (writer) reinterpret_cast<T*>(g.db2)[c] = Cvt<T>::from_f(v);
+        }
+      }
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------------------
+// host side
+// ----------------------------------------------------------------------------------------
+static int check_args(const fln_nga_args* a) {
+  if (a == nullptr) return FLN_ERR_NULL;
+  auto kind_ok = [](int k) { return k == FLN_LAYERNORM || k == FLN_RMSNORM || k == FLN_NO_NORM; };
+  if (!kind_ok(a->post_kind) || !kind_ok(a->kind)) return FLN_ERR_ARG;
+  if (a->gate_mode < FLN_GATE_NONE || a->gate_mode > FLN_GATE_ELEMENT) return FLN_ERR_ARG;
+  if (a->gate_act < FLN_GATE_ACT_NONE || a->gate_act > FLN_GATE_ACT_TANH) return FLN_ERR_ARG;
+  if (a->dtype != FLN_F32 && a->dtype != FLN_BF16 && a->dtype != FLN_F16) return FLN_ERR_DTYPE;
+  if (a->rows < 0 || a->cols <= 0 || a->cols > 0x7fffffff || a->rows > 0x7fffffff) return FLN_ERR_SHAPE;
+  if (a->rows > 0 && (a->group_rows <= 0 || a->rows % a->group_rows != 0)) return FLN_ERR_SHAPE;
+  if ((a->gate != nullptr) != (a->gate_mode != FLN_GATE_NONE) && a->rows > 0) return FLN_ERR_ARG;
+  if (a->post_kind == FLN_NO_NORM && (a->post_weight != nullptr || a->post_bias != nullptr)) return FLN_ERR_ARG;
+  if (a->kind == FLN_NO_NORM && (a->weight != nullptr || a->bias != nullptr)) return FLN_ERR_ARG;
+  return FLN_OK;
+}
+
+static NgaParams base_params(const fln_nga_args* a) {
+  NgaParams p = {};
+  p.x = a->x;
+  p.res = a->residual;
+  p.gate = a->gate;
+  p.w1 = a->post_weight;
+  p.b1 = a->post_bias;
+  p.w2 = a->weight;
+  p.b2 = a->bias;
+  p.rows = a->rows;
+  p.group_rows = a->group_rows;
+  p.cols = (int)a->cols;
+  p.post_kind = a->post_kind;
+  p.kind = a->kind;
+  p.gate_mode = a->gate_mode;
+  p.act = a->gate_act;
+  p.affine_grouped = a->affine_grouped != 0;
+  p.ba = a->branch_scale;
+  p.ra = a->residual_scale;
+  p.woff = a->weight_offset;
+  p.eps1 = a->post_eps;
+  p.eps2 = a->eps;
+  // groups matter only where something is held per group
+  if (p.gate_mode != FLN_GATE_GROUP && !p.affine_grouped) p.group_rows = a->rows;
+  return p;
+}
+
+// Slots of the loop kernels: 64 rows, more when that would make over a thousand of them.
+static void plan_slots(NgaParams* p) {
+  const int64_t groups = p->rows / p->group_rows;
+  int64_t most = 1024 / groups;
+  if (most < 1) most = 1;
+  int64_t chunk = 64;
+  if ((p->group_rows + chunk - 1) / chunk > most) chunk = (p->group_rows + most - 1) / most;
+  p->chunk = chunk;
+  p->slots_per_group = (p->group_rows + chunk - 1) / chunk;
+  p->slots = p->slots_per_group * groups;
+}
+
+static size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+template <typename T>
+static int run_backward(NgaParams p, const NgaGrads& g, cudaStream_t st) {
+  const int64_t grid = p.rows < 0x7fffffff ? p.rows : 0x7fffffff;
+  nga_bwd_loop_kernel<T><<<(unsigned)grid, kLoopThreads, 0, st>>>(p);
+  FLN_CHECK_LAUNCH();
+  if (p.acc != 0) {
+    const dim3 cg((unsigned)((p.cols + 31) / 32), (unsigned)(p.slots < 65535 ? p.slots : 65535));
+    nga_bwd_columns_kernel<T><<<cg, 256, 0, st>>>(p);
+    FLN_CHECK_LAUNCH();
+    const int64_t groups = p.rows / p.group_rows;
+    const dim3 fg((unsigned)((p.cols + 31) / 32), (unsigned)(groups + 1 < 65535 ? groups + 1 : 65535));
+    nga_finalize_kernel<T><<<fg, 32 * kFinalLanes, 0, st>>>(p, g, 1, (int)groups);
+    FLN_CHECK_LAUNCH();
+  }
+  return FLN_OK;
+}
+
+// the column sums of parameters when there are no rows: zeros
+static int zero_grads(const fln_nga_args* a, const NgaGrads& g, cudaStream_t st) {
+  const size_t n = (size_t)a->cols * (a->dtype == FLN_F32 ? 4 : 2);
+  void* const v[] = {g.dw1, g.db1, a->affine_grouped ? nullptr : g.dw2, a->affine_grouped ? nullptr : g.db2,
+                     a->gate_mode == FLN_GATE_VECTOR ? g.dgate : nullptr};
+  for (void* q : v)
+    if (q != nullptr && cudaMemsetAsync(q, 0, n, st) != cudaSuccess) {
+      cudaGetLastError();
+      return FLN_ERR_LAUNCH;
+    }
+  return FLN_OK;
+}
+
+}  // namespace fln
+
+using namespace fln;
+
+extern "C" int fln_norm_gate_add_norm_forward(const fln_nga_args* a, void* y, void* sum, float* post_mean,
+                                              float* post_rstd, float* mean, float* rstd, void* stream) {
+  const int rc = check_args(a);
+  if (rc != FLN_OK) return rc;
+  if (a->rows == 0) return FLN_OK;
+  if (a->x == nullptr || sum == nullptr) return FLN_ERR_NULL;
+  if (a->kind != FLN_NO_NORM && y == nullptr) return FLN_ERR_NULL;
+  NgaParams p = base_params(a);
+  p.y = y;
+  p.sum = sum;
+  p.mean1 = post_mean;
+  p.rstd1 = post_rstd;
+  p.mean2 = mean;
+  p.rstd2 = rstd;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const unsigned grid = (unsigned)p.rows;
+  switch (a->dtype) {
+    case FLN_F32:
+      nga_fwd_loop_kernel<float><<<grid, kLoopThreads, 0, st>>>(p);
+      break;
+    case FLN_BF16:
+      nga_fwd_loop_kernel<__nv_bfloat16><<<grid, kLoopThreads, 0, st>>>(p);
+      break;
+    default:
+      nga_fwd_loop_kernel<__half><<<grid, kLoopThreads, 0, st>>>(p);
+      break;
+  }
+  FLN_CHECK_LAUNCH();
+  return FLN_OK;
+}
+
+extern "C" size_t fln_norm_gate_add_norm_workspace_bytes(const fln_nga_args* a) {
+  if (check_args(a) != FLN_OK || a->rows == 0) return 0;
+  NgaParams p = base_params(a);
+  plan_slots(&p);
+  return align256((size_t)p.rows * 8) + (size_t)p.slots * 4 * (size_t)p.cols * 4;
+}
+
+extern "C" int fln_norm_gate_add_norm_backward(const fln_nga_args* a, const float* post_mean,
+                                               const float* post_rstd, const float* mean, const float* rstd,
+                                               const void* dy, const void* dsum, void* dx, void* dresidual,
+                                               void* dgate, void* dpost_weight, void* dpost_bias, void* dweight,
+                                               void* dbias, void* workspace, size_t workspace_bytes, void* stream) {
+  const int rc = check_args(a);
+  if (rc != FLN_OK) return rc;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (dgate != nullptr && a->gate_mode == FLN_GATE_NONE) return FLN_ERR_ARG;
+  if (a->post_kind == FLN_NO_NORM && (dpost_weight != nullptr || dpost_bias != nullptr)) return FLN_ERR_ARG;
+  if (a->kind == FLN_NO_NORM && (dweight != nullptr || dbias != nullptr || dy != nullptr)) return FLN_ERR_ARG;
+  const bool shared_gate = a->gate_mode == FLN_GATE_VECTOR || a->gate_mode == FLN_GATE_GROUP;
+  NgaGrads g;
+  g.dgate = shared_gate ? dgate : nullptr;
+  g.dw1 = dpost_weight;
+  g.db1 = dpost_bias;
+  g.dw2 = dweight;
+  g.db2 = dbias;
+  if (a->rows == 0) return zero_grads(a, g, st);
+  if (dy == nullptr && dsum == nullptr) return FLN_ERR_NULL;
+  if (a->x == nullptr) return FLN_ERR_NULL;
+  if (dy != nullptr && (rstd == nullptr || (a->kind == FLN_LAYERNORM && mean == nullptr)))
+    return FLN_ERR_NULL;
+  if (a->post_kind != FLN_NO_NORM && (post_rstd == nullptr || (a->post_kind == FLN_LAYERNORM && post_mean == nullptr)))
+    return FLN_ERR_NULL;
+  NgaParams p = base_params(a);
+  p.mean1 = const_cast<float*>(post_mean);
+  p.rstd1 = const_cast<float*>(post_rstd);
+  p.mean2 = const_cast<float*>(mean);
+  p.rstd2 = const_cast<float*>(rstd);
+  p.dy = dy;
+  p.ds = dsum;
+  p.dx = dx;
+  p.dres = dresidual;
+  p.dgate = dgate;
+  plan_slots(&p);
+  if (g.dw1 != nullptr || g.dgate != nullptr) p.acc |= kAccP;
+  if (g.db1 != nullptr || (g.dgate != nullptr && p.b1 != nullptr)) p.acc |= kAccQ;
+  if (g.dw2 != nullptr) p.acc |= kAccU;
+  if (g.db2 != nullptr) p.acc |= kAccV;
+  p.nacc = __builtin_popcount((unsigned)p.acc);
+  if (p.acc != 0) {
+    if (workspace == nullptr || workspace_bytes < fln_norm_gate_add_norm_workspace_bytes(a)) return FLN_ERR_WORKSPACE;
+    if (!is_aligned16(workspace)) return FLN_ERR_WORKSPACE;
+    p.row_c = reinterpret_cast<float*>(workspace);
+    p.partials = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + align256((size_t)p.rows * 8));
+  }
+  switch (a->dtype) {
+    case FLN_F32:
+      return run_backward<float>(p, g, st);
+    case FLN_BF16:
+      return run_backward<__nv_bfloat16>(p, g, st);
+    default:
+      return run_backward<__half>(p, g, st);
+  }
+}

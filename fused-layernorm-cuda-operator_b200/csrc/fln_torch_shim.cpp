@@ -27,6 +27,7 @@
 #include <vector>
 
 #include "fln_b200.h"
+#include "fln_torch_blocks.h"
 
 namespace {
 
@@ -628,6 +629,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("rstd"), py::arg("gamma") = py::none());
   m.def("device_status", []() { return fln_device_status(); },
         "read and clear the device status word (0 = no kernel reported a problem)");
+
+  fln_bind_blocks(m);  // norms around a block, head norm + rotary positions
 
   m.attr("__version__") = fln_version();
   m.attr("__cuda_version__") = fln_cuda_runtime_version();

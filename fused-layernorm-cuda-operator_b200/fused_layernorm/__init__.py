@@ -11,6 +11,8 @@ from .layernorm import (FusedLayerNorm, FusedLayerNormFunction, fused_layer_norm
 from .rmsnorm import (FusedRMSNorm, fused_add_layer_norm, fused_add_layer_norm_fp8, fused_add_norm_fp8_delayed,
                       fused_add_norm_fp8_rowwise, fused_add_norm_mxfp8, fused_add_norm_nvfp4, fused_add_rms_norm,
                       fused_add_rms_norm_fp8, fused_dropout_add_layer_norm, fused_rms_norm)
+from .blocks import (FusedNormGateAddNorm, FusedQKNormRotary, RotaryAxes, fused_norm_gate_add_norm, fused_qk_norm_rotary,
+                     fused_qk_norm_rotary_)
 
 __version__ = "1.0.0"
 
@@ -33,6 +35,12 @@ __all__ = [
     "fused_add_norm_mxfp8",
     "fused_add_norm_nvfp4",
     "fused_dropout_add_layer_norm",
+    "fused_norm_gate_add_norm",
+    "FusedNormGateAddNorm",
+    "RotaryAxes",
+    "fused_qk_norm_rotary",
+    "fused_qk_norm_rotary_",
+    "FusedQKNormRotary",
 ]
 
 import torch as _torch

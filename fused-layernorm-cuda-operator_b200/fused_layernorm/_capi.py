@@ -17,7 +17,10 @@ _PKG_DIR = Path(__file__).resolve().parents[1]
 LIB_PATH = _PKG_DIR / "libfln_b200.so"
 
 F32, BF16, F16, FP8_E4M3 = 0, 1, 2, 3
-LAYERNORM, RMSNORM = 0, 1
+LAYERNORM, RMSNORM, NO_NORM = 0, 1, 2
+GATE_NONE, GATE_VECTOR, GATE_GROUP, GATE_ELEMENT = 0, 1, 2, 3
+GATE_ACT_NONE, GATE_ACT_SIGMOID, GATE_ACT_SILU, GATE_ACT_TANH = 0, 1, 2, 3
+ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
 ACT_NONE, ACT_GELU_TANH, ACT_GELU_ERF = 0, 1, 2
 DTYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 
@@ -32,6 +35,8 @@ SYMBOLS = [
     "fln_norm_forward_fp8_delayed", "fln_norm_forward_fp8_rowwise", "fln_norm_forward_mxfp8",
     "fln_planner_selftest", "fln_sum_rows_f32", "fln_set_stage_override", "fln_set_wait_limit_ns",
     "fln_set_test_fault", "fln_set_static_scratch_limit", "fln_norm_backward_partial", "fln_dropout_add_norm_forward", "fln_dropout_backward", "fln_norm_forward_nvfp4",
+    "fln_norm_gate_add_norm_forward", "fln_norm_gate_add_norm_workspace_bytes", "fln_norm_gate_add_norm_backward",
+    "fln_qk_norm_rotary_forward", "fln_qk_norm_rotary_workspace_bytes", "fln_qk_norm_rotary_backward",
 ]
 STATIC_SCRATCH_BYTES = 24 << 20  # FLN_STATIC_SCRATCH_BYTES
 
@@ -41,6 +46,30 @@ class LaunchInfo(C.Structure):
                 ("threads_per_row", C.c_int), ("threads_per_cta", C.c_int), ("rows_per_cta", C.c_int),
                 ("grid", C.c_int64), ("sm_count", C.c_int), ("pipelined", C.c_int), ("stages", C.c_int),
                 ("vector_bytes", C.c_int)]
+
+
+class NgaArgs(C.Structure):
+    """fln_nga_args"""
+    _fields_ = ([(n, C.c_void_p) for n in ("x", "residual", "gate", "post_weight", "post_bias", "weight", "bias")]
+                + [(n, C.c_int64) for n in ("rows", "cols", "group_rows")]
+                + [(n, C.c_int) for n in ("dtype", "post_kind", "kind", "gate_mode", "gate_act", "affine_grouped")]
+                + [(n, C.c_float) for n in ("branch_scale", "residual_scale", "weight_offset", "post_eps", "eps")])
+
+
+class RotaryTensor(C.Structure):
+    """fln_rotary_tensor"""
+    _fields_ = ([("in_", C.c_void_p), ("out", C.c_void_p)]
+                + [(n, C.c_int64) for n in ("in_batch", "in_seq", "in_head", "out_batch", "out_seq", "out_head")]
+                + [("weight", C.c_void_p), ("bias", C.c_void_p), ("heads", C.c_int)])
+
+
+class RotaryArgs(C.Structure):
+    """fln_rotary_args"""
+    _fields_ = ([("t", RotaryTensor * 2), ("positions", C.c_void_p)]
+                + [(n, C.c_int64) for n in ("pos_axis", "pos_batch", "pos_seq")]
+                + [("turns", C.c_void_p), ("axis", C.c_void_p), ("batch", C.c_int64), ("seq", C.c_int64)]
+                + [(n, C.c_int) for n in ("head_dim", "pairs", "pos64", "layout", "dtype", "kind")]
+                + [(n, C.c_float) for n in ("weight_offset", "eps", "magnitude")])
 
 
 _lib = None
@@ -102,6 +131,14 @@ def lib() -> C.CDLL:
     L.fln_device_status.restype = i32
     L.fln_set_sm_reserve.argtypes = [i32]
     L.fln_set_sm_reserve.restype = None
+    L.fln_norm_gate_add_norm_forward.argtypes = [C.POINTER(NgaArgs)] + [vp] * 7
+    L.fln_norm_gate_add_norm_workspace_bytes.argtypes = [C.POINTER(NgaArgs)]
+    L.fln_norm_gate_add_norm_workspace_bytes.restype = sz
+    L.fln_norm_gate_add_norm_backward.argtypes = [C.POINTER(NgaArgs)] + [vp] * 14 + [sz, vp]
+    L.fln_qk_norm_rotary_forward.argtypes = [C.POINTER(RotaryArgs), vp]
+    L.fln_qk_norm_rotary_workspace_bytes.argtypes = [C.POINTER(RotaryArgs)]
+    L.fln_qk_norm_rotary_workspace_bytes.restype = sz
+    L.fln_qk_norm_rotary_backward.argtypes = [C.POINTER(RotaryArgs), vp * 2, vp * 2, vp * 2, vp, sz, vp]
     L.fln_layernorm_backward_static.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i32, vp]
     _lib = L
     return L

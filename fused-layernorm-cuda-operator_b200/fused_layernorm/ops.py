@@ -349,3 +349,95 @@ def _(kind, input, residual, gamma, beta, tensor_scale, epsilon):
     s = torch.empty_like(input, memory_format=torch.contiguous_format) if residual is not None else input.new_empty((0,))
     return (input.new_empty((rows, cols // 2), dtype=torch.uint8), s,
             input.new_empty((rows, cols // 16), dtype=torch.uint8), input.new_empty((1,), dtype=torch.float32))
+
+
+# ---------------------------------------------- norm -> gate -> residual add -> norm (blocks.py)
+NO_NORM = 2
+
+
+@torch.library.register_fake("fused_layernorm::norm_gate_add_norm_fwd")
+def _(input, residual, gate, post_weight, post_bias, weight, bias, post_kind, kind, gate_act, branch_scale,
+      residual_scale, weight_offset, post_eps, eps):
+    e = lambda: torch.empty_like(input, memory_format=torch.contiguous_format)
+    rows = input.numel() // input.shape[-1]
+    st = lambda want: input.new_empty((rows if want else 0,), dtype=torch.float32)
+    return (e() if kind != NO_NORM else input.new_empty((0,)), e(), st(post_kind == LAYERNORM), st(post_kind != NO_NORM),
+            st(kind == LAYERNORM), st(kind != NO_NORM))
+
+
+@torch.library.register_fake("fused_layernorm::norm_gate_add_norm_bwd")
+def _(grad_y, grad_sum, input, residual, gate, post_weight, post_bias, weight, bias, post_mean, post_rstd, mean, rstd,
+      post_kind, kind, gate_act, branch_scale, residual_scale, weight_offset, post_eps, eps, need):
+    need = list(need)
+    if grad_y is None:
+        need[5] = need[6] = False
+    like = (input, residual, gate, post_weight, post_bias, weight, bias)
+    return tuple(torch.empty_like(t, memory_format=torch.contiguous_format) if n and t is not None else input.new_empty((0,))
+                 for n, t in zip(need, like))
+
+
+def _nga_setup(ctx, inputs, output):
+    input, residual, gate, pw, pb, w, b = inputs[:7]
+    _y, _s, m1, r1, m2, r2 = output
+    ctx.save_for_backward(input, residual, gate, pw, pb, w, b, m1, r1, m2, r2)
+    ctx.conf = inputs[7:]
+    ctx.present = [t is not None for t in inputs[:7]]
+    ctx.set_materialize_grads(False)
+
+
+def _nga_backward(ctx, gy, gs, *_stats):
+    input, residual, gate, pw, pb, w, b, m1, r1, m2, r2 = ctx.saved_tensors
+    none = (None,) * (7 + len(ctx.conf))
+    if ctx.conf[1] == NO_NORM:
+        gy = None
+    if gy is None and gs is None:
+        return none
+    need = [bool(n) and p for n, p in zip(ctx.needs_input_grad[:7], ctx.present)]
+    out = ops.norm_gate_add_norm_bwd(gy, gs, input, residual, gate, pw, pb, w, b, m1, r1, m2, r2, *ctx.conf, need)
+    if gy is None:
+        need[5] = need[6] = False
+    return tuple(g if n else None for g, n in zip(out, need)) + none[7:]
+
+
+torch.library.register_autograd("fused_layernorm::norm_gate_add_norm_fwd", _nga_backward, setup_context=_nga_setup)
+
+
+# --------------------------------------------------------- head norm -> rotary positions (blocks.py)
+@torch.library.register_fake("fused_layernorm::qk_norm_rotary_fwd")
+def _(q, k, positions, turns, axis, q_weight, k_weight, q_bias, k_bias, pairs, axes, layout, kind, eps, weight_offset,
+      magnitude):
+    e = lambda t: torch.empty_like(t, memory_format=torch.contiguous_format) if t is not None else q.new_empty((0,))
+    return e(q), e(k)
+
+
+@torch.library.register_fake("fused_layernorm::qk_norm_rotary_bwd")
+def _(grad_q, grad_k, q, k, positions, turns, axis, q_weight, k_weight, q_bias, k_bias, pairs, axes, layout, kind, eps,
+      weight_offset, magnitude, need):
+    arrives = [grad_q is not None, grad_k is not None] * 3
+    return tuple(torch.empty_like(t, memory_format=torch.contiguous_format) if n and a and t is not None
+                 else q.new_empty((0,))
+                 for n, a, t in zip(need, arrives, (q, k, q_weight, k_weight, q_bias, k_bias)))
+
+
+def _rotary_setup(ctx, inputs, output):
+    ctx.save_for_backward(*inputs[:9])
+    ctx.conf = inputs[9:]
+    ctx.set_materialize_grads(False)
+
+
+def _rotary_backward(ctx, gq, gk):
+    t = ctx.saved_tensors
+    q, k, _pos, _turns, _axis, qw, kw, qb, kb = t
+    if k is None:
+        gk = None
+    arrives = [gq is not None, gk is not None] * 3
+    at = (0, 1, 5, 6, 7, 8)
+    need = [bool(ctx.needs_input_grad[i]) and t[i] is not None and a for i, a in zip(at, arrives)]
+    out = [None] * (9 + len(ctx.conf))
+    if any(need):
+        for i, n, g in zip(at, need, ops.qk_norm_rotary_bwd(gq, gk, *t, *ctx.conf, need)):
+            out[i] = g if n else None
+    return tuple(out)
+
+
+torch.library.register_autograd("fused_layernorm::qk_norm_rotary_fwd", _rotary_backward, setup_context=_rotary_setup)

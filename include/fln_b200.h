@@ -392,6 +392,111 @@ int fln_set_wait_limit_ns(unsigned long long ns);
  * return through their ordinary give-up paths.  No counterpart in the reference. */
 int fln_set_test_fault(int bits);
 
+/* ----------------------------------------------------------------------------------
+ * The norms around a block, fused with its gate and residual scale
+ *     s = residual_scale * residual + branch_scale * act(gate) * N1(x)
+ *     y = N2(s)
+ * N1 is the norm behind the block (`post_*`), N2 the norm in front of the next one; each is
+ * LayerNorm, RMSNorm or nothing (FLN_NO_NORM), scaled by (weight_offset + weight) and shifted by
+ * bias where those are given.  s is kept in 32 bits for N2 and rounded once, into `sum`.
+ * The rows come in groups of `group_rows` consecutive rows (the tokens of a sample;
+ * group_rows must divide rows): a gate of mode FLN_GATE_GROUP and, with affine_grouped, weight
+ * and bias hold one vector of `cols` per group, [rows / group_rows, cols].  No counterpart in
+ * the reference. */
+typedef enum { FLN_NO_NORM = 2 } fln_kind_ext;
+typedef enum {
+  FLN_GATE_NONE = 0,
+  FLN_GATE_VECTOR = 1, /* [cols]                       */
+  FLN_GATE_GROUP = 2,  /* [rows / group_rows, cols]    */
+  FLN_GATE_ELEMENT = 3 /* [rows, cols]                 */
+} fln_gate_mode;
+typedef enum { FLN_GATE_ACT_NONE = 0, FLN_GATE_ACT_SIGMOID = 1, FLN_GATE_ACT_SILU = 2, FLN_GATE_ACT_TANH = 3 } fln_gate_act;
+
+typedef struct {
+  const void* x;           /* [rows, cols], the output of the block             */
+  const void* residual;    /* [rows, cols] or NULL                              */
+  const void* gate;        /* by gate_mode; NULL for FLN_GATE_NONE              */
+  const void* post_weight; /* [cols] or NULL                                    */
+  const void* post_bias;   /* [cols] or NULL                                    */
+  const void* weight;      /* [cols] or, affine_grouped, one per group; or NULL */
+  const void* bias;        /* like weight                                       */
+  int64_t rows, cols, group_rows;
+  int dtype; /* FLN_F32, FLN_BF16 or FLN_F16, of all tensors */
+  int post_kind, kind;
+  int gate_mode, gate_act;
+  int affine_grouped;
+  float branch_scale, residual_scale, weight_offset, post_eps, eps;
+} fln_nga_args;
+
+/* y may be NULL when kind is FLN_NO_NORM, and only then.  The statistics (fp32 [rows], each may
+ * be NULL) are what the backward reads: post_mean / mean of a LayerNorm, post_rstd / rstd of
+ * either norm. */
+int fln_norm_gate_add_norm_forward(const fln_nga_args* a, void* y, void* sum, float* post_mean, float* post_rstd,
+                                   float* mean, float* rstd, void* stream);
+
+/* Bytes of scratch the backward of this problem needs when any of dgate (of a shared gate),
+ * dpost_weight, dpost_bias, dweight, dbias is asked for, and 0 for invalid arguments. */
+size_t fln_norm_gate_add_norm_workspace_bytes(const fln_nga_args* a);
+
+/* Gradients from dy (of y; may be NULL) and dsum (of sum; may be NULL, but not both) and the
+ * forward's inputs: the 32-bit sum is made again from x and residual.  Every gradient may be
+ * NULL (not computed); each has the shape and type of its tensor.  Sums over
+ * rows are made in 32 bits in a fixed order: repeated calls agree bit for bit. */
+int fln_norm_gate_add_norm_backward(const fln_nga_args* a, const float* post_mean,
+                                    const float* post_rstd, const float* mean, const float* rstd, const void* dy,
+                                    const void* dsum, void* dx, void* dresidual, void* dgate, void* dpost_weight,
+                                    void* dpost_bias, void* dweight, void* dbias, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
+/* ----------------------------------------------------------------------------------
+ * Norm of every q and k head, then the rotation of rotary positions with one or several axes.
+ * A row is one head of one token (`head_dim` elements); LayerNorm, RMSNorm or nothing, then the
+ * first 2 * pairs elements are rotated in pairs by
+ *     angle(token, i) = position[axis[i]][token] * inv_freq[i]
+ * with pairs (i, i + pairs) (FLN_ROTARY_HALF) or (2i, 2i + 1) (FLN_ROTARY_INTERLEAVED), and
+ * scaled by `magnitude`; the rest of the row is only normalized.  turns[i] is
+ * inv_freq[i] / (2 pi) as a 64-bit binary fraction: the product with an integer position modulo
+ * 2^64 is the fraction of a turn, exact to |position| * 2^-65 turns at any distance.
+ * Tokens are numbered [batch][seq]; strides are in elements, the last dimension is contiguous.
+ * No counterpart in the reference. */
+typedef enum { FLN_ROTARY_HALF = 0, FLN_ROTARY_INTERLEAVED = 1 } fln_rotary_layout;
+
+typedef struct {
+  const void* in; /* [batch, seq, heads, head_dim] with these strides */
+  void* out;      /* may be `in` with the same strides: every row is read before it is written */
+  int64_t in_batch, in_seq, in_head;
+  int64_t out_batch, out_seq, out_head;
+  const void* weight; /* [head_dim] or NULL */
+  const void* bias;   /* [head_dim] or NULL */
+  int heads;          /* 0: this tensor is absent */
+} fln_rotary_tensor;
+
+typedef struct {
+  fln_rotary_tensor t[2]; /* q, k */
+  const void* positions;  /* int32 or int64: element (axis a, batch b, seq s) at a * pos_axis + b * pos_batch + s * pos_seq */
+  int64_t pos_axis, pos_batch, pos_seq;
+  const uint64_t* turns;     /* device, [pairs] */
+  const unsigned char* axis; /* device, [pairs], each < number of axes */
+  int64_t batch, seq;
+  int head_dim, pairs;
+  int pos64;  /* 1: positions are int64, 0: int32 */
+  int layout; /* fln_rotary_layout */
+  int dtype;
+  int kind; /* fln_kind or FLN_NO_NORM */
+  float weight_offset, eps, magnitude;
+} fln_rotary_args;
+
+int fln_qk_norm_rotary_forward(const fln_rotary_args* a, void* stream);
+
+/* Scratch for the backward when any weight or bias gradient is asked for. */
+size_t fln_qk_norm_rotary_workspace_bytes(const fln_rotary_args* a);
+
+/* a->t[].in are the forward's inputs and a->t[].out the gradients of its outputs (read; with
+ * the out strides).  dx[i]: gradient of t[i].in, contiguous [batch, seq, heads, head_dim], may
+ * be NULL.  dweight / dbias: [head_dim], may be NULL.  Fixed order of summation. */
+int fln_qk_norm_rotary_backward(const fln_rotary_args* a, void* const dx[2], void* const dweight[2],
+                                void* const dbias[2], void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
