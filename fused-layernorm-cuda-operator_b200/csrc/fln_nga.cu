@@ -1,8 +1,23 @@
-// fln_norm_gate_add_norm: entry points, and the kernels that serve every row length, alignment
-// and type (element loads, the row read once per pass).  The formulas stand in fln_nga.cuh.
-#include "fln_nga.cuh"
+// fln_norm_gate_add_norm: entry points and launch plans; the kernels that serve every row length
+// and alignment (element loads, the row read once per pass), and the sum of the partial rows.
+// Rows of whole 16-byte vectors that fit a CTA's registers go to fln_nga_rows.cuh.  The formulas
+// stand in fln_nga.cuh.
+#include <initializer_list>
+
+#include "fln_nga_rows.cuh"
 
 namespace fln {
+
+// explicit instantiations live in fln_nga_{f32,bf16,f16}.cu
+#define FLN_NGA_DECLARE(T)                                                              \
+  template <>                                                                           \
+  int nga_fwd_rows<T>(const NgaParams&, const NgaGeom&, int, cudaStream_t);             \
+  template <>                                                                           \
+  int nga_bwd_rows<T>(const NgaParams&, const NgaGeom&, int, cudaStream_t);
+FLN_NGA_DECLARE(float)
+FLN_NGA_DECLARE(__nv_bfloat16)
+FLN_NGA_DECLARE(__half)
+#undef FLN_NGA_DECLARE
 
 constexpr int kLoopThreads = 256;
 
@@ -416,10 +431,123 @@ static void plan_slots(NgaParams* p) {
   p->slots = p->slots_per_group * groups;
 }
 
+// threads that own a row when each holds K of its nv vectors
+static int threads_per_row(int nv, int K) {
+  const int t = (nv + K - 1) / K;
+  if (t > 32) return (t + 31) & ~31;
+  int w = 1;
+  while (w < t) w <<= 1;
+  return w;
+}
+
+static bool row_vectors(const NgaParams& p, int es) { return p.cols % (16 / es) == 0 && p.cols <= (1 << 20); }
+
+// The forward's plan.  K = 0: not for the row kernels.
+static int plan_forward(const NgaParams& p, int es, NgaGeom* g) {
+  if (!row_vectors(p, es)) return 0;
+  const int nv = p.cols * es / 16, vec = 16 / es;
+  g->nv = nv;
+  int K = 2;
+  int fK = 0, ftpr = 0;
+  plan_override(&fK, &ftpr);
+  if (fK == 1 || fK == 2 || fK == 4) K = fK;
+  auto most = [&](int k) { return k * vec <= 16 ? 1024 : 512; };
+  if (threads_per_row(nv, K) > most(K)) K = 4;
+  if (threads_per_row(nv, K) > most(K)) return 0;
+  g->tpr = threads_per_row(nv, K);
+  g->R = g->tpr >= 128 ? 1 : (g->tpr > 32 ? 2 : 256 / g->tpr);
+  g->threads = g->R * g->tpr;
+  g->grid = (p.rows + g->R - 1) / g->R;
+  return K;
+}
+
+// The backward's plan: threads and shared memory so that an SM holds as many threads as the
+// kernels' registers allow (768 with 8 elements per thread, 512 with 16), at least two rows on
+// their way per row group.  Fills p's slots.  K = 0: not for the row kernels.
+static int plan_backward(NgaParams* p, int es, NgaGeom* g) {
+  if (!row_vectors(*p, es)) return 0;
+  const int vec = 16 / es;
+  const bool four = (p->acc & (kAccQ | kAccV)) != 0;
+  g->nv = p->cols * es / 16;
+  int K = 16 / vec;  // 16 elements per thread
+  if (four) K = 8 / vec;
+  int fK = 0, ftpr = 0;
+  plan_override(&fK, &ftpr);
+  if (fK == 1 || fK == 2 || (fK == 4 && es == 4)) K = fK;
+  auto most = [&](int k) { return k * vec <= 8 ? 768 : 512; };
+  if (threads_per_row(g->nv, K) > most(K)) K = 16 / vec;
+  if (threads_per_row(g->nv, K) > most(K)) return 0;
+  g->tpr = threads_per_row(g->nv, K);
+  g->R = g->tpr >= 128 ? 1 : (g->tpr > 32 ? 2 : 256 / g->tpr);
+  g->threads = g->R * g->tpr;
+  g->rep = g->tpr < 32 ? g->threads / 32 : g->R;
+  const NgaBwdLayout l = nga_bwd_layout(*p, es);
+  const size_t unit = (size_t)K * g->threads * 16;
+  const size_t room = 227 * 1024;
+  int ctas = most(K) / g->threads;
+  if (ctas < 1) ctas = 1;
+  for (; ctas >= 1; --ctas) {
+    const size_t per = room / ctas - 1024;  // the runtime keeps 1 KB of every CTA
+    const size_t fixed = kNgaBwdHeader + (size_t)l.params * unit;
+    if (fixed + 2 * (size_t)l.tensors * unit > per) continue;
+    int s = (int)((per - fixed) / ((size_t)l.tensors * unit));
+    if (s > 4) s = 4;
+    g->stages = s;
+    g->smem = fixed + (size_t)s * l.tensors * unit;
+    break;
+  }
+  if (ctas < 1) return 0;
+  // Slots: as many per group as give every CTA the same number of row steps, nearly; a slot's own
+  // cost (its partial rows) counts as one more step.
+  const int64_t groups = p->rows / p->group_rows, T = p->group_rows;
+  const int64_t slots_max = (T + g->R - 1) / g->R;
+  const int64_t cta = (int64_t)usable_sms() * ctas;
+  int64_t best = -1, best_cost = 0;
+  auto consider = [&](int64_t spg) {
+    if (spg < 1) spg = 1;
+    if (spg > slots_max) spg = slots_max;
+    const int64_t chunk = (T + spg - 1) / spg;
+    const int64_t n = (T + chunk - 1) / chunk * groups;
+    const int64_t cost = (n + cta - 1) / cta * ((chunk + g->R - 1) / g->R + 1);
+    if (best < 0 || cost < best_cost) {
+      best = spg;
+      best_cost = cost;
+    }
+  };
+  for (int64_t w = 1; w <= 8; ++w) consider(w * cta / groups);
+  consider(1);
+  p->chunk = (T + best - 1) / best;
+  p->slots_per_group = (T + p->chunk - 1) / p->chunk;
+  p->slots = p->slots_per_group * groups;
+  g->grid = p->slots < cta ? p->slots : cta;
+  return K;
+}
+
 static size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 template <typename T>
-static int run_backward(NgaParams p, const NgaGrads& g, cudaStream_t st) {
+static int finalize(const NgaParams& p, const NgaGrads& g, int rep, cudaStream_t st) {
+  const int64_t groups = p.rows / p.group_rows;
+  const dim3 fg((unsigned)((p.cols + 31) / 32), (unsigned)(groups + 1 < 65535 ? groups + 1 : 65535));
+  nga_finalize_kernel<T><<<fg, 32 * kFinalLanes, 0, st>>>(p, g, rep, (int)groups);
+  FLN_CHECK_LAUNCH();
+  return FLN_OK;
+}
+
+template <typename T>
+static int run_backward(NgaParams p, const NgaGrads& g, bool aligned, cudaStream_t st) {
+  if (aligned) {
+    NgaParams q = p;
+    NgaGeom geom = {};
+    const int K = plan_backward(&q, (int)sizeof(T), &geom);
+    if (K != 0) {
+      q.partials = p.row_c;  // the whole workspace: the row scalars are not kept
+      const int rc = nga_bwd_rows<T>(q, geom, K, st);
+      if (rc != FLN_OK || q.acc == 0) return rc;
+      return finalize<T>(q, g, geom.rep, st);
+    }
+  }
+  plan_slots(&p);
   const int64_t grid = p.rows < 0x7fffffff ? p.rows : 0x7fffffff;
   nga_bwd_loop_kernel<T><<<(unsigned)grid, kLoopThreads, 0, st>>>(p);
   FLN_CHECK_LAUNCH();
@@ -427,12 +555,15 @@ static int run_backward(NgaParams p, const NgaGrads& g, cudaStream_t st) {
     const dim3 cg((unsigned)((p.cols + 31) / 32), (unsigned)(p.slots < 65535 ? p.slots : 65535));
     nga_bwd_columns_kernel<T><<<cg, 256, 0, st>>>(p);
     FLN_CHECK_LAUNCH();
-    const int64_t groups = p.rows / p.group_rows;
-    const dim3 fg((unsigned)((p.cols + 31) / 32), (unsigned)(groups + 1 < 65535 ? groups + 1 : 65535));
-    nga_finalize_kernel<T><<<fg, 32 * kFinalLanes, 0, st>>>(p, g, 1, (int)groups);
-    FLN_CHECK_LAUNCH();
+    return finalize<T>(p, g, 1, st);
   }
   return FLN_OK;
+}
+
+static bool all_aligned(std::initializer_list<const void*> ps) {
+  for (const void* q : ps)
+    if (!is_aligned16(q)) return false;
+  return true;
 }
 
 // the column sums of parameters when there are no rows: zeros
@@ -467,6 +598,15 @@ extern "C" int fln_norm_gate_add_norm_forward(const fln_nga_args* a, void* y, vo
   p.mean2 = mean;
   p.rstd2 = rstd;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (all_aligned({a->x, a->residual, a->gate, a->post_weight, a->post_bias, a->weight, a->bias, y, sum})) {
+    NgaGeom g = {};
+    const int K = plan_forward(p, a->dtype == FLN_F32 ? 4 : 2, &g);
+    if (K != 0) {
+      if (a->dtype == FLN_F32) return nga_fwd_rows<float>(p, g, K, st);
+      if (a->dtype == FLN_BF16) return nga_fwd_rows<__nv_bfloat16>(p, g, K, st);
+      return nga_fwd_rows<__half>(p, g, K, st);
+    }
+  }
   const unsigned grid = (unsigned)p.rows;
   switch (a->dtype) {
     case FLN_F32:
@@ -485,9 +625,25 @@ extern "C" int fln_norm_gate_add_norm_forward(const fln_nga_args* a, void* y, vo
 
 extern "C" size_t fln_norm_gate_add_norm_workspace_bytes(const fln_nga_args* a) {
   if (check_args(a) != FLN_OK || a->rows == 0) return 0;
+  // the most that any of the plans takes: which one it is depends on the gradients asked for and
+  // on the alignment of all tensors
   NgaParams p = base_params(a);
+  const size_t row = 4 * (size_t)p.cols * 4;
   plan_slots(&p);
-  return align256((size_t)p.rows * 8) + (size_t)p.slots * 4 * (size_t)p.cols * 4;
+  size_t most = align256((size_t)p.rows * 8) + (size_t)p.slots * row;
+  for (int acc = kAccP | kAccU; acc <= 15; acc += kAccQ | kAccV) {
+    for (int grads = 1; grads <= 3; ++grads) {  // dy, dsum, both
+      NgaParams q = base_params(a);
+      NgaGeom g = {};
+      q.acc = acc;
+      q.dy = (grads & 1) != 0 && a->kind != FLN_NO_NORM ? a->x : nullptr;
+      q.ds = (grads & 2) != 0 ? a->x : nullptr;
+      if (plan_backward(&q, a->dtype == FLN_F32 ? 4 : 2, &g) == 0) continue;
+      const size_t n = (size_t)q.slots * g.rep * row;
+      if (n > most) most = n;
+    }
+  }
+  return most;
 }
 
 extern "C" int fln_norm_gate_add_norm_backward(const fln_nga_args* a, const float* post_mean,
@@ -525,7 +681,6 @@ extern "C" int fln_norm_gate_add_norm_backward(const fln_nga_args* a, const floa
   p.dx = dx;
   p.dres = dresidual;
   p.dgate = dgate;
-  plan_slots(&p);
   if (g.dw1 != nullptr || g.dgate != nullptr) p.acc |= kAccP;
   if (g.db1 != nullptr || (g.dgate != nullptr && p.b1 != nullptr)) p.acc |= kAccQ;
   if (g.dw2 != nullptr) p.acc |= kAccU;
@@ -537,12 +692,14 @@ extern "C" int fln_norm_gate_add_norm_backward(const fln_nga_args* a, const floa
     p.row_c = reinterpret_cast<float*>(workspace);
     p.partials = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + align256((size_t)p.rows * 8));
   }
+  const bool aligned = all_aligned({a->x, a->residual, a->gate, a->post_weight, a->post_bias, a->weight, dy, dsum, dx,
+                                    dresidual, dgate});
   switch (a->dtype) {
     case FLN_F32:
-      return run_backward<float>(p, g, st);
+      return run_backward<float>(p, g, aligned, st);
     case FLN_BF16:
-      return run_backward<__nv_bfloat16>(p, g, st);
+      return run_backward<__nv_bfloat16>(p, g, aligned, st);
     default:
-      return run_backward<__half>(p, g, st);
+      return run_backward<__half>(p, g, aligned, st);
   }
 }
