@@ -2,6 +2,8 @@
 // and alignment (element loads, the row read once per pass), and the sum of the partial rows.
 // Rows of whole 16-byte vectors that fit a CTA's registers go to fln_nga_rows.cuh.  The formulas
 // stand in fln_nga.cuh.
+#include <stdlib.h>
+
 #include <initializer_list>
 
 #include "fln_nga_rows.cuh"
@@ -442,61 +444,93 @@ static int threads_per_row(int nv, int K) {
 
 static bool row_vectors(const NgaParams& p, int es) { return p.cols % (16 / es) == 0 && p.cols <= (1 << 20); }
 
+// tuning (temporary)
+static int env(const char* n, int d) { const char* v = getenv(n); return v ? atoi(v) : d; }
+
+// rows per CTA: rows of 128 threads and more one at a time, shorter ones until there are 256 threads
+static void rows_per_cta(NgaGeom* g) {
+  g->R = g->tpr >= 128 ? 1 : (g->tpr > 32 ? 2 : 256 / g->tpr);
+  g->threads = g->R * g->tpr;
+}
+
 // The forward's plan.  K = 0: not for the row kernels.
 static int plan_forward(const NgaParams& p, int es, NgaGeom* g) {
   if (!row_vectors(p, es)) return 0;
   const int nv = p.cols * es / 16, vec = 16 / es;
   g->nv = nv;
-  int K = 2;
+  int E = 16;  // elements per thread
   int fK = 0, ftpr = 0;
   plan_override(&fK, &ftpr);
-  if (fK == 1 || fK == 2 || fK == 4) K = fK;
-  auto most = [&](int k) { return k * vec <= 16 ? 1024 : 512; };
-  if (threads_per_row(nv, K) > most(K)) K = 4;
-  if (threads_per_row(nv, K) > most(K)) return 0;
+  if (fK == 1 || fK == 2 || fK == 4) E = 8 * fK;
+  if (threads_per_row(nv, E / vec) > 512) E = E < 16 ? 16 : 32;
+  if (threads_per_row(nv, E / vec) > 512) E = 32;
+  if (threads_per_row(nv, E / vec) > 512) return 0;
+  const int K = E / vec;
   g->tpr = threads_per_row(nv, K);
-  g->R = g->tpr >= 128 ? 1 : (g->tpr > 32 ? 2 : 256 / g->tpr);
-  g->threads = g->R * g->tpr;
-  g->grid = (p.rows + g->R - 1) / g->R;
+  rows_per_cta(g);
+  const int tensors = 1 + (p.res != nullptr) + (p.gate_mode == FLN_GATE_ELEMENT);
+  g->stages = env("NGA_FS", 3);
+  g->smem = 512 + (size_t)g->stages * tensors * K * g->threads * 16;
+  while (g->smem > 220 * 1024) {
+    if (--g->stages < 2) return 0;
+    g->smem = 512 + (size_t)g->stages * tensors * K * g->threads * 16;
+  }
+  const int64_t groups = p.rows / p.group_rows;
+  const int64_t slots = (int64_t)sm_count() * (768 / g->threads > 0 ? 768 / g->threads : 1);
+  int64_t chunk = p.rows / (slots * env("NGA_FW", 6));
+  const int64_t cap = env("NGA_FC", 16);
+  if (chunk > cap * g->R) chunk = cap * g->R;
+  chunk = (chunk + g->R - 1) / g->R * g->R;
+  if (chunk < g->R) chunk = g->R;
+  if (chunk > p.group_rows) chunk = p.group_rows;
+  g->per_group = (p.group_rows + chunk - 1) / chunk;
+  g->chunk = (p.group_rows + g->per_group - 1) / g->per_group;
+  g->chunk = (g->chunk + g->R - 1) / g->R * g->R;
+  g->per_group = (p.group_rows + g->chunk - 1) / g->chunk;
+  g->grid = g->per_group * groups;
+  if (g->grid > 0x7fffffff) return 0;
   return K;
 }
 
 // The backward's plan: threads and shared memory so that an SM holds as many threads as the
-// kernels' registers allow (768 with 8 elements per thread, 512 with 16), at least two rows on
+// kernels' registers allow (640 with 8 elements per thread, 512 with 16), at least two rows on
 // their way per row group.  Fills p's slots.  K = 0: not for the row kernels.
 static int plan_backward(NgaParams* p, int es, NgaGeom* g) {
   if (!row_vectors(*p, es)) return 0;
   const int vec = 16 / es;
-  const bool four = (p->acc & (kAccQ | kAccV)) != 0;
   g->nv = p->cols * es / 16;
-  int K = 16 / vec;  // 16 elements per thread
-  if (four) K = 8 / vec;
+  auto most = [&](int e) { return e <= 8 ? 640 : 512; };
+  int E = nga_general(*p) ? 8 : 16;
   int fK = 0, ftpr = 0;
   plan_override(&fK, &ftpr);
-  if (fK == 1 || fK == 2 || (fK == 4 && es == 4)) K = fK;
-  auto most = [&](int k) { return k * vec <= 8 ? 768 : 512; };
-  if (threads_per_row(g->nv, K) > most(K)) K = 16 / vec;
-  if (threads_per_row(g->nv, K) > most(K)) return 0;
+  if (fK == 1 || fK == 2) E = 8 * fK;
+  if (threads_per_row(g->nv, E / vec) > most(E)) E = 16;
+  if (threads_per_row(g->nv, E / vec) > most(E)) return 0;
+  const int K = E / vec;
   g->tpr = threads_per_row(g->nv, K);
-  g->R = g->tpr >= 128 ? 1 : (g->tpr > 32 ? 2 : 256 / g->tpr);
-  g->threads = g->R * g->tpr;
+  rows_per_cta(g);
   g->rep = g->tpr < 32 ? g->threads / 32 : g->R;
-  const NgaBwdLayout l = nga_bwd_layout(*p, es);
   const size_t unit = (size_t)K * g->threads * 16;
-  const size_t room = 227 * 1024;
-  int ctas = most(K) / g->threads;
+  int ctas = most(E) / g->threads;
   if (ctas < 1) ctas = 1;
-  for (; ctas >= 1; --ctas) {
-    const size_t per = room / ctas - 1024;  // the runtime keeps 1 KB of every CTA
-    const size_t fixed = kNgaBwdHeader + (size_t)l.params * unit;
-    if (fixed + 2 * (size_t)l.tensors * unit > per) continue;
-    int s = (int)((per - fixed) / ((size_t)l.tensors * unit));
-    if (s > 4) s = 4;
-    g->stages = s;
-    g->smem = fixed + (size_t)s * l.tensors * unit;
-    break;
+  bool fits = false;
+  for (; ctas >= 1 && !fits; --ctas) {
+    const size_t per = (size_t)227 * 1024 / ctas - 1024;  // the runtime keeps 1 KB of every CTA
+    for (int csm = 1; csm >= 0 && !fits; --csm) {
+      const NgaBwdLayout l = nga_bwd_layout(*p, es, csm != 0);
+      const size_t fixed = kNgaBwdHeader + (size_t)l.coefs * unit, stage = (size_t)l.tensors * unit;
+      if (fixed + 2 * stage > per) continue;
+      int s = (int)((per - fixed) / stage);
+      const int cap = env("NGA_BS", 4);
+      if (s > cap) s = cap;
+      g->csm = csm;
+      g->stages = s;
+      g->smem = fixed + (size_t)s * stage;
+      fits = true;
+    }
+    if (fits) break;
   }
-  if (ctas < 1) return 0;
+  if (!fits) return 0;
   // Slots: as many per group as give every CTA the same number of row steps, nearly; a slot's own
   // cost (its partial rows) counts as one more step.
   const int64_t groups = p->rows / p->group_rows, T = p->group_rows;

@@ -5,6 +5,22 @@
 // A row is owned by `tpr` consecutive threads: a power of two within a warp, or whole warps.
 // Thread `lane` of them holds vectors lane, lane + tpr, ... (K of them, the last ones may lie
 // behind the row).
+//
+// At 16 bits these kernels run out of issue slots before they run out of HBM, so the arithmetic is
+// on register pairs (packed fp32), and what is constant over the rows of a group is folded into
+// 32-bit coefficients once per group:
+//     no gate or a shared one     C1 = ba * act(gate) * w1,  B1 = ba * act(gate) * b1
+//                                 s  = xh * C1 + B1 + ra * residual,    g1 = ds * C1
+//     a gate per element          C1 = ba * w1,  B1 = ba * b1,  a = act(gate)
+//                                 s  = a * (xh * C1 + B1) + ra * residual,
+//                                 dgate = ds * (xh * C1 + B1) * act'(gate),  g1 = ds * a * C1
+//     C2 = w2, B2 = b2            y  = sh * C2 + B2,                    g2 = dy * C2
+// The column sums P and Q are kept of ds (times a) and multiplied by ba when they are left.
+// The unfolded form on single floats took 48 (forward) and 84 (backward) instructions per element
+// at 16384 x 4096 bf16: 127 and 248 us.
+//
+// GEN = false: both norms RMSNorm or none and no bias, which is what most blocks have; no means, no
+// Q and V.  GEN = true: everything.
 #pragma once
 
 #include "fln_nga.cuh"
@@ -20,6 +36,8 @@ struct NgaGeom {
   int rep;      // backward: partial rows a CTA leaves per slot
   int64_t grid;
   size_t smem;
+  int csm;      // backward: coefficients in shared memory
+  int64_t chunk, per_group;  // forward: rows per CTA, CTAs per group
 };
 
 // ----------------------------------------------------------------------------------------
@@ -104,36 +122,40 @@ __device__ __forceinline__ void row_sum2(RowGroup& g, float& a, float& b) {
 // Mean and reciprocal deviation of the row held in v (zeros behind it).  LayerNorm: the spread is
 // taken about the mean of the warp, and the warps' spreads are joined with that of their means
 // about the row's, so one barrier is enough and nothing cancels.
-template <int K, int VEC>
-__device__ __forceinline__ void row_stats(RowGroup& g, int kind, const float (&v)[K][VEC], const bool (&ok)[K], float inv_n,
+template <int K, int V2, bool GEN>
+__device__ __forceinline__ void row_stats(RowGroup& g, int kind, const float2 (&v)[K][V2], const bool (&ok)[K], float inv_n,
                                           float eps, float& mean, float& rstd) {
   float q = 0.f;
   mean = 0.f;
-  if (kind == FLN_RMSNORM) {
+  if (!GEN || kind == FLN_RMSNORM) {
+    float2 t = f2(0.f);
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) q = fmaf(v[k][e], v[k][e], q);
+      for (int e = 0; e < V2; ++e) t = f2fma(v[k][e], v[k][e], t);
+    q = t.x + t.y;
     row_sum1(g, q);
   } else {
-    float s[1] = {0.f};
+    float2 t = f2(0.f);
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) s[0] += v[k][e];
+      for (int e = 0; e < V2; ++e) t = f2add(v[k][e], t);
+    float s[1] = {t.x + t.y};
     warp_sum<1>(s, g.width);
     const float m = s[0] / fmaxf(g.mine, 1.f);
-    float d2[1] = {0.f};
+    t = f2(0.f);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (ok[k]) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float d = v[k][e] - m;
-          d2[0] = fmaf(d, d, d2[0]);
+        for (int e = 0; e < V2; ++e) {
+          const float2 d = f2add(v[k][e], f2(-m));
+          t = f2fma(d, d, t);
         }
       }
     }
+    float d2[1] = {t.x + t.y};
     warp_sum<1>(d2, g.width);
     mean = m;
     q = d2[0];
@@ -151,131 +173,7 @@ __device__ __forceinline__ void row_stats(RowGroup& g, int kind, const float (&v
   rstd = rsqrtf(fmaf(q, inv_n, eps));
 }
 
-template <typename T, int VEC>
-__device__ __forceinline__ void param_vec(const T* p, int c, float (&f)[VEC]) {
-  unpack<T, VEC>(ld_param<T, VEC>(p + c), f);
-}
-
-// ----------------------------------------------------------------------------------------
-// forward: R rows per CTA, one pass.  GATE 0: none, 1: shared by rows, 2: an element each.
-// ----------------------------------------------------------------------------------------
-template <typename T, int K, int GATE>
-__global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 16 ? 1024 : 512) nga_fwd_rows_kernel(const NgaParams p, const NgaGeom g) {
-  constexpr bool EXACT = sizeof(T) == 4;
-  constexpr int VEC = 16 / (int)sizeof(T);
-  __shared__ float2 red[2 * 32];
-  RowGroup rg = row_group(g, K, VEC, red);
-  const int r_in = threadIdx.x / g.tpr, lane = threadIdx.x - r_in * g.tpr;
-  const int64_t row = (int64_t)blockIdx.x * g.R + r_in;
-  const bool live = row < p.rows;
-  const int64_t base = row * (int64_t)p.cols;
-  const float inv_n = 1.0f / (float)p.cols;
-  bool ok[K];
-  int col[K];
-  Pack<T, VEC> px[K], pr[K], pg[GATE == 2 ? K : 1];
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int v = lane + k * g.tpr;
-    ok[k] = live && v < g.nv;
-    col[k] = v * VEC;
-    if (ok[k]) {
-      px[k] = ld_stream<T, VEC>(reinterpret_cast<const T*>(p.x) + base + col[k]);
-      if (p.res != nullptr) pr[k] = ld_stream<T, VEC>(reinterpret_cast<const T*>(p.res) + base + col[k]);
-      if (GATE == 2) pg[k] = ld_stream<T, VEC>(reinterpret_cast<const T*>(p.gate) + base + col[k]);
-    }
-  }
-  // (p.group_rows is the row count where nothing is held per group, so this is then 0)
-  const int64_t goff =
-      p.group_rows < p.rows && live ? (int64_t)((uint32_t)row / (uint32_t)p.group_rows) * p.cols : 0;
-  float s[K][VEC];
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) s[k][e] = 0.f;
-    if (ok[k]) unpack<T, VEC>(px[k], s[k]);
-  }
-  float mean1 = 0.f, rstd1 = 1.f;
-  if (p.post_kind != FLN_NO_NORM) row_stats<K, VEC>(rg, p.post_kind, s, ok, inv_n, p.eps1, mean1, rstd1);
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    if (ok[k]) {
-      float f[VEC];
-      if (p.post_kind != FLN_NO_NORM) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) s[k][e] = (s[k][e] - mean1) * rstd1;
-        if (p.w1 != nullptr) {
-          param_vec<T, VEC>(reinterpret_cast<const T*>(p.w1), col[k], f);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) s[k][e] *= p.woff + f[e];
-        }
-        if (p.b1 != nullptr) {
-          param_vec<T, VEC>(reinterpret_cast<const T*>(p.b1), col[k], f);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) s[k][e] += f[e];
-        }
-      }
-      if (GATE == 1) param_vec<T, VEC>(reinterpret_cast<const T*>(p.gate) + (p.gate_mode == FLN_GATE_GROUP ? goff : 0), col[k], f);
-      if (GATE == 2) unpack<T, VEC>(pg[k], f);
-      if (GATE != 0) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) s[k][e] *= gate_act<EXACT>(f[e], p.act);
-      }
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) s[k][e] *= p.ba;
-      if (p.res != nullptr) {
-        unpack<T, VEC>(pr[k], f);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) s[k][e] = fmaf(p.ra, f[e], s[k][e]);
-      }
-      Pack<T, VEC> o;
-      pack<T, VEC>(s[k], o);
-      st_stream<T, VEC>(reinterpret_cast<T*>(p.sum) + base + col[k], o);
-    }
-  }
-  float mean2 = 0.f, rstd2 = 1.f;
-  if (p.kind != FLN_NO_NORM) {
-    row_stats<K, VEC>(rg, p.kind, s, ok, inv_n, p.eps2, mean2, rstd2);
-    const int64_t aoff = p.affine_grouped ? goff : 0;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      if (ok[k]) {
-        float f[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) s[k][e] = (s[k][e] - mean2) * rstd2;
-        if (p.w2 != nullptr) {
-          param_vec<T, VEC>(reinterpret_cast<const T*>(p.w2) + aoff, col[k], f);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) s[k][e] *= p.woff + f[e];
-        }
-        if (p.b2 != nullptr) {
-          param_vec<T, VEC>(reinterpret_cast<const T*>(p.b2) + aoff, col[k], f);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) s[k][e] += f[e];
-        }
-        Pack<T, VEC> o;
-        pack<T, VEC>(s[k], o);
-        st_stream<T, VEC>(reinterpret_cast<T*>(p.y) + base + col[k], o);
-      }
-    }
-  }
-  if (live && lane == 0) {
-    if (p.mean1 != nullptr && p.post_kind == FLN_LAYERNORM) p.mean1[row] = mean1;
-    if (p.rstd1 != nullptr && p.post_kind != FLN_NO_NORM) p.rstd1[row] = rstd1;
-    if (p.mean2 != nullptr && p.kind == FLN_LAYERNORM) p.mean2[row] = mean2;
-    if (p.rstd2 != nullptr && p.kind != FLN_NO_NORM) p.rstd2[row] = rstd2;
-  }
-}
-
-// ----------------------------------------------------------------------------------------
-// backward: persistent CTAs; CTA b takes slots b, b + grid, ...  Every thread keeps its own
-// vectors of the next rows on their way into its own places in shared memory (cp.async), so
-// staging needs no barrier and no flag; the barriers are those of the two row sums.  The column
-// sums stay in registers over a slot.
-//
-// shared memory: the exchange buffers, the parameters of the current group (w1, b1, w2 as they
-// are, act(gate) in 32 bits), then `stages` times the staged tensors; everything as
-// [vector k][thread], each thread touching its own 16 bytes.
-// ----------------------------------------------------------------------------------------
+// vectors between global memory, a thread's own places in shared memory, and register pairs
 __device__ __forceinline__ void cp_async16(void* smem, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(smem)), "l"(src)
                : "memory");
@@ -286,27 +184,250 @@ __device__ __forceinline__ void cp_async_wait_behind(int ahead) {  // at most `a
   else if (ahead == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
   else asm volatile("cp.async.wait_group 3;" ::: "memory");
 }
+template <typename T>
+__device__ __forceinline__ void take(const unsigned char* p, float2 (&f)[8 / sizeof(T)]) {
+  Pack<T, 16 / sizeof(T)> v;
+  *reinterpret_cast<uint4*>(&v) = *reinterpret_cast<const uint4*>(p);
+  unpack2<T, 16 / sizeof(T)>(v, f);
+}
+template <typename T>
+__device__ __forceinline__ void give(T* p, const float2 (&f)[8 / sizeof(T)]) {
+  Pack<T, 16 / sizeof(T)> v;
+  pack2<T, 16 / sizeof(T)>(f, v);
+  st_stream<T, 16 / sizeof(T)>(p, v);
+}
+template <typename T>
+__device__ __forceinline__ void param2(const void* p, int64_t at, float2 (&f)[8 / sizeof(T)]) {
+  unpack2<T, 16 / sizeof(T)>(ld_param<T, 16 / sizeof(T)>(reinterpret_cast<const T*>(p) + at), f);
+}
 
+// C1 and B1 of a vector of columns; `goff` is where the group's gate vector starts
+template <typename T, int GATE>
+__device__ __forceinline__ void coef1(const NgaParams& p, int col, int64_t goff, float2 (&c)[8 / sizeof(T)],
+                                      float2 (&b)[8 / sizeof(T)]) {
+  constexpr int V2 = 8 / (int)sizeof(T);
+#pragma unroll
+  for (int e = 0; e < V2; ++e) {
+    c[e] = f2(1.f);
+    b[e] = f2(0.f);
+  }
+  if (p.w1 != nullptr) {
+    param2<T>(p.w1, col, c);
+#pragma unroll
+    for (int e = 0; e < V2; ++e) c[e] = f2add(c[e], f2(p.woff));
+  }
+  if (p.b1 != nullptr) param2<T>(p.b1, col, b);
+  float2 a[V2];
+#pragma unroll
+  for (int e = 0; e < V2; ++e) a[e] = f2(1.f);
+  if (GATE == 1) {
+    param2<T>(p.gate, goff + col, a);
+#pragma unroll
+    for (int e = 0; e < V2; ++e)
+      a[e] = make_float2(gate_act<sizeof(T) == 4>(a[e].x, p.act), gate_act<sizeof(T) == 4>(a[e].y, p.act));
+  }
+#pragma unroll
+  for (int e = 0; e < V2; ++e) {
+    a[e] = f2mul(a[e], f2(p.ba));
+    c[e] = f2mul(c[e], a[e]);
+    b[e] = f2mul(b[e], a[e]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void coef2(const NgaParams& p, int64_t at, float2 (&c)[8 / sizeof(T)], float2 (&b)[8 / sizeof(T)]) {
+  constexpr int V2 = 8 / (int)sizeof(T);
+#pragma unroll
+  for (int e = 0; e < V2; ++e) {
+    c[e] = f2(1.f);
+    b[e] = f2(0.f);
+  }
+  if (p.w2 != nullptr) {
+    param2<T>(p.w2, at, c);
+#pragma unroll
+    for (int e = 0; e < V2; ++e) c[e] = f2add(c[e], f2(p.woff));
+  }
+  if (p.b2 != nullptr) param2<T>(p.b2, at, b);
+}
+
+// ----------------------------------------------------------------------------------------
+// forward: a CTA takes `chunk` consecutive rows of a group, R at a time.  Every thread keeps its
+// own vectors of the next rows on their way into its own places in shared memory (cp.async), so
+// staging needs no barrier and no flag; the barriers are those of the row sums.  A CTA is short
+// (a few rows), so that the hardware hands the chunks out and SMs with less bandwidth get fewer.
+// GATE 0: none, 1: shared by rows, 2: an element each.  HOLD: the coefficients stay in registers
+// over the chunk, else they are made again for every row (rows too long for that).
+// ----------------------------------------------------------------------------------------
+template <typename T, int K, int GATE, bool GEN, bool HOLD>
+__global__ void __launch_bounds__(512) nga_fwd_rows_kernel(const NgaParams p, const NgaGeom g) {
+  constexpr bool EXACT = sizeof(T) == 4;
+  constexpr int VEC = 16 / (int)sizeof(T), V2 = VEC / 2;
+  extern __shared__ __align__(128) unsigned char smem[];
+  RowGroup rg = row_group(g, K, VEC, reinterpret_cast<float2*>(smem));
+  const int tid = threadIdx.x;
+  const int r_in = tid / g.tpr, lane = tid - r_in * g.tpr;
+  const float inv_n = 1.0f / (float)p.cols;
+  const uint32_t unit = (uint32_t)K * g.threads * 16u;
+  unsigned char* stages = smem + 512 + tid * 16;
+  const int has_res = p.res != nullptr ? 1 : 0;
+  const uint32_t stage_bytes = (uint32_t)(1 + has_res + (GATE == 2 ? 1 : 0)) * unit;
+  const uint32_t gate_off = (uint32_t)(1 + has_res) * unit;
+  const int64_t group = blockIdx.x / g.per_group;
+  const int64_t first = group * p.group_rows + (blockIdx.x - group * g.per_group) * g.chunk;
+  int64_t last = (group + 1) * p.group_rows;
+  if (first + g.chunk < last) last = first + g.chunk;
+  const int64_t goff = p.gate_mode == FLN_GATE_GROUP ? group * p.cols : 0;
+  const int64_t aoff = p.affine_grouped ? group * p.cols : 0;
+  bool vok[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) vok[k] = lane + k * g.tpr < g.nv;
+  const int col0 = lane * VEC, colk = g.tpr * VEC;
+
+  int64_t ahead = first + r_in;
+  int in_stage = 0;
+  auto fetch = [&]() {
+    if (ahead < last) {
+      const int64_t o = ahead * (int64_t)p.cols + col0;
+      unsigned char* st = stages + (uint32_t)in_stage * stage_bytes;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        if (vok[k]) {
+          unsigned char* d = st + (uint32_t)(k * g.threads) * 16u;
+          cp_async16(d, reinterpret_cast<const T*>(p.x) + o + k * colk);
+          if (has_res) cp_async16(d + unit, reinterpret_cast<const T*>(p.res) + o + k * colk);
+          if (GATE == 2) cp_async16(d + gate_off, reinterpret_cast<const T*>(p.gate) + o + k * colk);
+        }
+      }
+      ahead += g.R;
+    }
+    cp_async_commit();
+    in_stage = in_stage + 1 == g.stages ? 0 : in_stage + 1;
+  };
+  for (int i = 0; i + 1 < g.stages; ++i) fetch();
+
+  float2 c1[HOLD ? K : 1][V2], b1[HOLD && GEN ? K : 1][V2], c2[HOLD ? K : 1][V2], b2[HOLD && GEN ? K : 1][V2];
+  if (HOLD) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (vok[k]) {
+        coef1<T, GATE>(p, col0 + k * colk, goff, c1[HOLD ? k : 0], b1[HOLD && GEN ? k : 0]);
+        coef2<T>(p, aoff + col0 + k * colk, c2[HOLD ? k : 0], b2[HOLD && GEN ? k : 0]);
+      }
+    }
+  }
+  const float2 ra = f2(p.ra);
+  int stage = 0;
+  for (int64_t row0 = first; row0 < last; row0 += g.R) {
+    fetch();
+    const int64_t row = row0 + r_in;
+    const bool live = row < last;
+    cp_async_wait_behind(g.stages - 1);
+    const unsigned char* st = stages + (uint32_t)stage * stage_bytes;
+    stage = stage + 1 == g.stages ? 0 : stage + 1;
+    float2 s[K][V2];
+    bool ok[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      ok[k] = live && vok[k];
+#pragma unroll
+      for (int e = 0; e < V2; ++e) s[k][e] = f2(0.f);
+      if (ok[k]) take<T>(st + (uint32_t)(k * g.threads) * 16u, s[k]);
+    }
+    float mean1 = 0.f, rstd1 = 1.f;
+    if (p.post_kind != FLN_NO_NORM) row_stats<K, V2, GEN>(rg, p.post_kind, s, ok, inv_n, p.eps1, mean1, rstd1);
+    T* sum = reinterpret_cast<T*>(p.sum) + row * (int64_t)p.cols + col0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (ok[k]) {
+        const unsigned char* d = st + (uint32_t)(k * g.threads) * 16u;
+        float2 tc[V2], tb[V2];
+        if (!HOLD) coef1<T, GATE>(p, col0 + k * colk, goff, tc, tb);
+#pragma unroll
+        for (int e = 0; e < V2; ++e) {
+          // (x - mean) * rstd: without a norm mean is 0 and rstd 1, and x passes as it is
+          if (GEN) s[k][e] = f2add(s[k][e], f2(-mean1));
+          s[k][e] = f2mul(s[k][e], f2(rstd1));
+          const float2 c = HOLD ? c1[HOLD ? k : 0][e] : tc[e];
+          const float2 b = HOLD ? b1[HOLD && GEN ? k : 0][e] : tb[e];
+          s[k][e] = GEN ? f2fma(s[k][e], c, b) : f2mul(s[k][e], c);
+        }
+        if (GATE == 2) {
+          float2 a[V2];
+          take<T>(d + gate_off, a);
+#pragma unroll
+          for (int e = 0; e < V2; ++e)
+            s[k][e] = f2mul(s[k][e], make_float2(gate_act<EXACT>(a[e].x, p.act), gate_act<EXACT>(a[e].y, p.act)));
+        }
+        if (has_res) {
+          float2 r[V2];
+          take<T>(d + unit, r);
+#pragma unroll
+          for (int e = 0; e < V2; ++e) s[k][e] = f2fma(r[e], ra, s[k][e]);
+        }
+        give<T>(sum + k * colk, s[k]);
+      }
+    }
+    float mean2 = 0.f, rstd2 = 1.f;
+    if (p.kind != FLN_NO_NORM) {
+      row_stats<K, V2, GEN>(rg, p.kind, s, ok, inv_n, p.eps2, mean2, rstd2);
+      T* y = reinterpret_cast<T*>(p.y) + row * (int64_t)p.cols + col0;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        if (ok[k]) {
+          float2 tc[V2], tb[V2];
+          if (!HOLD) coef2<T>(p, aoff + col0 + k * colk, tc, tb);
+#pragma unroll
+          for (int e = 0; e < V2; ++e) {
+            if (GEN) s[k][e] = f2add(s[k][e], f2(-mean2));
+            s[k][e] = f2mul(s[k][e], f2(rstd2));
+            const float2 c = HOLD ? c2[HOLD ? k : 0][e] : tc[e];
+            const float2 b = HOLD ? b2[HOLD && GEN ? k : 0][e] : tb[e];
+            s[k][e] = GEN ? f2fma(s[k][e], c, b) : f2mul(s[k][e], c);
+          }
+          give<T>(y + k * colk, s[k]);
+        }
+      }
+    }
+    if (live && lane == 0) {
+      if (p.mean1 != nullptr && p.post_kind == FLN_LAYERNORM) p.mean1[row] = mean1;
+      if (p.rstd1 != nullptr && p.post_kind != FLN_NO_NORM) p.rstd1[row] = rstd1;
+      if (p.mean2 != nullptr && p.kind == FLN_LAYERNORM) p.mean2[row] = mean2;
+      if (p.rstd2 != nullptr && p.kind != FLN_NO_NORM) p.rstd2[row] = rstd2;
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------------------
+// backward: persistent CTAs; CTA b takes slots b, b + grid, ...  Rows are staged as in the forward,
+// the column sums stay in registers over a slot.  CSM: the coefficients lie in shared memory, in 32
+// bits, each thread's own; else (no room) they are made again where they are used.
+// ----------------------------------------------------------------------------------------
 constexpr int kNgaBwdHeader = 512;
 
-// where a thread's pieces lie: in units of K * threads * 16 bytes behind the header
+// where a thread's pieces lie, in units of K * threads * 16 bytes behind the header; a coefficient
+// takes 4 / es units
 struct NgaBwdLayout {
-  int w1, b1, w2, a;           // parameters, -1: absent (a takes sizeof(float) / sizeof(T) units)
-  int x, res, dy, ds, gate;    // tensors inside a stage
-  int params, tensors;         // units
+  int c1, b1, c2;            // -1: absent
+  int x, res, dy, ds, gate;  // tensors inside a stage
+  int coefs, tensors;        // units
 };
-inline __host__ __device__ NgaBwdLayout nga_bwd_layout(const NgaParams& p, int es) {
+inline __host__ __device__ NgaBwdLayout nga_bwd_layout(const NgaParams& p, int es, bool csm) {
   NgaBwdLayout l;
   int n = 0;
-  l.w1 = p.w1 != nullptr ? n++ : -1;
-  l.b1 = p.b1 != nullptr ? n++ : -1;
-  l.w2 = p.w2 != nullptr && p.dy != nullptr ? n++ : -1;
-  l.a = -1;
-  if (p.gate_mode == FLN_GATE_VECTOR || p.gate_mode == FLN_GATE_GROUP) {
-    l.a = n;
-    n += 4 / es;
+  const int u = 4 / es;
+  l.c1 = l.b1 = l.c2 = -1;
+  if (csm) {
+    l.c1 = n;
+    n += u;
+    if (p.b1 != nullptr) {
+      l.b1 = n;
+      n += u;
+    }
+    if (p.w2 != nullptr && p.dy != nullptr) {
+      l.c2 = n;
+      n += u;
+    }
   }
-  l.params = n;
+  l.coefs = n;
   n = 0;
   l.x = n++;
   l.res = p.res != nullptr && p.dy != nullptr ? n++ : -1;
@@ -317,30 +438,26 @@ inline __host__ __device__ NgaBwdLayout nga_bwd_layout(const NgaParams& p, int e
   return l;
 }
 
-// FOUR: all four column sums are kept, else P and U only
-template <typename T, int K, int GATE, bool FOUR>
-__global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 768 : 512) nga_bwd_rows_kernel(const NgaParams p, const NgaGeom g) {
+template <typename T, int K, int GATE, bool GEN, bool CSM>
+__global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_bwd_rows_kernel(const NgaParams p, const NgaGeom g) {
   constexpr bool EXACT = sizeof(T) == 4;
-  constexpr int VEC = 16 / (int)sizeof(T);
+  constexpr int VEC = 16 / (int)sizeof(T), V2 = VEC / 2;
   extern __shared__ __align__(128) unsigned char smem[];
-  const NgaBwdLayout l = nga_bwd_layout(p, (int)sizeof(T));
+  const NgaBwdLayout l = nga_bwd_layout(p, (int)sizeof(T), CSM);
   RowGroup rg = row_group(g, K, VEC, reinterpret_cast<float2*>(smem));
   const int tid = threadIdx.x;
   const int r_in = tid / g.tpr, lane = tid - r_in * g.tpr;
   const float inv_n = 1.0f / (float)p.cols;
   const uint32_t unit = (uint32_t)K * g.threads * 16u;
-  unsigned char* par = smem + kNgaBwdHeader + tid * 16;
-  unsigned char* stages = par + (uint32_t)l.params * unit;
+  const uint32_t kstep = (uint32_t)g.threads * 16u;
+  unsigned char* coefs = smem + kNgaBwdHeader + tid * 16;
+  unsigned char* stages = coefs + (uint32_t)l.coefs * unit;
   const uint32_t stage_bytes = (uint32_t)l.tensors * unit;
+  const int col0 = lane * VEC, colk = g.tpr * VEC;
   bool vok[K];
-  int col[K];
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int v = lane + k * g.tpr;
-    vok[k] = v < g.nv;
-    col[k] = v * VEC;
-  }
-  auto at = [&](unsigned char* b, int piece, int k) { return b + (uint32_t)piece * unit + (uint32_t)(k * g.threads) * 16u; };
+  for (int k = 0; k < K; ++k) vok[k] = lane + k * g.tpr < g.nv;
+  const bool has_dy = p.dy != nullptr, has_ds = p.ds != nullptr, has_res = l.res >= 0;
 
   // the row sequence of this CTA: slot after slot, R rows at a time; one walker runs ahead
   struct Walker {
@@ -368,17 +485,17 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 768 : 512) nga_
     if (ahead.slot < p.slots) {
       const int64_t row = ahead.row + r_in;
       if (row < ahead.last) {
-        const int64_t base = row * (int64_t)p.cols;
+        const int64_t o = row * (int64_t)p.cols + col0;
         unsigned char* st = stages + (uint32_t)in_stage * stage_bytes;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           if (vok[k]) {
-            const int64_t o = base + col[k];
-            cp_async16(at(st, l.x, k), reinterpret_cast<const T*>(p.x) + o);
-            if (l.dy >= 0) cp_async16(at(st, l.dy, k), reinterpret_cast<const T*>(p.dy) + o);
-            if (l.res >= 0) cp_async16(at(st, l.res, k), reinterpret_cast<const T*>(p.res) + o);
-            if (l.ds >= 0) cp_async16(at(st, l.ds, k), reinterpret_cast<const T*>(p.ds) + o);
-            if (GATE == 2) cp_async16(at(st, l.gate, k), reinterpret_cast<const T*>(p.gate) + o);
+            unsigned char* d = st + k * kstep;
+            cp_async16(d, reinterpret_cast<const T*>(p.x) + o + k * colk);
+            if (has_res) cp_async16(d + l.res * unit, reinterpret_cast<const T*>(p.res) + o + k * colk);
+            if (has_dy) cp_async16(d + l.dy * unit, reinterpret_cast<const T*>(p.dy) + o + k * colk);
+            if (has_ds) cp_async16(d + l.ds * unit, reinterpret_cast<const T*>(p.ds) + o + k * colk);
+            if (GATE == 2) cp_async16(d + l.gate * unit, reinterpret_cast<const T*>(p.gate) + o + k * colk);
           }
         }
       }
@@ -389,276 +506,280 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 768 : 512) nga_
   };
   for (int i = 0; i + 1 < g.stages; ++i) fetch();
 
-  float acc_p[K][VEC], acc_u[K][VEC], acc_q[FOUR ? K : 1][VEC], acc_v[FOUR ? K : 1][VEC];
+  float2 acc_p[K][V2], acc_u[K][V2], acc_q[GEN ? K : 1][V2], acc_v[GEN ? K : 1][V2];
   auto clear = [&]() {
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        acc_p[k][e] = 0.f;
-        acc_u[k][e] = 0.f;
-        if (FOUR) {
-          acc_q[FOUR ? k : 0][e] = 0.f;
-          acc_v[FOUR ? k : 0][e] = 0.f;
+      for (int e = 0; e < V2; ++e) {
+        acc_p[k][e] = f2(0.f);
+        acc_u[k][e] = f2(0.f);
+        if (GEN) {
+          acc_q[GEN ? k : 0][e] = f2(0.f);
+          acc_v[GEN ? k : 0][e] = f2(0.f);
         }
       }
   };
   clear();
-  int64_t group = -1;
+  // the four scalars of a row, fetched one row ahead
+  struct Scalars {
+    float mean1, rstd1, mean2, rstd2;
+  };
+  auto scalars = [&](const Walker& w) {
+    Scalars s{0.f, 1.f, 0.f, 1.f};
+    if (w.slot < p.slots && w.row + r_in < w.last) {
+      const int64_t row = w.row + r_in;
+      if (p.post_kind != FLN_NO_NORM) s.rstd1 = __ldg(p.rstd1 + row);
+      if (GEN && p.post_kind == FLN_LAYERNORM) s.mean1 = __ldg(p.mean1 + row);
+      if (has_dy) s.rstd2 = __ldg(p.rstd2 + row);
+      if (GEN && has_dy && p.kind == FLN_LAYERNORM) s.mean2 = __ldg(p.mean2 + row);
+    }
+    return s;
+  };
+  Scalars sc_next = scalars(cur);
+  int64_t group = -1, goff = 0, aoff = 0;
   int stage = 0;
   bool opened = true;  // cur has come to a new slot
+  const float2 ra = f2(p.ra);
   while (cur.slot < p.slots) {
-    // parameters of a new group into this thread's places
-    const int64_t grp = opened ? cur.slot / p.slots_per_group : group;
-    if (grp != group) {
-      const bool first = group < 0;
-      group = grp;
+    if (opened) {
+      const int64_t grp = cur.slot / p.slots_per_group;
+      if (grp != group) {  // coefficients of a new group
+        const bool first = group < 0;
+        group = grp;
+        goff = p.gate_mode == FLN_GATE_GROUP ? grp * p.cols : 0;
+        aoff = p.affine_grouped ? grp * p.cols : 0;
+        if (CSM) {
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        if (!vok[k]) continue;
-        if (first) {
-          if (l.w1 >= 0) *reinterpret_cast<Pack<T, VEC>*>(at(par, l.w1, k)) = ld_param<T, VEC>(reinterpret_cast<const T*>(p.w1) + col[k]);
-          if (l.b1 >= 0) *reinterpret_cast<Pack<T, VEC>*>(at(par, l.b1, k)) = ld_param<T, VEC>(reinterpret_cast<const T*>(p.b1) + col[k]);
-        }
-        if (l.w2 >= 0 && (first || p.affine_grouped))
-          *reinterpret_cast<Pack<T, VEC>*>(at(par, l.w2, k)) =
-              ld_param<T, VEC>(reinterpret_cast<const T*>(p.w2) + (p.affine_grouped ? grp * p.cols : 0) + col[k]);
-        if (GATE == 1 && (first || p.gate_mode == FLN_GATE_GROUP)) {
-          float f[VEC];
-          param_vec<T, VEC>(reinterpret_cast<const T*>(p.gate) + (p.gate_mode == FLN_GATE_GROUP ? grp * p.cols : 0), col[k], f);
+          for (int k = 0; k < K; ++k) {
+            if (!vok[k]) continue;
+            float2 c[V2], b[V2];
+            auto put = [&](int piece, const float2 (&v)[V2]) {
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) f[e] = gate_act<EXACT>(f[e], p.act);
-#pragma unroll
-          for (int q = 0; q < VEC / 4; ++q)
-            *reinterpret_cast<float4*>(at(par, l.a + q, k)) = make_float4(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]);
+              for (int e = 0; e < V2; e += 2)
+                *reinterpret_cast<float4*>(coefs + (uint32_t)(piece + e / 2) * unit + k * kstep) =
+                    make_float4(v[e].x, v[e].y, v[e + 1].x, v[e + 1].y);
+            };
+            if (first || p.gate_mode == FLN_GATE_GROUP) {
+              coef1<T, GATE>(p, col0 + k * colk, goff, c, b);
+              put(l.c1, c);
+              if (l.b1 >= 0) put(l.b1, b);
+            }
+            if (l.c2 >= 0 && (first || p.affine_grouped)) {
+              coef2<T>(p, aoff + col0 + k * colk, c, b);
+              put(l.c2, c);
+            }
+          }
         }
       }
     }
     fetch();
+    const int64_t slot = cur.slot;
     const int64_t row = cur.row + r_in;
     const bool live = row < cur.last;
-    float mean1 = 0.f, rstd1 = 1.f, mean2 = 0.f, rstd2 = 1.f;
-    if (live) {
-      if (p.post_kind != FLN_NO_NORM) {
-        rstd1 = __ldg(p.rstd1 + row);
-        if (p.post_kind == FLN_LAYERNORM) mean1 = __ldg(p.mean1 + row);
-      }
-      if (l.dy >= 0) {
-        rstd2 = __ldg(p.rstd2 + row);
-        if (p.kind == FLN_LAYERNORM) mean2 = __ldg(p.mean2 + row);
-      }
-    }
+    const Scalars sc = sc_next;
+    step(cur);
+    opened = cur.slot != slot;
+    sc_next = scalars(cur);
     cp_async_wait_behind(g.stages - 1);
-    unsigned char* st = stages + (uint32_t)stage * stage_bytes;
+    const unsigned char* st = stages + (uint32_t)stage * stage_bytes;
     stage = stage + 1 == g.stages ? 0 : stage + 1;
-    const int64_t base = row * (int64_t)p.cols;
+    const int64_t base = row * (int64_t)p.cols + col0;
+    auto coef = [&](int piece, int k, float2 (&v)[V2]) {
+#pragma unroll
+      for (int e = 0; e < V2; e += 2) {
+        const float4 q = *reinterpret_cast<const float4*>(coefs + (uint32_t)(piece + e / 2) * unit + k * kstep);
+        v[e] = make_float2(q.x, q.y);
+        v[e + 1] = make_float2(q.z, q.w);
+      }
+    };
+    // C1 and (GEN) B1
+    auto first_coefs = [&](int k, float2 (&c)[V2], float2 (&b)[V2]) {
+      if (CSM) {
+        coef(l.c1, k, c);
+        if (GEN && l.b1 >= 0) {
+          coef(l.b1, k, b);
+        } else {
+#pragma unroll
+          for (int e = 0; e < V2; ++e) b[e] = f2(0.f);
+        }
+      } else {
+        coef1<T, GATE>(p, col0 + k * colk, goff, c, b);
+      }
+    };
 
-    float xh[K][VEC], sh[K][VEC], g2[K][VEC];
-    float r0 = 0.f, r1 = 0.f;
-    auto piece = [&](int which, int k, float (&f)[VEC]) {
-      unpack<T, VEC>(*reinterpret_cast<const Pack<T, VEC>*>(at(st, which, k)), f);
-    };
-    auto param = [&](int which, int k, float (&f)[VEC]) {
-      unpack<T, VEC>(*reinterpret_cast<const Pack<T, VEC>*>(at(par, which, k)), f);
-    };
-    auto shared_gate = [&](int k, float (&f)[VEC]) {
-#pragma unroll
-      for (int q = 0; q < VEC / 4; ++q) {
-        const float4 v = *reinterpret_cast<const float4*>(at(par, l.a + q, k));
-        f[4 * q] = v.x;
-        f[4 * q + 1] = v.y;
-        f[4 * q + 2] = v.z;
-        f[4 * q + 3] = v.w;
-      }
-    };
-    // N1's value from xhat
-    auto n1_of = [&](int k, float (&n)[VEC]) {
-      float f[VEC];
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) n[e] = xh[k][e];
-      if (l.w1 >= 0) {
-        param(l.w1, k, f);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) n[e] *= p.woff + f[e];
-      }
-      if (l.b1 >= 0) {
-        param(l.b1, k, f);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) n[e] += f[e];
-      }
-    };
+    float2 xh[K][V2], sh[K][V2], g2[K][V2];
+    float2 r0 = f2(0.f), r1 = f2(0.f);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const bool ok = live && vok[k];
+      const unsigned char* d = st + k * kstep;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        xh[k][e] = 0.f;
-        sh[k][e] = 0.f;
-        g2[k][e] = 0.f;
+      for (int e = 0; e < V2; ++e) {
+        xh[k][e] = f2(0.f);
+        sh[k][e] = f2(0.f);
+        g2[k][e] = f2(0.f);
       }
-      if (ok) {
-        piece(l.x, k, xh[k]);
-        if (p.post_kind != FLN_NO_NORM) {
+      if (live && vok[k]) {
+        take<T>(d, xh[k]);
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) xh[k][e] = (xh[k][e] - mean1) * rstd1;
+        for (int e = 0; e < V2; ++e) {
+          if (GEN) xh[k][e] = f2add(xh[k][e], f2(-sc.mean1));
+          xh[k][e] = f2mul(xh[k][e], f2(sc.rstd1));
         }
-        if (l.dy >= 0) {
-          float n[VEC], f[VEC];
-          n1_of(k, n);
-          if (GATE == 1) shared_gate(k, f);
+        if (has_dy) {
+          float2 c[V2], b[V2];
+          first_coefs(k, c, b);
+#pragma unroll
+          for (int e = 0; e < V2; ++e) sh[k][e] = GEN ? f2fma(xh[k][e], c[e], b[e]) : f2mul(xh[k][e], c[e]);
           if (GATE == 2) {
-            piece(l.gate, k, f);
+            take<T>(d + l.gate * unit, c);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) f[e] = gate_act<EXACT>(f[e], p.act);
+            for (int e = 0; e < V2; ++e)
+              sh[k][e] = f2mul(sh[k][e], make_float2(gate_act<EXACT>(c[e].x, p.act), gate_act<EXACT>(c[e].y, p.act)));
           }
-          if (GATE != 0) {
+          if (has_res) {
+            take<T>(d + l.res * unit, c);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) n[e] *= f[e];
+            for (int e = 0; e < V2; ++e) sh[k][e] = f2fma(c[e], ra, sh[k][e]);
           }
+          take<T>(d + l.dy * unit, g2[k]);
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) n[e] *= p.ba;
-          if (l.res >= 0) {
-            piece(l.res, k, f);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) n[e] = fmaf(p.ra, f[e], n[e]);
+          for (int e = 0; e < V2; ++e) {
+            if (GEN) sh[k][e] = f2add(sh[k][e], f2(-sc.mean2));
+            sh[k][e] = f2mul(sh[k][e], f2(sc.rstd2));
+            acc_u[k][e] = f2fma(g2[k][e], sh[k][e], acc_u[k][e]);
+            if (GEN) acc_v[GEN ? k : 0][e] = f2add(acc_v[GEN ? k : 0][e], g2[k][e]);
           }
-          piece(l.dy, k, g2[k]);
+          if (CSM ? l.c2 >= 0 : p.w2 != nullptr) {
+            if (CSM) coef(l.c2, k, c);
+            else coef2<T>(p, aoff + col0 + k * colk, c, b);
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            sh[k][e] = (n[e] - mean2) * rstd2;
-            acc_u[k][e] = fmaf(g2[k][e], sh[k][e], acc_u[k][e]);
-            if (FOUR) acc_v[FOUR ? k : 0][e] += g2[k][e];
-          }
-          if (l.w2 >= 0) {
-            param(l.w2, k, f);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) g2[k][e] *= p.woff + f[e];
+            for (int e = 0; e < V2; ++e) g2[k][e] = f2mul(g2[k][e], c[e]);
           }
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            r0 = fmaf(g2[k][e], sh[k][e], r0);
-            r1 += g2[k][e];
+          for (int e = 0; e < V2; ++e) {
+            r0 = f2fma(g2[k][e], sh[k][e], r0);
+            if (GEN) r1 = f2add(r1, g2[k][e]);
           }
         }
       }
     }
     float c1 = 0.f, c2 = 0.f;
-    if (l.dy >= 0) {
-      row_sum2(rg, r0, r1);
-      c1 = r0 * inv_n;
-      c2 = p.kind == FLN_LAYERNORM ? r1 * inv_n : 0.f;
+    if (has_dy) {
+      float a = r0.x + r0.y, b = r1.x + r1.y;
+      if (GEN) row_sum2(rg, a, b);
+      else row_sum1(rg, a);
+      c1 = a * inv_n;
+      c2 = GEN && p.kind == FLN_LAYERNORM ? b * inv_n : 0.f;
     }
-    r0 = 0.f;
-    r1 = 0.f;
+    r0 = f2(0.f);
+    r1 = f2(0.f);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (live && vok[k]) {
-        float d[VEC], f[VEC];
+        const unsigned char* st_k = st + k * kstep;
+        float2 d[V2], c[V2], b[V2];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) d[e] = 0.f;
-        if (l.ds >= 0) piece(l.ds, k, d);
-        if (l.dy >= 0) {
+        for (int e = 0; e < V2; ++e) d[e] = f2(0.f);
+        if (has_ds) take<T>(st_k + l.ds * unit, d);
+        if (has_dy) {
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) d[e] = fmaf(rstd2, fmaf(-sh[k][e], c1, g2[k][e] - c2), d[e]);
+          for (int e = 0; e < V2; ++e) {
+            const float2 q = f2fma(sh[k][e], f2(-c1), GEN ? f2add(g2[k][e], f2(-c2)) : g2[k][e]);
+            d[e] = f2fma(q, f2(sc.rstd2), d[e]);
+          }
         }
         if (p.dres != nullptr) {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) f[e] = p.ra * d[e];
-          Pack<T, VEC> o;
-          pack<T, VEC>(f, o);
-          st_stream<T, VEC>(reinterpret_cast<T*>(p.dres) + base + col[k], o);
-        }
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) d[e] *= p.ba;  // e of the formulas
-        if (GATE == 2) {
-          float gv[VEC];
-          piece(l.gate, k, gv);
-          if (p.dgate != nullptr) {
-            float n[VEC];
-            n1_of(k, n);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-              float a, da;
-              gate_act_grad<EXACT>(gv[e], p.act, &a, &da);
-              f[e] = d[e] * n[e] * da;
-              d[e] *= a;
-            }
-            Pack<T, VEC> o;
-            pack<T, VEC>(f, o);
-            st_stream<T, VEC>(reinterpret_cast<T*>(p.dgate) + base + col[k], o);
+          if (p.ra == 1.0f) {
+            give<T>(reinterpret_cast<T*>(p.dres) + base + k * colk, d);
           } else {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) d[e] *= gate_act<EXACT>(gv[e], p.act);
+            for (int e = 0; e < V2; ++e) c[e] = f2mul(d[e], ra);
+            give<T>(reinterpret_cast<T*>(p.dres) + base + k * colk, c);
+          }
+        }
+        first_coefs(k, c, b);
+        if (GATE == 2) {
+          float2 gv[V2];
+          take<T>(st_k + l.gate * unit, gv);
+          if (p.dgate != nullptr) {
+            float2 o[V2];
+#pragma unroll
+            for (int e = 0; e < V2; ++e) {
+              const float2 n = GEN ? f2fma(xh[k][e], c[e], b[e]) : f2mul(xh[k][e], c[e]);
+              float2 a, da;
+              gate_act_grad<EXACT>(gv[e].x, p.act, &a.x, &da.x);
+              gate_act_grad<EXACT>(gv[e].y, p.act, &a.y, &da.y);
+              o[e] = f2mul(f2mul(d[e], n), da);
+              d[e] = f2mul(d[e], a);
+            }
+            give<T>(reinterpret_cast<T*>(p.dgate) + base + k * colk, o);
+          } else {
+#pragma unroll
+            for (int e = 0; e < V2; ++e)
+              d[e] = f2mul(d[e], make_float2(gate_act<EXACT>(gv[e].x, p.act), gate_act<EXACT>(gv[e].y, p.act)));
           }
         }
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          acc_p[k][e] = fmaf(d[e], xh[k][e], acc_p[k][e]);
-          if (FOUR) acc_q[FOUR ? k : 0][e] += d[e];
-        }
-        if (GATE == 1) {
-          shared_gate(k, f);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) d[e] *= f[e];
-        }
-        if (l.w1 >= 0) {
-          param(l.w1, k, f);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) d[e] *= p.woff + f[e];
-        }
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          g2[k][e] = d[e];  // g1 from here on
-          r0 = fmaf(d[e], xh[k][e], r0);
-          r1 += d[e];
+        for (int e = 0; e < V2; ++e) {
+          acc_p[k][e] = f2fma(d[e], xh[k][e], acc_p[k][e]);
+          if (GEN) acc_q[GEN ? k : 0][e] = f2add(acc_q[GEN ? k : 0][e], d[e]);
+          g2[k][e] = f2mul(d[e], c[e]);  // g1 from here on
+          r0 = f2fma(g2[k][e], xh[k][e], r0);
+          if (GEN) r1 = f2add(r1, g2[k][e]);
         }
       }
     }
     if (p.dx != nullptr) {
       float d1 = 0.f, d2 = 0.f;
       if (p.post_kind != FLN_NO_NORM) {
-        row_sum2(rg, r0, r1);
-        d1 = r0 * inv_n;
-        d2 = p.post_kind == FLN_LAYERNORM ? r1 * inv_n : 0.f;
+        float a = r0.x + r0.y, b = r1.x + r1.y;
+        if (GEN) row_sum2(rg, a, b);
+        else row_sum1(rg, a);
+        d1 = a * inv_n;
+        d2 = GEN && p.post_kind == FLN_LAYERNORM ? b * inv_n : 0.f;
       }
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         if (live && vok[k]) {
           if (p.post_kind != FLN_NO_NORM) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) g2[k][e] = rstd1 * fmaf(-xh[k][e], d1, g2[k][e] - d2);
+            for (int e = 0; e < V2; ++e) {
+              const float2 q = f2fma(xh[k][e], f2(-d1), GEN ? f2add(g2[k][e], f2(-d2)) : g2[k][e]);
+              g2[k][e] = f2mul(q, f2(sc.rstd1));
+            }
           }
-          Pack<T, VEC> o;
-          pack<T, VEC>(g2[k], o);
-          st_stream<T, VEC>(reinterpret_cast<T*>(p.dx) + base + col[k], o);
+          give<T>(reinterpret_cast<T*>(p.dx) + base + k * colk, g2[k]);
         }
       }
     }
-    const int64_t slot = cur.slot;
-    step(cur);
-    opened = cur.slot != slot;
     if (opened) {
       // the slot's sums: one partial row per row group, or per warp where a warp holds several
       if (p.acc != 0) {
         const int who = g.tpr < 32 ? tid >> 5 : r_in;
         float* out = p.partials + (slot * g.rep + who) * (int64_t)p.nacc * p.cols;
-        auto leave = [&](float (&acc)[VEC], int k, int which) {
+        auto leave = [&](float2 (&acc)[V2], int k, int which, float scale) {
           if (!(p.acc & which)) return;
           for (int off = 16; off >= g.tpr; off >>= 1) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], off);
+            for (int e = 0; e < V2; ++e) {
+              acc[e].x += __shfl_xor_sync(0xffffffffu, acc[e].x, off);
+              acc[e].y += __shfl_xor_sync(0xffffffffu, acc[e].y, off);
+            }
           }
           if (!vok[k] || (g.tpr < 32 && (tid & 31) >= g.tpr)) return;
-          float* q = out + (int64_t)__popc(p.acc & (which - 1)) * p.cols + col[k];
+          float* q = out + (int64_t)__popc(p.acc & (which - 1)) * p.cols + col0 + k * colk;
 #pragma unroll
-          for (int e = 0; e < VEC; e += 4) *reinterpret_cast<float4*>(q + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
+          for (int e = 0; e < V2; e += 2)
+            *reinterpret_cast<float4*>(q + 2 * e) =
+                make_float4(acc[e].x * scale, acc[e].y * scale, acc[e + 1].x * scale, acc[e + 1].y * scale);
         };
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-          leave(acc_p[k], k, kAccP);
-          if (FOUR) leave(acc_q[FOUR ? k : 0], k, kAccQ);
-          leave(acc_u[k], k, kAccU);
-          if (FOUR) leave(acc_v[FOUR ? k : 0], k, kAccV);
+          leave(acc_p[k], k, kAccP, p.ba);
+          if (GEN) leave(acc_q[GEN ? k : 0], k, kAccQ, p.ba);
+          leave(acc_u[k], k, kAccU, 1.f);
+          if (GEN) leave(acc_v[GEN ? k : 0], k, kAccV, 1.f);
         }
       }
       clear();
@@ -675,28 +796,13 @@ int nga_bwd_rows(const NgaParams& p, const NgaGeom& g, int K, cudaStream_t st);
 inline int nga_gate_of(const NgaParams& p) {
   return p.gate_mode == FLN_GATE_NONE ? 0 : (p.gate_mode == FLN_GATE_ELEMENT ? 2 : 1);
 }
-
-template <typename T, int K>
-static int nga_fwd_rows_k(const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
-  const unsigned grid = (unsigned)g.grid;
-  switch (nga_gate_of(p)) {
-    case 0:
-      nga_fwd_rows_kernel<T, K, 0><<<grid, g.threads, 0, st>>>(p, g);
-      break;
-    case 1:
-      nga_fwd_rows_kernel<T, K, 1><<<grid, g.threads, 0, st>>>(p, g);
-      break;
-    default:
-      nga_fwd_rows_kernel<T, K, 2><<<grid, g.threads, 0, st>>>(p, g);
-      break;
-  }
-  FLN_CHECK_LAUNCH();
-  return FLN_OK;
+inline bool nga_general(const NgaParams& p) {
+  return p.post_kind == FLN_LAYERNORM || p.kind == FLN_LAYERNORM || p.b1 != nullptr || p.b2 != nullptr ||
+         (p.acc & (kAccQ | kAccV)) != 0;
 }
 
-template <typename T, int K, int GATE, bool FOUR>
-static int nga_bwd_rows_one(const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
-  auto kern = nga_bwd_rows_kernel<T, K, GATE, FOUR>;
+template <typename F>
+static int nga_launch(F kern, const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
   if (g.smem > 48 * 1024 &&
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)g.smem) != cudaSuccess) {
     cudaGetLastError();
@@ -706,34 +812,45 @@ static int nga_bwd_rows_one(const NgaParams& p, const NgaGeom& g, cudaStream_t s
   FLN_CHECK_LAUNCH();
   return FLN_OK;
 }
-template <typename T, int K>
+template <typename T, int K, int GATE>
+static int nga_fwd_rows_k(const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
+  constexpr bool HOLD = K * 16 / (int)sizeof(T) <= 16;
+  return nga_general(p) ? nga_launch(nga_fwd_rows_kernel<T, K, GATE, true, HOLD>, p, g, st)
+                        : nga_launch(nga_fwd_rows_kernel<T, K, GATE, false, HOLD>, p, g, st);
+}
+template <typename T, int K, int GATE>
 static int nga_bwd_rows_k(const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
-  const bool four = (p.acc & (kAccQ | kAccV)) != 0;
-  switch (nga_gate_of(p)) {
-    case 0:
-      return four ? nga_bwd_rows_one<T, K, 0, true>(p, g, st) : nga_bwd_rows_one<T, K, 0, false>(p, g, st);
-    case 1:
-      return four ? nga_bwd_rows_one<T, K, 1, true>(p, g, st) : nga_bwd_rows_one<T, K, 1, false>(p, g, st);
-    default:
-      return four ? nga_bwd_rows_one<T, K, 2, true>(p, g, st) : nga_bwd_rows_one<T, K, 2, false>(p, g, st);
-  }
+  if (g.csm)
+    return nga_general(p) ? nga_launch(nga_bwd_rows_kernel<T, K, GATE, true, true>, p, g, st)
+                          : nga_launch(nga_bwd_rows_kernel<T, K, GATE, false, true>, p, g, st);
+  return nga_general(p) ? nga_launch(nga_bwd_rows_kernel<T, K, GATE, true, false>, p, g, st)
+                        : nga_launch(nga_bwd_rows_kernel<T, K, GATE, false, false>, p, g, st);
 }
 
+#define FLN_NGA_GATES(F, T, K)              \
+  switch (nga_gate_of(p)) {                 \
+    case 0:                                 \
+      return F<T, K, 0>(p, g, st);          \
+    case 1:                                 \
+      return F<T, K, 1>(p, g, st);          \
+    default:                                \
+      return F<T, K, 2>(p, g, st);          \
+  }
+// vectors per thread: 8, 16 or (forward) 32 elements
 #define FLN_NGA_INSTANTIATE(T)                                                                       \
   template <>                                                                                        \
   int nga_fwd_rows<T>(const NgaParams& p, const NgaGeom& g, int K, cudaStream_t st) {                \
-    if (K == 1) return nga_fwd_rows_k<T, 1>(p, g, st);                                               \
-    if (K == 2) return nga_fwd_rows_k<T, 2>(p, g, st);                                               \
-    if (K == 4) return nga_fwd_rows_k<T, 4>(p, g, st);                                               \
+    constexpr int K8 = (int)sizeof(T) / 2;                                                           \
+    if (K == K8) FLN_NGA_GATES(nga_fwd_rows_k, T, K8)                                                \
+    if (K == 2 * K8) FLN_NGA_GATES(nga_fwd_rows_k, T, 2 * K8)                                        \
+    if (K == 4 * K8) FLN_NGA_GATES(nga_fwd_rows_k, T, 4 * K8)                                        \
     return FLN_ERR_UNSUPPORTED;                                                                      \
   }                                                                                                  \
   template <>                                                                                        \
   int nga_bwd_rows<T>(const NgaParams& p, const NgaGeom& g, int K, cudaStream_t st) {                \
-    if (K == 1) return nga_bwd_rows_k<T, 1>(p, g, st);                                               \
-    if (K == 2) return nga_bwd_rows_k<T, 2>(p, g, st);                                               \
-    if constexpr (sizeof(T) == 4) {                                                                  \
-      if (K == 4) return nga_bwd_rows_k<T, 4>(p, g, st);                                             \
-    }                                                                                                \
+    constexpr int K8 = (int)sizeof(T) / 2;                                                           \
+    if (K == K8) FLN_NGA_GATES(nga_bwd_rows_k, T, K8)                                                \
+    if (K == 2 * K8) FLN_NGA_GATES(nga_bwd_rows_k, T, 2 * K8)                                        \
     return FLN_ERR_UNSUPPORTED;                                                                      \
   }
 
