@@ -517,7 +517,7 @@ static int plan_backward(NgaParams* p, int es, NgaGeom* g) {
   for (; ctas >= 1 && !fits; --ctas) {
     const size_t per = (size_t)227 * 1024 / ctas - 1024;  // the runtime keeps 1 KB of every CTA
     for (int csm = 1; csm >= 0 && !fits; --csm) {
-      const NgaBwdLayout l = nga_bwd_layout(*p, es, csm != 0);
+      const NgaBwdLayout l = nga_bwd_layout(*p, es, csm != 0, nga_general(*p));
       const size_t fixed = kNgaBwdHeader + (size_t)l.coefs * unit, stage = (size_t)l.tensors * unit;
       if (fixed + 2 * stage > per) continue;
       int s = (int)((per - fixed) / stage);
@@ -540,7 +540,8 @@ static int plan_backward(NgaParams* p, int es, NgaGeom* g) {
   auto consider = [&](int64_t spg) {
     if (spg < 1) spg = 1;
     if (spg > slots_max) spg = slots_max;
-    const int64_t chunk = (T + spg - 1) / spg;
+    int64_t chunk = (T + spg - 1) / spg;
+    chunk = (chunk + g->R - 1) / g->R * g->R;
     const int64_t n = (T + chunk - 1) / chunk * groups;
     const int64_t cost = (n + cta - 1) / cta * ((chunk + g->R - 1) / g->R + 1);
     if (best < 0 || cost < best_cost) {
@@ -550,10 +551,11 @@ static int plan_backward(NgaParams* p, int es, NgaGeom* g) {
   };
   for (int64_t w = 1; w <= 8; ++w) consider(w * cta / groups);
   consider(1);
-  p->chunk = (T + best - 1) / best;
+  p->chunk = ((T + best - 1) / best + g->R - 1) / g->R * g->R;
   p->slots_per_group = (T + p->chunk - 1) / p->chunk;
   p->slots = p->slots_per_group * groups;
   g->grid = p->slots < cta ? p->slots : cta;
+  if (p->slots > 0x7fffffff - g->grid) return 0;
   return K;
 }
 

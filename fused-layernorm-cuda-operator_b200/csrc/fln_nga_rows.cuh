@@ -40,6 +40,11 @@ struct NgaGeom {
   int64_t chunk, per_group;  // forward: rows per CTA, CTAs per group
 };
 
+// Rows per CTA where the threads per row are known at compile time (TPR != 0: the row is whole,
+// cols == TPR * K * vector; every offset is then a constant): 48 -> 34 -> xx instructions per
+// element of the bf16 forward at 4096 columns.
+__host__ __device__ constexpr int fixed_rows(int tpr) { return tpr >= 128 ? 1 : (tpr > 32 ? 2 : 256 / tpr); }
+
 // ----------------------------------------------------------------------------------------
 // sums over the threads of a row
 // ----------------------------------------------------------------------------------------
@@ -52,14 +57,17 @@ struct RowGroup {
   float2* red; // [2 buffers][32 warps]
   int flip;
 };
+template <int TPR>
 __device__ __forceinline__ RowGroup row_group(const NgaGeom& g, int K, int vec, float2* red) {
   RowGroup r;
-  r.width = g.tpr < 32 ? g.tpr : 32;
-  r.wpr = g.tpr <= 32 ? 1 : g.tpr >> 5;
-  r.warp0 = g.tpr <= 32 ? (int)(threadIdx.x >> 5) : (int)(threadIdx.x / g.tpr) * r.wpr;
+  const int tpr = TPR ? TPR : g.tpr;
+  r.width = tpr < 32 ? tpr : 32;
+  r.wpr = tpr <= 32 ? 1 : tpr >> 5;
+  r.warp0 = tpr <= 32 ? (int)(threadIdx.x >> 5) : (int)(threadIdx.x / tpr) * r.wpr;
   r.red = red;
   r.flip = 0;
   auto count = [&](int w) {  // elements of the row in its warp w
+    if (TPR) return (float)(K * 32 * vec);
     int n = 0;
     for (int k = 0; k < K; ++k) {
       int left = g.nv - (k * g.tpr + w * 32);
@@ -184,6 +192,8 @@ __device__ __forceinline__ void cp_async_wait_behind(int ahead) {  // at most `a
   else if (ahead == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
   else asm volatile("cp.async.wait_group 3;" ::: "memory");
 }
+// v, or zeros (not v times zero, which would be NaN where v is infinite)
+__device__ __forceinline__ float2 f2only(bool on, float2 v) { return make_float2(on ? v.x : 0.f, on ? v.y : 0.f); }
 template <typename T>
 __device__ __forceinline__ void take(const unsigned char* p, float2 (&f)[8 / sizeof(T)]) {
   Pack<T, 16 / sizeof(T)> v;
@@ -257,16 +267,21 @@ __device__ __forceinline__ void coef2(const NgaParams& p, int64_t at, float2 (&c
 // GATE 0: none, 1: shared by rows, 2: an element each.  HOLD: the coefficients stay in registers
 // over the chunk, else they are made again for every row (rows too long for that).
 // ----------------------------------------------------------------------------------------
-template <typename T, int K, int GATE, bool GEN, bool HOLD>
+template <typename T, int K, int GATE, bool GEN, bool HOLD, int TPR>
 __global__ void __launch_bounds__(512) nga_fwd_rows_kernel(const NgaParams p, const NgaGeom g) {
   constexpr bool EXACT = sizeof(T) == 4;
   constexpr int VEC = 16 / (int)sizeof(T), V2 = VEC / 2;
   extern __shared__ __align__(128) unsigned char smem[];
-  RowGroup rg = row_group(g, K, VEC, reinterpret_cast<float2*>(smem));
+  constexpr bool FULL = TPR != 0;
+  const int tpr = FULL ? TPR : g.tpr;
+  const int R = FULL ? fixed_rows(TPR) : g.R;
+  const int threads = FULL ? TPR * fixed_rows(TPR) : g.threads;
+  const int cols = FULL ? TPR * K * VEC : p.cols;
+  RowGroup rg = row_group<TPR>(g, K, VEC, reinterpret_cast<float2*>(smem));
   const int tid = threadIdx.x;
-  const int r_in = tid / g.tpr, lane = tid - r_in * g.tpr;
-  const float inv_n = 1.0f / (float)p.cols;
-  const uint32_t unit = (uint32_t)K * g.threads * 16u;
+  const int r_in = tid / tpr, lane = tid - r_in * tpr;
+  const float inv_n = 1.0f / (float)cols;
+  const uint32_t unit = (uint32_t)K * threads * 16u;
   unsigned char* stages = smem + 512 + tid * 16;
   const int has_res = p.res != nullptr ? 1 : 0;
   const uint32_t stage_bytes = (uint32_t)(1 + has_res + (GATE == 2 ? 1 : 0)) * unit;
@@ -275,29 +290,33 @@ __global__ void __launch_bounds__(512) nga_fwd_rows_kernel(const NgaParams p, co
   const int64_t first = group * p.group_rows + (blockIdx.x - group * g.per_group) * g.chunk;
   int64_t last = (group + 1) * p.group_rows;
   if (first + g.chunk < last) last = first + g.chunk;
-  const int64_t goff = p.gate_mode == FLN_GATE_GROUP ? group * p.cols : 0;
-  const int64_t aoff = p.affine_grouped ? group * p.cols : 0;
+  const int64_t goff = p.gate_mode == FLN_GATE_GROUP ? group * cols : 0;
+  const int64_t aoff = p.affine_grouped ? group * cols : 0;
   bool vok[K];
 #pragma unroll
-  for (int k = 0; k < K; ++k) vok[k] = lane + k * g.tpr < g.nv;
-  const int col0 = lane * VEC, colk = g.tpr * VEC;
+  for (int k = 0; k < K; ++k) vok[k] = FULL || (K == 2 && k == 0) || lane + k * tpr < g.nv;  // (tpr <= nv where K is 2)
+  // A lane whose last vectors lie behind the row works on the row's last vector instead; what goes
+  // into the sums is set to zero there and nothing is stored, so the arithmetic has no branches.
+  int col[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) col[k] = (vok[k] ? lane + k * tpr : g.nv - 1) * VEC;
 
-  int64_t ahead = first + r_in;
+  // row groups behind the last row work on the last row once more (and write the same values), so
+  // that nothing below depends on it
+  int64_t ahead = first;
   int in_stage = 0;
   auto fetch = [&]() {
     if (ahead < last) {
-      const int64_t o = ahead * (int64_t)p.cols + col0;
+      const int64_t o = (ahead + r_in < last ? ahead + r_in : last - 1) * (int64_t)cols;
       unsigned char* st = stages + (uint32_t)in_stage * stage_bytes;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        if (vok[k]) {
-          unsigned char* d = st + (uint32_t)(k * g.threads) * 16u;
-          cp_async16(d, reinterpret_cast<const T*>(p.x) + o + k * colk);
-          if (has_res) cp_async16(d + unit, reinterpret_cast<const T*>(p.res) + o + k * colk);
-          if (GATE == 2) cp_async16(d + gate_off, reinterpret_cast<const T*>(p.gate) + o + k * colk);
-        }
+        unsigned char* d = st + (uint32_t)(k * threads) * 16u;
+        cp_async16(d, reinterpret_cast<const T*>(p.x) + o + col[k]);
+        if (has_res) cp_async16(d + unit, reinterpret_cast<const T*>(p.res) + o + col[k]);
+        if (GATE == 2) cp_async16(d + gate_off, reinterpret_cast<const T*>(p.gate) + o + col[k]);
       }
-      ahead += g.R;
+      ahead += R;
     }
     cp_async_commit();
     in_stage = in_stage + 1 == g.stages ? 0 : in_stage + 1;
@@ -308,39 +327,36 @@ __global__ void __launch_bounds__(512) nga_fwd_rows_kernel(const NgaParams p, co
   if (HOLD) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (vok[k]) {
-        coef1<T, GATE>(p, col0 + k * colk, goff, c1[HOLD ? k : 0], b1[HOLD && GEN ? k : 0]);
-        coef2<T>(p, aoff + col0 + k * colk, c2[HOLD ? k : 0], b2[HOLD && GEN ? k : 0]);
-      }
+      coef1<T, GATE>(p, col[k], goff, c1[HOLD ? k : 0], b1[HOLD && GEN ? k : 0]);
+      coef2<T>(p, aoff + col[k], c2[HOLD ? k : 0], b2[HOLD && GEN ? k : 0]);
     }
   }
   const float2 ra = f2(p.ra);
   int stage = 0;
-  for (int64_t row0 = first; row0 < last; row0 += g.R) {
+  for (int64_t row0 = first; row0 < last; row0 += R) {
     fetch();
-    const int64_t row = row0 + r_in;
-    const bool live = row < last;
+    const int64_t row = row0 + r_in < last ? row0 + r_in : last - 1;
     cp_async_wait_behind(g.stages - 1);
     const unsigned char* st = stages + (uint32_t)stage * stage_bytes;
     stage = stage + 1 == g.stages ? 0 : stage + 1;
     float2 s[K][V2];
-    bool ok[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      ok[k] = live && vok[k];
+      take<T>(st + (uint32_t)(k * threads) * 16u, s[k]);
+      if (!FULL) {
 #pragma unroll
-      for (int e = 0; e < V2; ++e) s[k][e] = f2(0.f);
-      if (ok[k]) take<T>(st + (uint32_t)(k * g.threads) * 16u, s[k]);
+        for (int e = 0; e < V2; ++e) s[k][e] = f2only(vok[k], s[k][e]);
+      }
     }
     float mean1 = 0.f, rstd1 = 1.f;
-    if (p.post_kind != FLN_NO_NORM) row_stats<K, V2, GEN>(rg, p.post_kind, s, ok, inv_n, p.eps1, mean1, rstd1);
-    T* sum = reinterpret_cast<T*>(p.sum) + row * (int64_t)p.cols + col0;
+    if (p.post_kind != FLN_NO_NORM) row_stats<K, V2, GEN>(rg, p.post_kind, s, vok, inv_n, p.eps1, mean1, rstd1);
+    T* sum = reinterpret_cast<T*>(p.sum) + row * (int64_t)cols;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (ok[k]) {
-        const unsigned char* d = st + (uint32_t)(k * g.threads) * 16u;
+      {
+        const unsigned char* d = st + (uint32_t)(k * threads) * 16u;
         float2 tc[V2], tb[V2];
-        if (!HOLD) coef1<T, GATE>(p, col0 + k * colk, goff, tc, tb);
+        if (!HOLD) coef1<T, GATE>(p, col[k], goff, tc, tb);
 #pragma unroll
         for (int e = 0; e < V2; ++e) {
           // (x - mean) * rstd: without a norm mean is 0 and rstd 1, and x passes as it is
@@ -363,18 +379,22 @@ __global__ void __launch_bounds__(512) nga_fwd_rows_kernel(const NgaParams p, co
 #pragma unroll
           for (int e = 0; e < V2; ++e) s[k][e] = f2fma(r[e], ra, s[k][e]);
         }
-        give<T>(sum + k * colk, s[k]);
+        if (vok[k]) give<T>(sum + col[k], s[k]);
+        if (!FULL) {
+#pragma unroll
+          for (int e = 0; e < V2; ++e) s[k][e] = f2only(vok[k], s[k][e]);
+        }
       }
     }
     float mean2 = 0.f, rstd2 = 1.f;
     if (p.kind != FLN_NO_NORM) {
-      row_stats<K, V2, GEN>(rg, p.kind, s, ok, inv_n, p.eps2, mean2, rstd2);
-      T* y = reinterpret_cast<T*>(p.y) + row * (int64_t)p.cols + col0;
+      row_stats<K, V2, GEN>(rg, p.kind, s, vok, inv_n, p.eps2, mean2, rstd2);
+      T* y = reinterpret_cast<T*>(p.y) + row * (int64_t)cols;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        if (ok[k]) {
+        {
           float2 tc[V2], tb[V2];
-          if (!HOLD) coef2<T>(p, aoff + col0 + k * colk, tc, tb);
+          if (!HOLD) coef2<T>(p, aoff + col[k], tc, tb);
 #pragma unroll
           for (int e = 0; e < V2; ++e) {
             if (GEN) s[k][e] = f2add(s[k][e], f2(-mean2));
@@ -383,11 +403,11 @@ __global__ void __launch_bounds__(512) nga_fwd_rows_kernel(const NgaParams p, co
             const float2 b = HOLD ? b2[HOLD && GEN ? k : 0][e] : tb[e];
             s[k][e] = GEN ? f2fma(s[k][e], c, b) : f2mul(s[k][e], c);
           }
-          give<T>(y + k * colk, s[k]);
+          if (vok[k]) give<T>(y + col[k], s[k]);
         }
       }
     }
-    if (live && lane == 0) {
+    if (lane == 0) {
       if (p.mean1 != nullptr && p.post_kind == FLN_LAYERNORM) p.mean1[row] = mean1;
       if (p.rstd1 != nullptr && p.post_kind != FLN_NO_NORM) p.rstd1[row] = rstd1;
       if (p.mean2 != nullptr && p.kind == FLN_LAYERNORM) p.mean2[row] = mean2;
@@ -400,6 +420,7 @@ __global__ void __launch_bounds__(512) nga_fwd_rows_kernel(const NgaParams p, co
 // backward: persistent CTAs; CTA b takes slots b, b + grid, ...  Rows are staged as in the forward,
 // the column sums stay in registers over a slot.  CSM: the coefficients lie in shared memory, in 32
 // bits, each thread's own; else (no room) they are made again where they are used.
+// SET: which tensors there are, 1: x, residual, dy and dsum, 2: x and dsum, 0: found out at run time.
 // ----------------------------------------------------------------------------------------
 constexpr int kNgaBwdHeader = 512;
 
@@ -410,99 +431,119 @@ struct NgaBwdLayout {
   int x, res, dy, ds, gate;  // tensors inside a stage
   int coefs, tensors;        // units
 };
-inline __host__ __device__ NgaBwdLayout nga_bwd_layout(const NgaParams& p, int es, bool csm) {
-  NgaBwdLayout l;
-  int n = 0;
+__host__ __device__ constexpr NgaBwdLayout nga_layout(int es, bool csm, bool bias, bool res, bool dy, bool ds, bool gate) {
+  NgaBwdLayout l = {-1, -1, -1, 0, -1, -1, -1, -1, 0, 0};
   const int u = 4 / es;
-  l.c1 = l.b1 = l.c2 = -1;
+  int n = 0;
   if (csm) {
     l.c1 = n;
     n += u;
-    if (p.b1 != nullptr) {
+    if (bias) {
       l.b1 = n;
       n += u;
     }
-    if (p.w2 != nullptr && p.dy != nullptr) {
+    if (dy) {
       l.c2 = n;
       n += u;
     }
   }
   l.coefs = n;
-  n = 0;
-  l.x = n++;
-  l.res = p.res != nullptr && p.dy != nullptr ? n++ : -1;
-  l.dy = p.dy != nullptr ? n++ : -1;
-  l.ds = p.ds != nullptr ? n++ : -1;
-  l.gate = p.gate_mode == FLN_GATE_ELEMENT ? n++ : -1;
+  n = 1;
+  if (res) l.res = n++;
+  if (dy) l.dy = n++;
+  if (ds) l.ds = n++;
+  if (gate) l.gate = n++;
   l.tensors = n;
   return l;
 }
+// (GEN kernels keep a place for B1 whether there is one or not)
+inline __host__ __device__ NgaBwdLayout nga_bwd_layout(const NgaParams& p, int es, bool csm, bool gen) {
+  return nga_layout(es, csm, gen, p.res != nullptr && p.dy != nullptr, p.dy != nullptr, p.ds != nullptr,
+                    p.gate_mode == FLN_GATE_ELEMENT);
+}
+inline int nga_set_of(const NgaParams& p) {
+  if (p.res != nullptr && p.dy != nullptr && p.ds != nullptr) return 1;
+  if (p.dy == nullptr && p.ds != nullptr) return 2;
+  return 0;
+}
 
-template <typename T, int K, int GATE, bool GEN, bool CSM>
+template <typename T, int K, int GATE, bool GEN, bool CSM, int TPR, int SET>
 __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_bwd_rows_kernel(const NgaParams p, const NgaGeom g) {
   constexpr bool EXACT = sizeof(T) == 4;
   constexpr int VEC = 16 / (int)sizeof(T), V2 = VEC / 2;
   extern __shared__ __align__(128) unsigned char smem[];
-  const NgaBwdLayout l = nga_bwd_layout(p, (int)sizeof(T), CSM);
-  RowGroup rg = row_group(g, K, VEC, reinterpret_cast<float2*>(smem));
+  const bool has_dy = SET == 1 || (SET == 0 && p.dy != nullptr);
+  const bool has_ds = SET != 0 || p.ds != nullptr;
+  const bool has_res = SET == 1 || (SET == 0 && has_dy && p.res != nullptr);
+  const NgaBwdLayout l = nga_layout((int)sizeof(T), CSM, GEN, has_res, has_dy, has_ds, GATE == 2);
+  constexpr bool FULL = TPR != 0;
+  const int tpr = FULL ? TPR : g.tpr;
+  const int R = FULL ? fixed_rows(TPR) : g.R;
+  const int threads = FULL ? TPR * fixed_rows(TPR) : g.threads;
+  const int cols = FULL ? TPR * K * VEC : p.cols;
+  constexpr bool ONE = FULL && fixed_rows(FULL ? TPR : 1) == 1;  // one row at a time: never behind the slot
+  RowGroup rg = row_group<TPR>(g, K, VEC, reinterpret_cast<float2*>(smem));
   const int tid = threadIdx.x;
-  const int r_in = tid / g.tpr, lane = tid - r_in * g.tpr;
-  const float inv_n = 1.0f / (float)p.cols;
-  const uint32_t unit = (uint32_t)K * g.threads * 16u;
-  const uint32_t kstep = (uint32_t)g.threads * 16u;
+  const int r_in = ONE ? 0 : tid / tpr, lane = tid - r_in * tpr;
+  const float inv_n = 1.0f / (float)cols;
+  const uint32_t unit = (uint32_t)K * threads * 16u;
+  const uint32_t kstep = (uint32_t)threads * 16u;
   unsigned char* coefs = smem + kNgaBwdHeader + tid * 16;
   unsigned char* stages = coefs + (uint32_t)l.coefs * unit;
   const uint32_t stage_bytes = (uint32_t)l.tensors * unit;
-  const int col0 = lane * VEC, colk = g.tpr * VEC;
+  const uint32_t ring_bytes = (uint32_t)g.stages * stage_bytes;
   bool vok[K];
 #pragma unroll
-  for (int k = 0; k < K; ++k) vok[k] = lane + k * g.tpr < g.nv;
-  const bool has_dy = p.dy != nullptr, has_ds = p.ds != nullptr, has_res = l.res >= 0;
+  for (int k = 0; k < K; ++k) vok[k] = FULL || (K == 2 && k == 0) || lane + k * tpr < g.nv;  // (tpr <= nv where K is 2)
+  // Lanes behind the row work on its last vector, row groups behind the slot on its last row; what
+  // goes into the sums is set to zero there and nothing is stored, so the arithmetic has no branches.
+  int col[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) col[k] = (vok[k] ? lane + k * tpr : g.nv - 1) * VEC;
 
-  // the row sequence of this CTA: slot after slot, R rows at a time; one walker runs ahead
+  // The row sequence of this CTA: slot after slot, R rows at a time; one walker runs ahead.
   struct Walker {
-    int64_t slot, row, last;
+    int slot, row, last;  // row: of the CTA's first row group
   };
+  const int nslots = (int)p.slots, grid = (int)gridDim.x;
   auto open = [&](Walker& w) {
-    if (w.slot < p.slots) {
+    if (w.slot < nslots) {
       const SlotRows sr = slot_rows(p, w.slot);
-      w.row = sr.first;
-      w.last = sr.last;
+      w.row = (int)sr.first;
+      w.last = (int)sr.last;
     }
   };
   auto step = [&](Walker& w) {
-    w.row += g.R;
+    w.row += R;
     if (w.row >= w.last) {
-      w.slot += gridDim.x;
+      w.slot += grid;
       open(w);
     }
   };
-  Walker ahead{(int64_t)blockIdx.x, 0, 0};
+  auto my_row = [&](const Walker& w) { return ONE ? w.row : (w.row + r_in < w.last ? w.row + r_in : w.last - 1); };
+  Walker ahead{(int)blockIdx.x, 0, 0};
   open(ahead);
   Walker cur = ahead;
-  int in_stage = 0;  // stage the walker fills next
+  uint32_t fill = 0;  // byte offset of the stage the walker fills next
   auto fetch = [&]() {
-    if (ahead.slot < p.slots) {
-      const int64_t row = ahead.row + r_in;
-      if (row < ahead.last) {
-        const int64_t o = row * (int64_t)p.cols + col0;
-        unsigned char* st = stages + (uint32_t)in_stage * stage_bytes;
+    if (ahead.slot < nslots) {
+      unsigned char* st = stages + fill;
+      const int64_t at = (int64_t)my_row(ahead) * cols;
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-          if (vok[k]) {
-            unsigned char* d = st + k * kstep;
-            cp_async16(d, reinterpret_cast<const T*>(p.x) + o + k * colk);
-            if (has_res) cp_async16(d + l.res * unit, reinterpret_cast<const T*>(p.res) + o + k * colk);
-            if (has_dy) cp_async16(d + l.dy * unit, reinterpret_cast<const T*>(p.dy) + o + k * colk);
-            if (has_ds) cp_async16(d + l.ds * unit, reinterpret_cast<const T*>(p.ds) + o + k * colk);
-            if (GATE == 2) cp_async16(d + l.gate * unit, reinterpret_cast<const T*>(p.gate) + o + k * colk);
-          }
-        }
+      for (int k = 0; k < K; ++k) {
+        unsigned char* d = st + k * kstep;
+        const int64_t o = at + col[k];
+        cp_async16(d, reinterpret_cast<const T*>(p.x) + o);
+        if (has_res) cp_async16(d + l.res * unit, reinterpret_cast<const T*>(p.res) + o);
+        if (has_dy) cp_async16(d + l.dy * unit, reinterpret_cast<const T*>(p.dy) + o);
+        if (has_ds) cp_async16(d + l.ds * unit, reinterpret_cast<const T*>(p.ds) + o);
+        if (GATE == 2) cp_async16(d + l.gate * unit, reinterpret_cast<const T*>(p.gate) + o);
       }
       step(ahead);
     }
     cp_async_commit();  // a group per step, also an empty one, so that the count tells the row
-    in_stage = in_stage + 1 == g.stages ? 0 : in_stage + 1;
+    fill += stage_bytes;
+    if (fill == ring_bytes) fill = 0;
   };
   for (int i = 0; i + 1 < g.stages; ++i) fetch();
 
@@ -527,8 +568,8 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
   };
   auto scalars = [&](const Walker& w) {
     Scalars s{0.f, 1.f, 0.f, 1.f};
-    if (w.slot < p.slots && w.row + r_in < w.last) {
-      const int64_t row = w.row + r_in;
+    if (w.slot < nslots) {
+      const int row = my_row(w);
       if (p.post_kind != FLN_NO_NORM) s.rstd1 = __ldg(p.rstd1 + row);
       if (GEN && p.post_kind == FLN_LAYERNORM) s.mean1 = __ldg(p.mean1 + row);
       if (has_dy) s.rstd2 = __ldg(p.rstd2 + row);
@@ -538,21 +579,37 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
   };
   Scalars sc_next = scalars(cur);
   int64_t group = -1, goff = 0, aoff = 0;
-  int stage = 0;
+  uint32_t drain = 0;  // byte offset of the stage in hand
   bool opened = true;  // cur has come to a new slot
   const float2 ra = f2(p.ra);
-  while (cur.slot < p.slots) {
+  auto coef = [&](int piece, int k, float2 (&v)[V2]) {
+#pragma unroll
+    for (int e = 0; e < V2; e += 2) {
+      const float4 q = *reinterpret_cast<const float4*>(coefs + (uint32_t)(piece + e / 2) * unit + k * kstep);
+      v[e] = make_float2(q.x, q.y);
+      v[e + 1] = make_float2(q.z, q.w);
+    }
+  };
+  // C1 and (GEN) B1
+  auto first_coefs = [&](int k, float2 (&c)[V2], float2 (&b)[V2]) {
+    if (CSM) {
+      coef(l.c1, k, c);
+      if (GEN) coef(l.b1, k, b);
+    } else {
+      coef1<T, GATE>(p, col[k], goff, c, b);
+    }
+  };
+  while (cur.slot < nslots) {
     if (opened) {
       const int64_t grp = cur.slot / p.slots_per_group;
       if (grp != group) {  // coefficients of a new group
         const bool first = group < 0;
         group = grp;
-        goff = p.gate_mode == FLN_GATE_GROUP ? grp * p.cols : 0;
-        aoff = p.affine_grouped ? grp * p.cols : 0;
+        goff = p.gate_mode == FLN_GATE_GROUP ? grp * cols : 0;
+        aoff = p.affine_grouped ? grp * cols : 0;
         if (CSM) {
 #pragma unroll
           for (int k = 0; k < K; ++k) {
-            if (!vok[k]) continue;
             float2 c[V2], b[V2];
             auto put = [&](int piece, const float2 (&v)[V2]) {
 #pragma unroll
@@ -561,12 +618,12 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
                     make_float4(v[e].x, v[e].y, v[e + 1].x, v[e + 1].y);
             };
             if (first || p.gate_mode == FLN_GATE_GROUP) {
-              coef1<T, GATE>(p, col0 + k * colk, goff, c, b);
+              coef1<T, GATE>(p, col[k], goff, c, b);
               put(l.c1, c);
-              if (l.b1 >= 0) put(l.b1, b);
+              if (GEN) put(l.b1, b);
             }
-            if (l.c2 >= 0 && (first || p.affine_grouped)) {
-              coef2<T>(p, aoff + col0 + k * colk, c, b);
+            if (has_dy && (first || p.affine_grouped)) {
+              coef2<T>(p, aoff + col[k], c, b);
               put(l.c2, c);
             }
           }
@@ -574,52 +631,24 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
       }
     }
     fetch();
-    const int64_t slot = cur.slot;
-    const int64_t row = cur.row + r_in;
-    const bool live = row < cur.last;
+    const int slot = cur.slot;
+    const bool live = ONE || cur.row + r_in < cur.last;
+    const int64_t base = (int64_t)my_row(cur) * cols;
     const Scalars sc = sc_next;
     step(cur);
     opened = cur.slot != slot;
     sc_next = scalars(cur);
     cp_async_wait_behind(g.stages - 1);
-    const unsigned char* st = stages + (uint32_t)stage * stage_bytes;
-    stage = stage + 1 == g.stages ? 0 : stage + 1;
-    const int64_t base = row * (int64_t)p.cols + col0;
-    auto coef = [&](int piece, int k, float2 (&v)[V2]) {
-#pragma unroll
-      for (int e = 0; e < V2; e += 2) {
-        const float4 q = *reinterpret_cast<const float4*>(coefs + (uint32_t)(piece + e / 2) * unit + k * kstep);
-        v[e] = make_float2(q.x, q.y);
-        v[e + 1] = make_float2(q.z, q.w);
-      }
-    };
-    // C1 and (GEN) B1
-    auto first_coefs = [&](int k, float2 (&c)[V2], float2 (&b)[V2]) {
-      if (CSM) {
-        coef(l.c1, k, c);
-        if (GEN && l.b1 >= 0) {
-          coef(l.b1, k, b);
-        } else {
-#pragma unroll
-          for (int e = 0; e < V2; ++e) b[e] = f2(0.f);
-        }
-      } else {
-        coef1<T, GATE>(p, col0 + k * colk, goff, c, b);
-      }
-    };
+    const unsigned char* st = stages + drain;
+    drain += stage_bytes;
+    if (drain == ring_bytes) drain = 0;
 
     float2 xh[K][V2], sh[K][V2], g2[K][V2];
     float2 r0 = f2(0.f), r1 = f2(0.f);
+    {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const unsigned char* d = st + k * kstep;
-#pragma unroll
-      for (int e = 0; e < V2; ++e) {
-        xh[k][e] = f2(0.f);
-        sh[k][e] = f2(0.f);
-        g2[k][e] = f2(0.f);
-      }
-      if (live && vok[k]) {
+      for (int k = 0; k < K; ++k) {
+        const unsigned char* d = st + k * kstep;
         take<T>(d, xh[k]);
 #pragma unroll
         for (int e = 0; e < V2; ++e) {
@@ -643,21 +672,19 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
             for (int e = 0; e < V2; ++e) sh[k][e] = f2fma(c[e], ra, sh[k][e]);
           }
           take<T>(d + l.dy * unit, g2[k]);
+          if (!(FULL && ONE)) {
+#pragma unroll
+            for (int e = 0; e < V2; ++e) g2[k][e] = f2only(live && vok[k], g2[k][e]);
+          }
+          if (CSM) coef(l.c2, k, c);
+          else coef2<T>(p, aoff + col[k], c, b);
 #pragma unroll
           for (int e = 0; e < V2; ++e) {
             if (GEN) sh[k][e] = f2add(sh[k][e], f2(-sc.mean2));
             sh[k][e] = f2mul(sh[k][e], f2(sc.rstd2));
             acc_u[k][e] = f2fma(g2[k][e], sh[k][e], acc_u[k][e]);
             if (GEN) acc_v[GEN ? k : 0][e] = f2add(acc_v[GEN ? k : 0][e], g2[k][e]);
-          }
-          if (CSM ? l.c2 >= 0 : p.w2 != nullptr) {
-            if (CSM) coef(l.c2, k, c);
-            else coef2<T>(p, aoff + col0 + k * colk, c, b);
-#pragma unroll
-            for (int e = 0; e < V2; ++e) g2[k][e] = f2mul(g2[k][e], c[e]);
-          }
-#pragma unroll
-          for (int e = 0; e < V2; ++e) {
+            g2[k][e] = f2mul(g2[k][e], c[e]);
             r0 = f2fma(g2[k][e], sh[k][e], r0);
             if (GEN) r1 = f2add(r1, g2[k][e]);
           }
@@ -674,14 +701,20 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
     }
     r0 = f2(0.f);
     r1 = f2(0.f);
+    {
+      T* dres = reinterpret_cast<T*>(p.dres) + base;
+      T* dgate = reinterpret_cast<T*>(p.dgate) + base;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      if (live && vok[k]) {
+      for (int k = 0; k < K; ++k) {
+        const bool ok = live && vok[k];
         const unsigned char* st_k = st + k * kstep;
         float2 d[V2], c[V2], b[V2];
+        if (has_ds) {
+          take<T>(st_k + l.ds * unit, d);
+        } else {
 #pragma unroll
-        for (int e = 0; e < V2; ++e) d[e] = f2(0.f);
-        if (has_ds) take<T>(st_k + l.ds * unit, d);
+          for (int e = 0; e < V2; ++e) d[e] = f2(0.f);
+        }
         if (has_dy) {
 #pragma unroll
           for (int e = 0; e < V2; ++e) {
@@ -689,14 +722,14 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
             d[e] = f2fma(q, f2(sc.rstd2), d[e]);
           }
         }
-        if (p.dres != nullptr) {
-          if (p.ra == 1.0f) {
-            give<T>(reinterpret_cast<T*>(p.dres) + base + k * colk, d);
-          } else {
+        if (!(FULL && ONE)) {
 #pragma unroll
-            for (int e = 0; e < V2; ++e) c[e] = f2mul(d[e], ra);
-            give<T>(reinterpret_cast<T*>(p.dres) + base + k * colk, c);
-          }
+          for (int e = 0; e < V2; ++e) d[e] = f2only(ok, d[e]);
+        }
+        if (p.dres != nullptr) {
+#pragma unroll
+          for (int e = 0; e < V2; ++e) c[e] = f2mul(d[e], ra);
+          if (ok) give<T>(dres + col[k], c);
         }
         first_coefs(k, c, b);
         if (GATE == 2) {
@@ -713,7 +746,7 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
               o[e] = f2mul(f2mul(d[e], n), da);
               d[e] = f2mul(d[e], a);
             }
-            give<T>(reinterpret_cast<T*>(p.dgate) + base + k * colk, o);
+            if (ok) give<T>(dgate + col[k], o);
           } else {
 #pragma unroll
             for (int e = 0; e < V2; ++e)
@@ -739,9 +772,10 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
         d1 = a * inv_n;
         d2 = GEN && p.post_kind == FLN_LAYERNORM ? b * inv_n : 0.f;
       }
+      {
+        T* dx = reinterpret_cast<T*>(p.dx) + base;
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        if (live && vok[k]) {
+        for (int k = 0; k < K; ++k) {
           if (p.post_kind != FLN_NO_NORM) {
 #pragma unroll
             for (int e = 0; e < V2; ++e) {
@@ -749,26 +783,26 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
               g2[k][e] = f2mul(q, f2(sc.rstd1));
             }
           }
-          give<T>(reinterpret_cast<T*>(p.dx) + base + k * colk, g2[k]);
+          if (live && vok[k]) give<T>(dx + col[k], g2[k]);
         }
       }
     }
     if (opened) {
       // the slot's sums: one partial row per row group, or per warp where a warp holds several
       if (p.acc != 0) {
-        const int who = g.tpr < 32 ? tid >> 5 : r_in;
-        float* out = p.partials + (slot * g.rep + who) * (int64_t)p.nacc * p.cols;
+        const int who = tpr < 32 ? tid >> 5 : r_in;
+        float* out = p.partials + ((int64_t)slot * g.rep + who) * (int64_t)p.nacc * cols;
         auto leave = [&](float2 (&acc)[V2], int k, int which, float scale) {
           if (!(p.acc & which)) return;
-          for (int off = 16; off >= g.tpr; off >>= 1) {
+          for (int off = 16; off >= tpr; off >>= 1) {
 #pragma unroll
             for (int e = 0; e < V2; ++e) {
               acc[e].x += __shfl_xor_sync(0xffffffffu, acc[e].x, off);
               acc[e].y += __shfl_xor_sync(0xffffffffu, acc[e].y, off);
             }
           }
-          if (!vok[k] || (g.tpr < 32 && (tid & 31) >= g.tpr)) return;
-          float* q = out + (int64_t)__popc(p.acc & (which - 1)) * p.cols + col0 + k * colk;
+          if (!vok[k] || (tpr < 32 && (tid & 31) >= tpr)) return;
+          float* q = out + (int64_t)__popc(p.acc & (which - 1)) * cols + col[k];
 #pragma unroll
           for (int e = 0; e < V2; e += 2)
             *reinterpret_cast<float4*>(q + 2 * e) =
@@ -812,19 +846,66 @@ static int nga_launch(F kern, const NgaParams& p, const NgaGeom& g, cudaStream_t
   FLN_CHECK_LAUNCH();
   return FLN_OK;
 }
+// the compile-time rows: 16 elements per thread, 128 to 8192 columns (powers of two)
+template <typename T, int K, int GATE, int TPR>
+static int nga_fwd_rows_t(const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
+  constexpr bool HOLD = K * 16 / (int)sizeof(T) <= 16;
+  return nga_general(p) ? nga_launch(nga_fwd_rows_kernel<T, K, GATE, true, HOLD, TPR>, p, g, st)
+                        : nga_launch(nga_fwd_rows_kernel<T, K, GATE, false, HOLD, TPR>, p, g, st);
+}
 template <typename T, int K, int GATE>
 static int nga_fwd_rows_k(const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
-  constexpr bool HOLD = K * 16 / (int)sizeof(T) <= 16;
-  return nga_general(p) ? nga_launch(nga_fwd_rows_kernel<T, K, GATE, true, HOLD>, p, g, st)
-                        : nga_launch(nga_fwd_rows_kernel<T, K, GATE, false, HOLD>, p, g, st);
+  if constexpr (K * 16 / (int)sizeof(T) == 16) {
+    if (g.nv == K * g.tpr) {
+      switch (g.tpr) {
+        case 8:
+          return nga_fwd_rows_t<T, K, GATE, 8>(p, g, st);
+        case 64:
+          return nga_fwd_rows_t<T, K, GATE, 64>(p, g, st);
+        case 128:
+          return nga_fwd_rows_t<T, K, GATE, 128>(p, g, st);
+        case 256:
+          return nga_fwd_rows_t<T, K, GATE, 256>(p, g, st);
+        case 512:
+          return nga_fwd_rows_t<T, K, GATE, 512>(p, g, st);
+      }
+    }
+  }
+  return nga_fwd_rows_t<T, K, GATE, 0>(p, g, st);
+}
+template <typename T, int K, int GATE, bool GEN>
+static int nga_bwd_rows_g(const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
+  const int set = nga_set_of(p);
+  if (!g.csm) return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, false, 0, 0>, p, g, st);
+  // compile-time rows where the registers allow: 16 elements per thread, 8 of the general form
+  if constexpr (K * 16 / (int)sizeof(T) == (GEN ? 8 : 16)) {
+    if (g.nv == K * g.tpr && set == 1) {
+      switch (g.tpr) {
+        case 64:
+          return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 64, 1>, p, g, st);
+        case 128:
+          return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 128, 1>, p, g, st);
+        case 256:
+          return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 256, 1>, p, g, st);
+        case 512:
+          return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 512, 1>, p, g, st);
+      }
+    }
+    if (g.nv == K * g.tpr && set == 2) {
+      switch (g.tpr) {
+        case 8:
+          return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 8, 2>, p, g, st);
+        case 16:
+          return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 16, 2>, p, g, st);
+      }
+    }
+  }
+  if (set == 1) return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, 1>, p, g, st);
+  return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, 0>, p, g, st);
 }
 template <typename T, int K, int GATE>
 static int nga_bwd_rows_k(const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
-  if (g.csm)
-    return nga_general(p) ? nga_launch(nga_bwd_rows_kernel<T, K, GATE, true, true>, p, g, st)
-                          : nga_launch(nga_bwd_rows_kernel<T, K, GATE, false, true>, p, g, st);
-  return nga_general(p) ? nga_launch(nga_bwd_rows_kernel<T, K, GATE, true, false>, p, g, st)
-                        : nga_launch(nga_bwd_rows_kernel<T, K, GATE, false, false>, p, g, st);
+  return nga_general(p) ? nga_bwd_rows_g<T, K, GATE, true>(p, g, st) : nga_bwd_rows_g<T, K, GATE, false>(p, g, st);
 }
 
 #define FLN_NGA_GATES(F, T, K)              \
