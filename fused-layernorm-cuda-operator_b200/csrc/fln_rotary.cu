@@ -114,7 +114,7 @@ static RotPlan make_rot_plan(const fln_rotary_args* a, void* const* dx, RotParam
     return l;
   };
   plan.U = 1;
-  if (lanes(1) > 32 || lanes(3) * 3 * 5 < lanes(1) * 4) plan.U = 3;
+  if (lanes(1) > 32 || (V <= 4 && lanes(3) * 3 * 5 < lanes(1) * 4)) plan.U = 3;
   if (lanes(plan.U) > 32) plan.U = 8;
   int l = lanes(plan.U), lg = 0;
   while ((1 << lg) < l) ++lg;
@@ -230,10 +230,11 @@ extern "C" int fln_qk_norm_rotary_backward(const fln_rotary_args* a, void* const
   if (dx == nullptr || dweight == nullptr || dbias == nullptr) return FLN_ERR_NULL;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const size_t es = a->dtype == FLN_F32 ? 4 : 2;
-  bool sums = false;
+  bool sums = false, want_db = false;
   for (int i = 0; i < 2; ++i) {
     if (a->kind == FLN_NO_NORM && (dweight[i] != nullptr || dbias[i] != nullptr)) return FLN_ERR_ARG;
     sums = sums || dweight[i] != nullptr || dbias[i] != nullptr;
+    want_db = want_db || dbias[i] != nullptr;
     // a tensor without rows: its sums are zeros
     if (empty(a) || a->t[i].heads == 0) {
       void* const z[] = {dweight[i], dbias[i]};
@@ -252,6 +253,7 @@ extern "C" int fln_qk_norm_rotary_backward(const fln_rotary_args* a, void* const
   int n0, n1;
   bwd_grid(a, &n0, &n1);
   p.nb0 = n0;
+  p.want_db = want_db ? 1 : 0;
   if (sums) {
     if (workspace == nullptr || workspace_bytes < fln_qk_norm_rotary_workspace_bytes(a) || !is_aligned16(workspace))
       return FLN_ERR_WORKSPACE;

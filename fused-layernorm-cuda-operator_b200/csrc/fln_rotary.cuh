@@ -49,6 +49,7 @@ struct RotParams {
   // the k heads.  backward: the first nb0 CTAs take q, the others k; items of `per_split` heads.
   int splits[2], per_split[2];
   int nb0;
+  int want_db;  // a bias gradient is asked for
 };
 
 constexpr int kRotThreads = 256;
@@ -65,235 +66,354 @@ __device__ __forceinline__ void unit_columns(const RotParams& p, int u, int& lo,
   }
 }
 
-// cosine and sine (times the magnitude) of the V pairs of a unit
-template <int V>
-__device__ __forceinline__ void unit_angles(const RotParams& p, int u, int b, int s, float (&c)[V], float (&sn)[V]) {
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    c[j] = 1.f;
-    sn[j] = 0.f;
+// Tables in shared memory, in 32 bits.  Every warp keeps the cosines and sines of its token, one
+// entry per pair and 1 / 0 behind them (units of the part that is not rotated): the lanes make the
+// angles between them, P / 32 each, and all row groups of the warp read them.  The CTA keeps
+// weight_offset + weight and bias of both tensors.  (With the angles made by every lane for its own
+// unit and held in registers beside the weights, the bf16 forward at 8192 x 48 x 128 ran with 80
+// registers, 16.7 instructions per element, 55 us.)
+struct RotTables {
+  float *c, *s;  // of this warp: [units * V] each
+  float *w, *b;  // of q; those of k lie `step` behind them
+  int step;
+};
+__host__ __device__ constexpr size_t rot_tables_floats(int units, int V, int dim, bool gen) {
+  return (size_t)(kRotThreads / 32) * 2 * units * V + (size_t)(gen ? 4 : 2) * ((dim + 3) & ~3);
+}
+template <typename T, int V, bool GEN>
+__device__ __forceinline__ RotTables rot_tables(const RotParams& p, float* mem) {
+  RotTables t;
+  const int n = p.units * V, warp = threadIdx.x >> 5, dim4 = (p.dim + 3) & ~3;
+  t.c = mem + warp * 2 * n;
+  t.s = t.c + n;
+  t.w = mem + (kRotThreads / 32) * 2 * n;
+  t.b = t.w + dim4;
+  t.step = GEN ? 2 * dim4 : dim4;
+  for (int i = threadIdx.x & 31; i < n; i += 32) {
+    t.c[i] = 1.f;
+    t.s[i] = 0.f;
   }
-  if (u >= p.rot_units) return;
+  for (int i = threadIdx.x; i < 2 * p.dim; i += kRotThreads) {
+    const int which = i >= p.dim ? 1 : 0, c = i - which * p.dim;
+    const T* w = reinterpret_cast<const T*>(p.t[which].weight);
+    t.w[which * t.step + c] = w != nullptr ? p.woff + Cvt<T>::to_f(w[c]) : 1.f;
+    if (GEN) {
+      const T* b = reinterpret_cast<const T*>(p.t[which].bias);
+      t.b[which * t.step + c] = b != nullptr ? Cvt<T>::to_f(b[c]) : 0.f;
+    }
+  }
+  __syncthreads();
+  return t;
+}
+// the angles of a token into its warp's table
+__device__ __forceinline__ void token_angles(const RotParams& p, const RotTables& t, int b, int s) {
   const int64_t at0 = (int64_t)b * p.pos_batch + (int64_t)s * p.pos_seq;
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int i = u * V + j;
+  __syncwarp();  // nobody reads the last token's any more
+  for (int i = threadIdx.x & 31; i < p.pairs; i += 32) {
     const int64_t at = at0 + (int64_t)__ldg(p.axis + i) * p.pos_axis;
-    const long long pos = p.pos64 ? reinterpret_cast<const long long*>(p.positions)[at]
-                                  : (long long)reinterpret_cast<const int*>(p.positions)[at];
+    const long long pos = p.pos64 ? __ldg(reinterpret_cast<const long long*>(p.positions) + at)
+                                  : (long long)__ldg(reinterpret_cast<const int*>(p.positions) + at);
     const long long frac = (long long)((unsigned long long)pos * __ldg(p.turns + i));
     // frac / 2^64 turns = frac / 2^63 half turns, in [-1, 1]
     float sv, cv;
     sincospif(__ll2float_rn(frac) * 1.0842021724855044e-19f, &sv, &cv);
-    c[j] = cv * p.mag;
-    sn[j] = sv * p.mag;
+    t.c[i] = cv * p.mag;
+    t.s[i] = sv * p.mag;
+  }
+  __syncwarp();
+}
+// V floats of a table
+template <int V>
+__device__ __forceinline__ void table_take(const float* t, float (&f)[V]) {
+  if constexpr (V >= 4) {
+#pragma unroll
+    for (int j = 0; j < V; j += 4) {
+      const float4 q = *reinterpret_cast<const float4*>(t + j);
+      f[j] = q.x;
+      f[j + 1] = q.y;
+      f[j + 2] = q.z;
+      f[j + 3] = q.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = t[j];
+  }
+}
+// a unit's share of a row table, as register pairs
+template <int V>
+__device__ __forceinline__ void table_unit(const float* t, int lo, int hi, float2 (&f)[V]) {
+  float a[V], b[V];
+  table_take<V>(t + lo, a);
+  table_take<V>(t + hi, b);
+  if constexpr (V == 1) {
+    f[0] = make_float2(a[0], b[0]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) {
+      f[j] = make_float2(a[2 * j], a[2 * j + 1]);
+      f[V / 2 + j] = make_float2(b[2 * j], b[2 * j + 1]);
+    }
   }
 }
 
-// the two vectors of a unit of one row as floats e[0, V) and e[V, 2V); zeros where absent
+// A unit as V register pairs: f[0, V / 2) its first vector and f[V / 2, V) its second one; with
+// V == 1 both elements in one pair.
 template <typename T, int V>
-__device__ __forceinline__ void unit_load(const T* row, int lo, int hi, bool ok, Pack<T, V>& a, Pack<T, V>& b) {
+struct UnitPack {
+  Pack<T, V> a, b;
+};
+// (absent vectors read as zeros)
+template <typename T, int V, bool WHOLE>
+__device__ __forceinline__ UnitPack<T, V> unit_load(const T* row, int lo, int hi, bool lo_ok, bool hi_ok) {
+  UnitPack<T, V> u;
+  if (!WHOLE) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    a.e[j] = Cvt<T>::from_f(0.f);
-    b.e[j] = Cvt<T>::from_f(0.f);
+    for (int j = 0; j < V; ++j) {
+      u.a.e[j] = Cvt<T>::from_f(0.f);
+      u.b.e[j] = Cvt<T>::from_f(0.f);
+    }
   }
-  if (ok) {
-    a = ld_stream<T, V>(row + lo);
-    if (hi >= 0) b = ld_stream<T, V>(row + hi);
-  }
+  if (WHOLE || lo_ok) u.a = ld_stream<T, V>(row + lo);
+  if (WHOLE || hi_ok) u.b = ld_stream<T, V>(row + hi);
+  return u;
 }
 template <typename T, int V>
-__device__ __forceinline__ void unit_param(const T* w, int lo, int hi, bool ok, float fill, float (&f)[2 * V]) {
+__device__ __forceinline__ void unit_unpack(const UnitPack<T, V>& u, float2 (&f)[V]) {
+  if constexpr (V == 1) {
+    f[0] = make_float2(Cvt<T>::to_f(u.a.e[0]), Cvt<T>::to_f(u.b.e[0]));
+  } else {
+    float2 t[V / 2];
+    unpack2<T, V>(u.a, t);
 #pragma unroll
-  for (int j = 0; j < 2 * V; ++j) f[j] = fill;
-  if (w == nullptr || !ok) return;
-  float t[V];
-  unpack<T, V>(ld_param<T, V>(w + lo), t);
+    for (int j = 0; j < V / 2; ++j) f[j] = t[j];
+    unpack2<T, V>(u.b, t);
 #pragma unroll
-  for (int j = 0; j < V; ++j) f[j] = t[j];
-  if (hi >= 0) {
-    unpack<T, V>(ld_param<T, V>(w + hi), t);
-#pragma unroll
-    for (int j = 0; j < V; ++j) f[V + j] = t[j];
-  }
-}
-template <typename T, int V>
-__device__ __forceinline__ void unit_store(T* row, int lo, int hi, const float (&f)[2 * V]) {
-  float t[V];
-  Pack<T, V> o;
-#pragma unroll
-  for (int j = 0; j < V; ++j) t[j] = f[j];
-  pack<T, V>(t, o);
-  st_plain<T, V>(row + lo, o);
-  if (hi >= 0) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) t[j] = f[V + j];
-    pack<T, V>(t, o);
-    st_plain<T, V>(row + hi, o);
+    for (int j = 0; j < V / 2; ++j) f[V / 2 + j] = t[j];
   }
 }
 template <typename T, int V>
-__device__ __forceinline__ void unit_unpack(const Pack<T, V>& a, const Pack<T, V>& b, float (&f)[2 * V]) {
-  float t[V];
-  unpack<T, V>(a, t);
+__device__ __forceinline__ void unit_store(T* row, int lo, int hi, bool hi_ok, const float2 (&f)[V]) {
+  if constexpr (V == 1) {
+    row[lo] = Cvt<T>::from_f(f[0].x);
+    if (hi_ok) row[hi] = Cvt<T>::from_f(f[0].y);
+  } else {
+    float2 t[V / 2];
+    Pack<T, V> o;
 #pragma unroll
-  for (int j = 0; j < V; ++j) f[j] = t[j];
-  unpack<T, V>(b, t);
+    for (int j = 0; j < V / 2; ++j) t[j] = f[j];
+    pack2<T, V>(t, o);
+    st_plain<T, V>(row + lo, o);
+    if (hi_ok) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) f[V + j] = t[j];
+      for (int j = 0; j < V / 2; ++j) t[j] = f[V / 2 + j];
+      pack2<T, V>(t, o);
+      st_plain<T, V>(row + hi, o);
+    }
+  }
 }
-
-// rotation by the angle (sign = 1) or back (sign = -1) of the V pairs of a unit
+// rotation of the V pairs of a unit by the angle, or back
 template <int V, bool HALF, bool BACK>
-__device__ __forceinline__ void unit_rotate(float (&f)[2 * V], const float (&c)[V], const float (&s)[V]) {
+__device__ __forceinline__ void unit_rotate(float2 (&f)[V], const float (&c)[V], const float (&s)[V]) {
+  if constexpr (HALF && V > 1) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int ia = HALF ? j : 2 * j, ib = HALF ? V + j : 2 * j + 1;
-    const float a = f[ia], b = f[ib];
-    f[ia] = BACK ? fmaf(b, s[j], a * c[j]) : fmaf(-b, s[j], a * c[j]);
-    f[ib] = BACK ? fmaf(-a, s[j], b * c[j]) : fmaf(a, s[j], b * c[j]);
+    for (int j = 0; j < V / 2; ++j) {
+      const float2 cc = make_float2(c[2 * j], c[2 * j + 1]);
+      const float2 ss = make_float2(s[2 * j], s[2 * j + 1]), ns = make_float2(-s[2 * j], -s[2 * j + 1]);
+      const float2 a = f[j], b = f[V / 2 + j];
+      f[j] = f2fma(b, BACK ? ss : ns, f2mul(a, cc));
+      f[V / 2 + j] = f2fma(a, BACK ? ns : ss, f2mul(b, cc));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float a = f[j].x, b = f[j].y;
+      f[j].x = BACK ? fmaf(b, s[j], a * c[j]) : fmaf(-b, s[j], a * c[j]);
+      f[j].y = BACK ? fmaf(-a, s[j], b * c[j]) : fmaf(a, s[j], b * c[j]);
+    }
   }
 }
 
-template <int N>
+template <int N, int LL>
 __device__ __forceinline__ void lane_sum(float (&v)[N], int log2_l) {
-  for (int off = (1 << log2_l) >> 1; off > 0; off >>= 1) {
+  if constexpr (LL >= 0) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], off);
+    for (int off = (1 << LL) >> 1; off > 0; off >>= 1) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], off);
+    }
+  } else {
+    for (int off = (1 << log2_l) >> 1; off > 0; off >>= 1) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], off);
+    }
   }
 }
 
-// Statistics of NB rows at once: x becomes xh = (x - mean) * rstd in place (untouched without a
-// norm).  Elements behind the row count as zeros of the centred row.
-template <int NB, int U, int V>
-__device__ __forceinline__ void rows_normalize(const RotParams& p, float (&x)[NB][U][2 * V], const bool (&lo_ok)[U],
-                                               const bool (&hi_ok)[U], float (&rstd)[NB]) {
-#pragma unroll
-  for (int n = 0; n < NB; ++n) rstd[n] = 1.f;
-  if (p.kind == FLN_NO_NORM) return;
-  const float inv_d = 1.0f / (float)p.dim;
-  float v[NB];
-  if (p.kind == FLN_LAYERNORM) {
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      v[n] = 0.f;
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int j = 0; j < 2 * V; ++j) v[n] += x[n][u][j];
-    }
-    lane_sum<NB>(v, p.log2_l);
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      const float mean = v[n] * inv_d;
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int j = 0; j < 2 * V; ++j)
-          if (j < V ? lo_ok[u] : hi_ok[u]) x[n][u][j] -= mean;
-    }
-  }
-#pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    v[n] = 0.f;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int j = 0; j < 2 * V; ++j) v[n] = fmaf(x[n][u][j], x[n][u][j], v[n]);
-  }
-  lane_sum<NB>(v, p.log2_l);
-#pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    rstd[n] = rsqrtf(fmaf(v[n], inv_d, p.eps));
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int j = 0; j < 2 * V; ++j) x[n][u][j] *= rstd[n];
-  }
+// v where the element exists, else 0: elements behind the row must not count as -mean
+template <int V>
+__device__ __forceinline__ float2 in_row(float2 v, int j, bool lo_ok, bool hi_ok) {
+  if constexpr (V == 1) return make_float2(lo_ok ? v.x : 0.f, hi_ok ? v.y : 0.f);
+  const bool ok = j < V / 2 ? lo_ok : hi_ok;
+  return make_float2(ok ? v.x : 0.f, ok ? v.y : 0.f);
 }
+
+// what every lane of both kernels holds of its place in the row
+template <int V, int U, bool HALF>
+struct RotLane {
+  int L, groups, grp, ul;
+  int lo[U], hi[U];          // first columns of the unit's vectors (of another vector where there is none)
+  int at[U];                 // its first entry in the table of angles
+  bool lo_ok[U], hi_ok[U];
+  template <int LL>
+  __device__ __forceinline__ void init(const RotParams& p) {
+    const int lane = threadIdx.x & 31;
+    const int ll = LL >= 0 ? LL : p.log2_l;
+    L = 1 << ll;
+    groups = 32 >> ll;
+    grp = lane >> ll;
+    ul = lane & (L - 1);
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int u = ul + k * L;
+      lo_ok[k] = u < p.units;
+      unit_columns<V, HALF>(p, lo_ok[k] ? u : 0, lo[k], hi[k]);
+      hi_ok[k] = lo_ok[k] && hi[k] >= 0;
+      if (hi[k] < 0) hi[k] = lo[k];
+      at[k] = (lo_ok[k] ? u : 0) * V;
+      if (LL >= 0) lo_ok[k] = hi_ok[k] = true;  // whole units on every lane
+    }
+  }
+};
 
 // ----------------------------------------------------------------------------------------
 // forward: a warp takes items (token, run of heads); each of its 32 / L row groups takes every
 // (32 / L)-th head of the run, NB of them at a time so that NB rows are on their way from memory
-// together.  All lanes of a warp make the same number of turns, so the shuffles are whole.
+// together.  All lanes of a warp make the same number of turns, so the shuffles are whole.  The
+// rows stay packed as they came; they are unpacked once for the sums and once more for the
+// result, which costs an instruction per element and saves the registers that let more warps
+// (and so more loads) be in flight.
+// GEN: layer norm or bias.  LL >= 0: log2 of the lanes per row, known at compile time.
 // ----------------------------------------------------------------------------------------
-template <typename T, int V, int U, bool HALF, int NB>
-__global__ void __launch_bounds__(kRotThreads) rotary_fwd_kernel(const RotParams p) {
-  const int lane = threadIdx.x & 31;
-  const int L = 1 << p.log2_l;
-  const int groups = 32 >> p.log2_l;
-  const int grp = lane >> p.log2_l, ul = lane & (L - 1);
-  int lo[U], hi[U];
-  bool lo_ok[U], hi_ok[U];
-#pragma unroll
-  for (int k = 0; k < U; ++k) {
-    const int u = ul + k * L;
-    lo_ok[k] = u < p.units;
-    lo[k] = hi[k] = 0;
-    if (lo_ok[k]) unit_columns<V, HALF>(p, u, lo[k], hi[k]);
-    hi_ok[k] = lo_ok[k] && hi[k] >= 0;
-  }
-  const int64_t items = (int64_t)p.tokens * p.splits[0];
-  const int64_t step = (int64_t)gridDim.x * (kRotThreads / 32);
-  const int heads_all = p.t[0].heads + p.t[1].heads;
-  for (int64_t it = (int64_t)blockIdx.x * (kRotThreads / 32) + (threadIdx.x >> 5); it < items; it += step) {
-    const int token = (int)(it / p.splits[0]);
-    const int part = (int)(it - (int64_t)token * p.splits[0]);
-    const int h0 = part * p.per_split[0];
-    const int h1 = h0 + p.per_split[0] < heads_all ? h0 + p.per_split[0] : heads_all;
-    const int b = token / p.seq, s = token - b * p.seq;
-    float cs[U][V], sn[U][V];
-#pragma unroll
-    for (int k = 0; k < U; ++k) unit_angles<V>(p, ul + k * L, b, s, cs[k], sn[k]);
+#ifndef ROT_FMB
+#define ROT_FMB 3
+#endif
+#ifndef ROT_NBF
+#define ROT_NBF 2
+#endif
+template <typename T, int V, int U, bool HALF, int NB, bool GEN, int LL>
+__global__ void __launch_bounds__(kRotThreads, V * U <= 8 ? ROT_FMB : 1) rotary_fwd_kernel(const RotParams p) {
+  RotLane<V, U, HALF> r;
+  r.template init<LL>(p);
+  extern __shared__ __align__(16) float tables[];
+  const RotTables tab = rot_tables<T, V, GEN>(p, tables);
+  constexpr bool WHOLE = LL >= 0;
+  const float inv_d = 1.0f / (float)p.dim;
+  const int splits = p.splits[0], per = p.per_split[0];
+  const int64_t items = (int64_t)p.tokens * splits;
+  const int64_t stride = (int64_t)gridDim.x * (kRotThreads / 32);
+  const int q_heads = p.t[0].heads, heads_all = q_heads + p.t[1].heads;
+  for (int64_t it = (int64_t)blockIdx.x * (kRotThreads / 32) + (threadIdx.x >> 5); it < items; it += stride) {
+    int token, h0 = 0, h1 = heads_all;
+    if (splits == 1) {
+      token = (int)it;
+    } else {
+      token = (int)(it / splits);
+      h0 = (int)(it - (int64_t)token * splits) * per;
+      h1 = h0 + per < heads_all ? h0 + per : heads_all;
+    }
+    const int b = p.tokens == p.seq ? 0 : token / p.seq, s = token - b * p.seq;
+    bool angles = false;
 #pragma unroll 1
     for (int which = 0; which < 2; ++which) {
       const RotTensor& t = p.t[which];
-      const int first = which == 0 ? h0 : (h0 > p.t[0].heads ? h0 - p.t[0].heads : 0);
-      const int end = which == 0 ? (h1 < p.t[0].heads ? h1 : p.t[0].heads) : h1 - p.t[0].heads;
+      const int first = which == 0 ? h0 : (h0 > q_heads ? h0 - q_heads : 0);
+      const int end = which == 0 ? (h1 < q_heads ? h1 : q_heads) : h1 - q_heads;
       if (first >= end) continue;
-      float w[U][2 * V], bi[U][2 * V];
-#pragma unroll
-      for (int k = 0; k < U; ++k) {
-        unit_param<T, V>(reinterpret_cast<const T*>(t.weight), lo[k], hi[k], lo_ok[k], t.weight != nullptr ? 0.f : 1.f, w[k]);
-        unit_param<T, V>(reinterpret_cast<const T*>(t.bias), lo[k], hi[k], lo_ok[k], 0.f, bi[k]);
-        if (t.weight != nullptr) {
-#pragma unroll
-          for (int j = 0; j < 2 * V; ++j) w[k][j] += p.woff;
-        }
-      }
       const T* in = reinterpret_cast<const T*>(t.in) + (int64_t)b * t.in_batch + (int64_t)s * t.in_seq;
       T* out = reinterpret_cast<T*>(t.out) + (int64_t)b * t.out_batch + (int64_t)s * t.out_seq;
 #pragma unroll 1
-      for (int h = first; h < end; h += groups * NB) {
-        Pack<T, V> pa[NB][U], pb[NB][U];
+      for (int h = first; h < end; h += r.groups * NB) {
+        UnitPack<T, V> x[NB][U];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-          const int hh = h + n * groups + grp;
+          // (row groups behind the last head take it once more and store nothing)
+          const int hh = min(h + n * r.groups + r.grp, end - 1);
+          const T* row = in + (int64_t)hh * t.in_head;
 #pragma unroll
-          for (int k = 0; k < U; ++k)
-            unit_load<T, V>(in + (int64_t)hh * t.in_head, lo[k], hi[k], hh < end && lo_ok[k], pa[n][k], pb[n][k]);
+          for (int k = 0; k < U; ++k) x[n][k] = unit_load<T, V, WHOLE>(row, r.lo[k], r.hi[k], r.lo_ok[k], r.hi_ok[k]);
         }
-        float x[NB][U][2 * V], rstd[NB];
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-          for (int k = 0; k < U; ++k) unit_unpack<T, V>(pa[n][k], pb[n][k], x[n][k]);
-        rows_normalize<NB, U, V>(p, x, lo_ok, hi_ok, rstd);
+        if (!angles) {  // behind the first loads, so that both wait for memory together
+          angles = true;
+          token_angles(p, tab, b, s);
+        }
+        float mean[NB], rstd[NB];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-          const int hh = h + n * groups + grp;
-          if (hh < end) {
+          mean[n] = 0.f;
+          rstd[n] = 1.f;
+        }
+        if (p.kind != FLN_NO_NORM) {
+          float v[NB];
+          if (GEN && p.kind == FLN_LAYERNORM) {
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+              float2 a = f2(0.f);
+#pragma unroll
+              for (int k = 0; k < U; ++k) {
+                float2 f[V];
+                unit_unpack<T, V>(x[n][k], f);
+#pragma unroll
+                for (int j = 0; j < V; ++j) a = f2add(a, f[j]);
+              }
+              v[n] = a.x + a.y;
+            }
+            lane_sum<NB, LL>(v, p.log2_l);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) mean[n] = v[n] * inv_d;
+          }
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            float2 a = f2(0.f);
 #pragma unroll
             for (int k = 0; k < U; ++k) {
-              if (lo_ok[k]) {
-                float f[2 * V];
+              float2 f[V];
+              unit_unpack<T, V>(x[n][k], f);
 #pragma unroll
-                for (int j = 0; j < 2 * V; ++j) f[j] = fmaf(x[n][k][j], w[k][j], bi[k][j]);
-                unit_rotate<V, HALF, false>(f, cs[k], sn[k]);
-                unit_store<T, V>(out + (int64_t)hh * t.out_head, lo[k], hi[k], f);
+              for (int j = 0; j < V; ++j) {
+                if (GEN) {
+                  f[j] = f2add(f[j], f2(-mean[n]));
+                  if (!WHOLE) f[j] = in_row<V>(f[j], j, r.lo_ok[k], r.hi_ok[k]);
+                }
+                a = f2fma(f[j], f[j], a);
               }
             }
+            v[n] = a.x + a.y;
+          }
+          lane_sum<NB, LL>(v, p.log2_l);
+#pragma unroll
+          for (int n = 0; n < NB; ++n) rstd[n] = rsqrtf(fmaf(v[n], inv_d, p.eps));
+        }
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          const int hh = h + n * r.groups + r.grp;
+          T* row = out + (int64_t)hh * t.out_head;
+#pragma unroll
+          for (int k = 0; k < U; ++k) {
+            float2 f[V], w[V], bi[V];
+            float cs[V], sn[V];
+            unit_unpack<T, V>(x[n][k], f);
+            table_unit<V>(tab.w + which * tab.step, r.lo[k], r.hi[k], w);
+            if (GEN) table_unit<V>(tab.b + which * tab.step, r.lo[k], r.hi[k], bi);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+              if (GEN) f[j] = f2add(f[j], f2(-mean[n]));
+              f[j] = f2mul(f[j], f2(rstd[n]));
+              f[j] = GEN ? f2fma(f[j], w[j], bi[j]) : f2mul(f[j], w[j]);
+            }
+            table_take<V>(tab.c + r.at[k], cs);
+            table_take<V>(tab.s + r.at[k], sn);
+            unit_rotate<V, HALF, false>(f, cs, sn);
+            if (hh < end && r.lo_ok[k]) unit_store<T, V>(row, r.lo[k], r.hi[k], r.hi_ok[k], f);
           }
         }
       }
@@ -303,130 +423,189 @@ __global__ void __launch_bounds__(kRotThreads) rotary_fwd_kernel(const RotParams
 
 // ----------------------------------------------------------------------------------------
 // backward: the rows are normalized again from the inputs (nothing but them is kept), the
-// gradient is rotated back, and the norm is differentiated.  The sums for weight and bias stay
-// in the lanes' registers over all rows of a CTA and are added in a fixed order at its end, so a
-// CTA works for one tensor only.
+// gradient is rotated back, and the norm is differentiated:
+//     dn = rotated back,  g = dn * w,  c1 = mean(g * xh), c2 = mean(g) (LayerNorm),
+//     dx = rstd * ((g - c2) - xh * c1),  dw = sum dn * xh,  db = sum dn
+// RMSNorm needs one exchange between the lanes: mean(g * xh) = rstd * mean(g * x).  The sums for
+// weight and bias stay in the lanes' registers over all rows of a CTA and are added in a fixed
+// order at its end, so a CTA works for one tensor only.
 // ----------------------------------------------------------------------------------------
-template <typename T, int V, int U, bool HALF, int NB>
-__global__ void __launch_bounds__(kRotThreads) rotary_bwd_kernel(const RotParams p) {
-  extern __shared__ float sacc[];  // [warps][2][dim]
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int L = 1 << p.log2_l;
-  const int groups = 32 >> p.log2_l;
-  const int grp = lane >> p.log2_l, ul = lane & (L - 1);
+template <typename T, int V, int U, bool HALF, int NB, bool GEN, int LL>
+__global__ void __launch_bounds__(kRotThreads, V * U <= 8 ? 2 : 1) rotary_bwd_kernel(const RotParams p) {
+  extern __shared__ __align__(16) float sacc[];  // the tables; at the end [warps][2][dim]
+  const RotTables tab = rot_tables<T, V, GEN>(p, sacc);
+  constexpr bool WHOLE = LL >= 0;
+  const int warp = threadIdx.x >> 5;
+  RotLane<V, U, HALF> r;
+  r.template init<LL>(p);
   const int which = (int)blockIdx.x < p.nb0 ? 0 : 1;
   const RotTensor& t = p.t[which];
   const int cta = which == 0 ? (int)blockIdx.x : (int)blockIdx.x - p.nb0;
   const int ctas = which == 0 ? p.nb0 : (int)gridDim.x - p.nb0;
-  int lo[U], hi[U];
-  bool lo_ok[U], hi_ok[U];
-  float w[U][2 * V], dw[U][2 * V], db[U][2 * V];
+  float2 dw[U][V], db[GEN ? U : 1][V];
 #pragma unroll
   for (int k = 0; k < U; ++k) {
-    const int u = ul + k * L;
-    lo_ok[k] = u < p.units;
-    lo[k] = hi[k] = 0;
-    if (lo_ok[k]) unit_columns<V, HALF>(p, u, lo[k], hi[k]);
-    hi_ok[k] = lo_ok[k] && hi[k] >= 0;
-    unit_param<T, V>(reinterpret_cast<const T*>(t.weight), lo[k], hi[k], lo_ok[k], t.weight != nullptr ? 0.f : 1.f, w[k]);
 #pragma unroll
-    for (int j = 0; j < 2 * V; ++j) {
-      if (t.weight != nullptr) w[k][j] += p.woff;
-      dw[k][j] = 0.f;
-      db[k][j] = 0.f;
+    for (int j = 0; j < V; ++j) {
+      dw[k][j] = f2(0.f);
+      if (GEN) db[GEN ? k : 0][j] = f2(0.f);
     }
   }
   const float inv_d = 1.0f / (float)p.dim;
-  const int splits = p.splits[which], per_split = p.per_split[which];
+  const int splits = p.splits[which], per = p.per_split[which];
   const int64_t items = (int64_t)p.tokens * splits;
-  const int64_t step = (int64_t)ctas * (kRotThreads / 32);
-  for (int64_t it = (int64_t)cta * (kRotThreads / 32) + warp; it < items; it += step) {
-    const int token = (int)(it / splits);
-    const int h0 = (int)(it - (int64_t)token * splits) * per_split;
-    const int end = h0 + per_split < t.heads ? h0 + per_split : t.heads;
-    const int b = token / p.seq, s = token - b * p.seq;
-    float cs[U][V], sn[U][V];
-#pragma unroll
-    for (int k = 0; k < U; ++k) unit_angles<V>(p, ul + k * L, b, s, cs[k], sn[k]);
+  const int64_t stride = (int64_t)ctas * (kRotThreads / 32);
+  for (int64_t it = (int64_t)cta * (kRotThreads / 32) + warp; it < items; it += stride) {
+    int token, h0 = 0, end = t.heads;
+    if (splits == 1) {
+      token = (int)it;
+    } else {
+      token = (int)(it / splits);
+      h0 = (int)(it - (int64_t)token * splits) * per;
+      end = h0 + per < t.heads ? h0 + per : t.heads;
+    }
+    const int b = p.tokens == p.seq ? 0 : token / p.seq, s = token - b * p.seq;
     const T* in = reinterpret_cast<const T*>(t.in) + (int64_t)b * t.in_batch + (int64_t)s * t.in_seq;
     const T* go = reinterpret_cast<const T*>(t.out) + (int64_t)b * t.out_batch + (int64_t)s * t.out_seq;
     T* dx = reinterpret_cast<T*>(t.dx) + (int64_t)token * t.heads * p.dim;
 #pragma unroll 1
-    for (int h = h0; h < end; h += groups * NB) {
-      Pack<T, V> pa[NB][U], pb[NB][U], ga[NB][U], gb[NB][U];
+    for (int h = h0; h < end; h += r.groups * NB) {
+      UnitPack<T, V> px[NB][U], pg[NB][U];
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
-        const int hh = h + n * groups + grp;
+        // (row groups behind the last head read it once more; their gradient is zero)
+        const int hh = min(h + n * r.groups + r.grp, end - 1);
 #pragma unroll
         for (int k = 0; k < U; ++k) {
-          const bool ok = hh < end && lo_ok[k];
-          unit_load<T, V>(in + (int64_t)hh * t.in_head, lo[k], hi[k], ok, pa[n][k], pb[n][k]);
-          unit_load<T, V>(go + (int64_t)hh * t.out_head, lo[k], hi[k], ok, ga[n][k], gb[n][k]);
+          px[n][k] = unit_load<T, V, WHOLE>(in + (int64_t)hh * t.in_head, r.lo[k], r.hi[k], r.lo_ok[k], r.hi_ok[k]);
+          pg[n][k] = unit_load<T, V, WHOLE>(go + (int64_t)hh * t.out_head, r.lo[k], r.hi[k], r.lo_ok[k], r.hi_ok[k]);
         }
       }
-      float x[NB][U][2 * V], rstd[NB];
-#pragma unroll
-      for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int k = 0; k < U; ++k) unit_unpack<T, V>(pa[n][k], pb[n][k], x[n][k]);
-      rows_normalize<NB, U, V>(p, x, lo_ok, hi_ok, rstd);
-      float g[NB][U][2 * V], red[2 * NB];
+      if (h == h0) token_angles(p, tab, b, s);
+      float mean[NB], rstd[NB], c1[NB], c2[NB];
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
-        float r0 = 0.f, r1 = 0.f;
+        mean[n] = 0.f;
+        rstd[n] = 1.f;
+        c1[n] = c2[n] = 0.f;
+      }
+      if (p.kind != FLN_NO_NORM) {
+        if (GEN && p.kind == FLN_LAYERNORM) {
+          float v[NB];
 #pragma unroll
-        for (int k = 0; k < U; ++k) {
-          unit_unpack<T, V>(ga[n][k], gb[n][k], g[n][k]);
-          unit_rotate<V, HALF, true>(g[n][k], cs[k], sn[k]);
+          for (int n = 0; n < NB; ++n) {
+            float2 a = f2(0.f);
 #pragma unroll
-          for (int j = 0; j < 2 * V; ++j) {
-            dw[k][j] = fmaf(g[n][k][j], x[n][k][j], dw[k][j]);
-            db[k][j] += g[n][k][j];
-            g[n][k][j] *= w[k][j];
-            r0 = fmaf(g[n][k][j], x[n][k][j], r0);
-            r1 += g[n][k][j];
+            for (int k = 0; k < U; ++k) {
+              float2 f[V];
+              unit_unpack<T, V>(px[n][k], f);
+#pragma unroll
+              for (int j = 0; j < V; ++j) a = f2add(a, f[j]);
+            }
+            v[n] = a.x + a.y;
           }
-        }
-        red[2 * n] = r0;
-        red[2 * n + 1] = r1;
-      }
-      if (p.kind != FLN_NO_NORM) lane_sum<2 * NB>(red, p.log2_l);
-      if (t.dx == nullptr) continue;
+          lane_sum<NB, LL>(v, p.log2_l);
 #pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        const int hh = h + n * groups + grp;
-        if (hh < end) {
-          const float c1 = red[2 * n] * inv_d;
-          const float c2 = p.kind == FLN_LAYERNORM ? red[2 * n + 1] * inv_d : 0.f;
+          for (int n = 0; n < NB; ++n) mean[n] = v[n] * inv_d;
+        }
+        constexpr int NS = GEN ? 3 : 2;
+        float v[NS * NB];  // the squares, g times the centred row, g
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          float2 a = f2(0.f), gx = f2(0.f), gs = f2(0.f);
 #pragma unroll
           for (int k = 0; k < U; ++k) {
-            if (lo_ok[k]) {
-              if (p.kind != FLN_NO_NORM) {
+            float2 x[V], g[V], w[V];
+            float cs[V], sn[V];
+            unit_unpack<T, V>(px[n][k], x);
+            unit_unpack<T, V>(pg[n][k], g);
+            table_take<V>(tab.c + r.at[k], cs);
+            table_take<V>(tab.s + r.at[k], sn);
+            unit_rotate<V, HALF, true>(g, cs, sn);
+            table_unit<V>(tab.w + which * tab.step, r.lo[k], r.hi[k], w);
 #pragma unroll
-                for (int j = 0; j < 2 * V; ++j) g[n][k][j] = rstd[n] * fmaf(-x[n][k][j], c1, g[n][k][j] - c2);
+            for (int j = 0; j < V; ++j) {
+              if (GEN) {
+                x[j] = f2add(x[j], f2(-mean[n]));
+                if (!WHOLE) x[j] = in_row<V>(x[j], j, r.lo_ok[k], r.hi_ok[k]);
               }
-              unit_store<T, V>(dx + (int64_t)hh * p.dim, lo[k], hi[k], g[n][k]);
+              const float2 q = f2mul(g[j], w[j]);
+              a = f2fma(x[j], x[j], a);
+              gx = f2fma(q, x[j], gx);
+              if (GEN) gs = f2add(gs, q);
             }
           }
+          v[NS * n] = a.x + a.y;
+          v[NS * n + 1] = gx.x + gx.y;
+          if (GEN) v[NS * n + NS - 1] = gs.x + gs.y;
+        }
+        lane_sum<NS * NB, LL>(v, p.log2_l);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          rstd[n] = rsqrtf(fmaf(v[NS * n], inv_d, p.eps));
+          c1[n] = rstd[n] * v[NS * n + 1] * inv_d;
+          if (GEN && p.kind == FLN_LAYERNORM) c2[n] = v[NS * n + NS - 1] * inv_d;
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const int hh = h + n * r.groups + r.grp;
+        const bool live = hh < end;
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          float2 x[V], g[V], w[V];
+          float cs[V], sn[V];
+          unit_unpack<T, V>(px[n][k], x);
+          unit_unpack<T, V>(pg[n][k], g);
+          table_take<V>(tab.c + r.at[k], cs);
+          table_take<V>(tab.s + r.at[k], sn);
+          unit_rotate<V, HALF, true>(g, cs, sn);
+          table_unit<V>(tab.w + which * tab.step, r.lo[k], r.hi[k], w);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            if (GEN) x[j] = f2add(x[j], f2(-mean[n]));
+            x[j] = f2mul(x[j], f2(rstd[n]));
+            if (live) {
+              dw[k][j] = f2fma(g[j], x[j], dw[k][j]);
+              if (GEN) db[GEN ? k : 0][j] = f2add(db[GEN ? k : 0][j], g[j]);
+            }
+            g[j] = f2mul(g[j], w[j]);
+            if (p.kind != FLN_NO_NORM) {
+              if (GEN) g[j] = f2add(g[j], f2(-c2[n]));
+              g[j] = f2mul(f2fma(x[j], f2(-c1[n]), g[j]), f2(rstd[n]));
+            }
+          }
+          if (t.dx != nullptr && live && r.lo_ok[k])
+            unit_store<T, V>(dx + (int64_t)hh * p.dim, r.lo[k], r.hi[k], r.hi_ok[k], g);
         }
       }
     }
   }
   if (t.partials == nullptr) return;
+  __syncthreads();  // the tables are done with
   // row groups of the warp, then the warps of the CTA
 #pragma unroll
   for (int k = 0; k < U; ++k) {
 #pragma unroll
-    for (int j = 0; j < 2 * V; ++j) {
-      for (int off = 16; off >= L; off >>= 1) {
-        dw[k][j] += __shfl_xor_sync(0xffffffffu, dw[k][j], off);
-        db[k][j] += __shfl_xor_sync(0xffffffffu, db[k][j], off);
+    for (int j = 0; j < V; ++j) {
+      for (int off = 16; off >= r.L; off >>= 1) {
+        dw[k][j].x += __shfl_xor_sync(0xffffffffu, dw[k][j].x, off);
+        dw[k][j].y += __shfl_xor_sync(0xffffffffu, dw[k][j].y, off);
+        if (GEN) {
+          db[GEN ? k : 0][j].x += __shfl_xor_sync(0xffffffffu, db[GEN ? k : 0][j].x, off);
+          db[GEN ? k : 0][j].y += __shfl_xor_sync(0xffffffffu, db[GEN ? k : 0][j].y, off);
+        }
       }
-      const bool ok = j < V ? lo_ok[k] : hi_ok[k];
-      const int c = (j < V ? lo[k] + j : hi[k] + j - V);
-      if (grp == 0 && ok) {
-        sacc[(warp * 2) * p.dim + c] = dw[k][j];
-        sacc[(warp * 2 + 1) * p.dim + c] = db[k][j];
+      if (r.grp == 0) {
+        const int i = 2 * j;  // elements i and i + 1 of the unit, of the first vector and then the second
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const bool second = i + e >= V;
+          if (second ? !r.hi_ok[k] : !r.lo_ok[k]) continue;
+          const int c = second ? r.hi[k] + i + e - V : r.lo[k] + i + e;
+          sacc[(warp * 2) * p.dim + c] = e == 0 ? dw[k][j].x : dw[k][j].y;
+          sacc[(warp * 2 + 1) * p.dim + c] = GEN ? (e == 0 ? db[GEN ? k : 0][j].x : db[GEN ? k : 0][j].y) : 0.f;
+        }
       }
     }
   }
@@ -447,22 +626,43 @@ struct RotPlan {
 template <typename T>
 int rotary_launch(const RotParams& p, const RotPlan& plan, bool backward, unsigned grid, cudaStream_t st);
 
-template <typename T, int V, int U>
-static int rotary_launch_vu(const RotParams& p, bool half, bool backward, unsigned grid, cudaStream_t st) {
-  // rows in flight per row group: 64 bytes of each tensor per lane where the registers allow it
-  constexpr int W = V * U * (int)sizeof(T);
-  constexpr int NBF = W <= 16 ? 4 : (W <= 32 ? 2 : 1);
-  constexpr int NBB = W <= 16 ? 2 : 1;
+template <typename T, int V, int U, bool HALF, bool GEN, int LL>
+static int rotary_launch_one(const RotParams& p, bool backward, unsigned grid, cudaStream_t st) {
+  // rows in flight per row group: 128 bytes of each tensor per lane where the registers allow it
+  constexpr int W = 2 * V * U * (int)sizeof(T);
+  constexpr int NBF = W <= 32 ? ROT_NBF : (W <= 64 ? 2 : 1);
+  constexpr int NBB = W <= 32 ? 2 : 1;
+  size_t smem = rot_tables_floats(p.units, V, p.dim, GEN) * sizeof(float);
   if (!backward) {
-    if (half) rotary_fwd_kernel<T, V, U, true, NBF><<<grid, kRotThreads, 0, st>>>(p);
-    else rotary_fwd_kernel<T, V, U, false, NBF><<<grid, kRotThreads, 0, st>>>(p);
+    rotary_fwd_kernel<T, V, U, HALF, NBF, GEN, LL><<<grid, kRotThreads, smem, st>>>(p);
   } else {
-    const size_t smem = (size_t)(kRotThreads / 32) * 2 * p.dim * sizeof(float);
-    if (half) rotary_bwd_kernel<T, V, U, true, NBB><<<grid, kRotThreads, smem, st>>>(p);
-    else rotary_bwd_kernel<T, V, U, false, NBB><<<grid, kRotThreads, smem, st>>>(p);
+    const size_t sums = (size_t)(kRotThreads / 32) * 2 * p.dim * sizeof(float);
+    if (sums > smem) smem = sums;
+    rotary_bwd_kernel<T, V, U, HALF, NBB, GEN, LL><<<grid, kRotThreads, smem, st>>>(p);
   }
   FLN_CHECK_LAUNCH();
   return FLN_OK;
+}
+template <typename T, int V, int U, bool HALF, bool GEN>
+static int rotary_launch_ll(const RotParams& p, bool backward, unsigned grid, cudaStream_t st) {
+  // heads that fill the lanes with whole 16-byte vectors (64, 128 and 256 elements of 16 bits) have
+  // their own kernels
+  if constexpr (U == 1 && V * (int)sizeof(T) == 16) {
+    if (2 * p.units * V != p.dim || p.units != 1 << p.log2_l) return rotary_launch_one<T, V, U, HALF, GEN, -1>(p, backward, grid, st);
+    if (p.log2_l == 2) return rotary_launch_one<T, V, U, HALF, GEN, 2>(p, backward, grid, st);
+    if (p.log2_l == 3) return rotary_launch_one<T, V, U, HALF, GEN, 3>(p, backward, grid, st);
+    if (p.log2_l == 4) return rotary_launch_one<T, V, U, HALF, GEN, 4>(p, backward, grid, st);
+  }
+  return rotary_launch_one<T, V, U, HALF, GEN, -1>(p, backward, grid, st);
+}
+template <typename T, int V, int U>
+static int rotary_launch_vu(const RotParams& p, bool half, bool backward, unsigned grid, cudaStream_t st) {
+  const bool gen = p.kind == FLN_LAYERNORM || p.t[0].bias != nullptr || p.t[1].bias != nullptr || p.want_db;
+  if (half)
+    return gen ? rotary_launch_ll<T, V, U, true, true>(p, backward, grid, st)
+               : rotary_launch_ll<T, V, U, true, false>(p, backward, grid, st);
+  return gen ? rotary_launch_ll<T, V, U, false, true>(p, backward, grid, st)
+             : rotary_launch_ll<T, V, U, false, false>(p, backward, grid, st);
 }
 
 template <typename T, int V>
@@ -471,7 +671,8 @@ static int rotary_launch_v(const RotParams& p, const RotPlan& plan, bool backwar
     case 1:
       return rotary_launch_vu<T, V, 1>(p, plan.half, backward, grid, st);
     case 3:
-      return rotary_launch_vu<T, V, 3>(p, plan.half, backward, grid, st);
+      if constexpr (V <= 4) return rotary_launch_vu<T, V, 3>(p, plan.half, backward, grid, st);
+      return FLN_ERR_UNSUPPORTED;
     case 8:
       if constexpr (V <= 2) return rotary_launch_vu<T, V, 8>(p, plan.half, backward, grid, st);
       return FLN_ERR_UNSUPPORTED;
