@@ -7,10 +7,14 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/autograd.h>
 #include <torch/extension.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/library.h>
 
 #include <algorithm>
 #include <array>
+#include <mutex>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -215,7 +219,7 @@ std::array<Tensor, 7> nga_backward(const OptTensor& dy_o, const OptTensor& dsum_
     if (need[i] && present) g[i] = new_cuda(t->sizes(), input.scalar_type(), input);
   };
   want(0, true, input);
-  want(1, has(residual), residual);
+  want(1, true, input);  // (asked for only where there was one; without a second norm it is not kept)
   want(2, has(gate), gate);
   want(3, has(w1), w1);
   want(4, has(b1), b1);
@@ -247,47 +251,52 @@ void refuse_double_backward(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, " has no second derivative: call backward without create_graph=True");
 }
 
-// One node for all seven inputs.  Outputs: (y, sum), or (sum) when there is no second norm.
-struct NgaAutograd : public torch::autograd::Function<NgaAutograd> {
-  static torch::autograd::tensor_list forward(torch::autograd::AutogradContext* ctx, const Tensor& input,
-                                              const OptTensor& residual, const OptTensor& gate, const OptTensor& w1,
-                                              const OptTensor& b1, const OptTensor& w2, const OptTensor& b2,
-                                              int64_t post_kind, int64_t kind, int64_t act, double ba, double ra,
-                                              double woff, double eps1, double eps2) {
-    at::AutoDispatchBelowADInplaceOrView guard;
-    const NgaConf c{post_kind, kind, act, ba, ra, woff, eps1, eps2};
-    NgaOut o = nga_forward(input, residual, gate, w1, b1, w2, b2, c, true);
-    auto t = [](const OptTensor& v) { return has(v) ? *v : Tensor(); };
-    ctx->save_for_backward({input, t(residual), t(gate), t(w1), t(b1), t(w2), t(b2), o.mean1,
-                            o.rstd1, o.mean2, o.rstd2});
-    // needs_input_grad counts only the tensor arguments that are present
-    const OptTensor* in[7] = {nullptr, &residual, &gate, &w1, &b1, &w2, &b2};
-    std::vector<int64_t> at{0};
-    int64_t next = 1;
-    for (int i = 1; i < 7; ++i) at.push_back(has(*in[i]) ? next++ : -1);
-    ctx->saved_data["at"] = at;
-    ctx->saved_data["i"] = std::vector<int64_t>{post_kind, kind, act};
-    ctx->saved_data["f"] = std::vector<double>{ba, ra, woff, eps1, eps2};
-    ctx->set_materialize_grads(false);
-    if (kind == FLN_NO_NORM) return {o.sum};
-    return {o.y, o.sum};
+// The autograd nodes are written against torch's Node directly: a node made by
+// torch::autograd::Function keeps its constants in a dictionary and its tensors in lists, some
+// 20 us per step on the host, more than the kernels take at small sizes.
+using torch::autograd::SavedVariable;
+using torch::autograd::variable_list;
+SavedVariable saved(const OptTensor& t) { return has(t) ? SavedVariable(*t, false) : SavedVariable(); }
+OptTensor unpacked(const SavedVariable& v) {
+  Tensor t = v.unpack();
+  return t.defined() ? OptTensor(t) : std::nullopt;
+}
+Tensor or_undefined(const OptTensor& t) { return has(t) ? *t : Tensor(); }
+void refuse_forward_mode(std::initializer_list<const OptTensor*> ts, const char* what) {
+  for (const OptTensor* t : ts)
+    TORCH_CHECK(!has(*t) || !torch::autograd::isFwGradDefined(*t), what, " has no forward-mode derivative");
+}
+template <typename N>
+std::shared_ptr<N> make_node(torch::autograd::edge_list&& edges) {
+  auto n = std::shared_ptr<N>(new N(), torch::autograd::deleteNode);
+  n->set_next_edges(std::move(edges));
+  return n;
+}
+
+// gradients of input, residual, gate, post_weight, post_bias, weight, bias from those of (y, sum),
+// or of (sum) when there is no second norm
+struct NgaNode : public torch::autograd::Node {
+  SavedVariable in[7], stat[4];
+  NgaConf c{};
+  std::string name() const override { return "NormGateAddNormBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (auto& v : in) v.reset_data();
+    for (auto& v : stat) v.reset_data();
   }
-  static torch::autograd::tensor_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::tensor_list grads) {
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
     refuse_double_backward("fused_norm_gate_add_norm");
-    auto v = ctx->get_saved_variables();
-    const auto at = ctx->saved_data["at"].toIntVector();
-    const auto i = ctx->saved_data["i"].toIntVector();
-    const auto f = ctx->saved_data["f"].toDoubleVector();
-    const NgaConf c{i[0], i[1], i[2], f[0], f[1], f[2], f[3], f[4]};
     const Tensor dy = c.kind == FLN_NO_NORM ? Tensor() : grads[0];
     const Tensor ds = c.kind == FLN_NO_NORM ? grads[0] : grads[1];
-    torch::autograd::tensor_list out(15);
+    variable_list out(7);
     if (!dy.defined() && !ds.defined()) return out;
     NgaNeed need;
-    for (int j = 0; j < 7; ++j) need[j] = at[j] >= 0 && ctx->needs_input_grad((size_t)at[j]);
-    auto g = nga_backward(opt(dy), opt(ds), v[0], opt(v[1]), opt(v[2]), opt(v[3]), opt(v[4]), opt(v[5]), opt(v[6]),
-                          opt(v[7]), opt(v[8]), opt(v[9]), opt(v[10]), c, need);
-    for (int j = 0; j < 7; ++j) out[j] = g[j];
+    for (size_t j = 0; j < 7; ++j) need[j] = task_should_compute_output(j);
+    auto g = nga_backward(opt(dy), opt(ds), *unpacked(in[0]), unpacked(in[1]), unpacked(in[2]), unpacked(in[3]),
+                          unpacked(in[4]), unpacked(in[5]), unpacked(in[6]), unpacked(stat[0]), unpacked(stat[1]),
+                          unpacked(stat[2]), unpacked(stat[3]), c, need);
+    for (size_t j = 0; j < 7; ++j) out[j] = g[j];
     return out;
   }
 };
@@ -309,9 +318,25 @@ std::tuple<OptTensor, Tensor> norm_gate_add_norm(const Tensor& input, const OptT
     NgaOut o = nga_forward(input, residual, gate, w1, b1, w2, b2, {post_kind, kind, act, ba, ra, woff, eps1, eps2}, false);
     return {opt(o.y), o.sum};
   }
-  auto o = NgaAutograd::apply(input, residual, gate, w1, b1, w2, b2, post_kind, kind, act, ba, ra, woff, eps1, eps2);
-  if (kind == FLN_NO_NORM) return {std::nullopt, o[0]};
-  return {o[0], o[1]};
+  refuse_forward_mode({&in, &residual, &gate, &w1, &b1, &w2, &b2}, "fused_norm_gate_add_norm");
+  const NgaConf c{post_kind, kind, act, ba, ra, woff, eps1, eps2};
+  NgaOut o;
+  {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    o = nga_forward(input, residual, gate, w1, b1, w2, b2, c, true);
+  }
+  auto n = make_node<NgaNode>(torch::autograd::collect_next_edges(input, or_undefined(residual), or_undefined(gate),
+                                                                  or_undefined(w1), or_undefined(b1), or_undefined(w2),
+                                                                  or_undefined(b2)));
+  const OptTensor* ts[7] = {&in, &residual, &gate, &w1, &b1, &w2, &b2};
+  for (int i = 0; i < 7; ++i)
+    if (i != 1 || kind != FLN_NO_NORM) n->in[i] = saved(*ts[i]);
+  const Tensor* st[4] = {&o.mean1, &o.rstd1, &o.mean2, &o.rstd2};
+  for (int i = 0; i < 4; ++i) n->stat[i] = saved(opt(*st[i]));
+  n->c = c;
+  if (kind != FLN_NO_NORM) torch::autograd::set_history(o.y, n);
+  torch::autograd::set_history(o.sum, n);
+  return {opt(o.y), o.sum};
 }
 
 // operator forms (torch.compile): absent tensors are empty ones
@@ -595,43 +620,25 @@ std::array<Tensor, 6> rot_backward(const OptTensor& dq, const OptTensor& dk, con
   return g;
 }
 
-struct RotAutograd : public torch::autograd::Function<RotAutograd> {
-  static torch::autograd::tensor_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const OptTensor& k,
-                                              const Tensor& positions, const Tensor& turns, const Tensor& axis,
-                                              const OptTensor& qw, const OptTensor& kw, const OptTensor& qb,
-                                              const OptTensor& kb, int64_t pairs, int64_t axes, int64_t layout,
-                                              int64_t kind, double eps, double woff, double mag) {
-    at::AutoDispatchBelowADInplaceOrView guard;
-    const RotConf c{pairs, axes, layout, kind, eps, woff, mag};
-    auto o = rot_forward(q, k, positions, turns, axis, {qw, kw, qb, kb}, c, false);
-    auto t = [](const OptTensor& v) { return has(v) ? *v : Tensor(); };
-    ctx->save_for_backward({q, t(k), positions, turns, axis, t(qw), t(kw), t(qb), t(kb)});
-    // needs_input_grad counts only the tensor arguments that are present: q, k, positions, turns, axis, weights
-    int64_t next = has(k) ? 5 : 4;
-    std::vector<int64_t> at{0, has(k) ? (int64_t)1 : (int64_t)-1};
-    for (const OptTensor* w : {&qw, &kw, &qb, &kb}) at.push_back(has(*w) ? next++ : -1);
-    ctx->saved_data["at"] = at;
-    ctx->saved_data["i"] = std::vector<int64_t>{pairs, axes, layout, kind};
-    ctx->saved_data["f"] = std::vector<double>{eps, woff, mag};
-    ctx->set_materialize_grads(false);
-    if (has(k)) return {o.first, o.second};
-    return {o.first};
+// gradients of q, k, q_weight, k_weight, q_bias, k_bias
+struct RotNode : public torch::autograd::Node {
+  SavedVariable in[9];  // q, k, positions, turns, axis, weights, biases
+  RotConf c{};
+  std::string name() const override { return "QKNormRotaryBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (auto& v : in) v.reset_data();
   }
-  static torch::autograd::tensor_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::tensor_list grads) {
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
     refuse_double_backward("fused_qk_norm_rotary");
-    auto v = ctx->get_saved_variables();
-    const auto at = ctx->saved_data["at"].toIntVector();
-    const auto i = ctx->saved_data["i"].toIntVector();
-    const auto f = ctx->saved_data["f"].toDoubleVector();
-    const RotConf c{i[0], i[1], i[2], i[3], f[0], f[1], f[2]};
     std::array<bool, 6> need;
-    for (int j = 0; j < 6; ++j) need[j] = at[j] >= 0 && ctx->needs_input_grad((size_t)at[j]);
-    auto g = rot_backward(opt(grads[0]), grads.size() > 1 ? opt(grads[1]) : std::nullopt, v[0], opt(v[1]), v[2], v[3],
-                          v[4], {opt(v[5]), opt(v[6]), opt(v[7]), opt(v[8])}, c, need);
-    torch::autograd::tensor_list out(16);
-    out[0] = g[0];
-    out[1] = g[1];
-    for (int j = 0; j < 4; ++j) out[5 + j] = g[2 + j];
+    for (size_t j = 0; j < 6; ++j) need[j] = task_should_compute_output(j);
+    auto g = rot_backward(opt(grads[0]), grads.size() > 1 ? opt(grads[1]) : std::nullopt, *unpacked(in[0]),
+                          unpacked(in[1]), *unpacked(in[2]), *unpacked(in[3]), *unpacked(in[4]),
+                          {unpacked(in[5]), unpacked(in[6]), unpacked(in[7]), unpacked(in[8])}, c, need);
+    variable_list out(6);
+    for (size_t j = 0; j < 6; ++j) out[j] = g[j];
     return out;
   }
 };
@@ -648,8 +655,22 @@ std::tuple<Tensor, OptTensor> qk_norm_rotary(const Tensor& q, const OptTensor& k
     auto o = rot_forward(q, k, positions, turns, axis, {qw, kw, qb, kb}, {pairs, axes, layout, kind, eps, woff, mag}, in_place);
     return {o.first, opt(o.second)};
   }
-  auto o = RotAutograd::apply(q, k, positions, turns, axis, qw, kw, qb, kb, pairs, axes, layout, kind, eps, woff, mag);
-  return {o[0], has(k) ? OptTensor(o[1]) : std::nullopt};
+  refuse_forward_mode({&qo, &k, &qw, &kw, &qb, &kb}, "fused_qk_norm_rotary");
+  const RotConf c{pairs, axes, layout, kind, eps, woff, mag};
+  std::pair<Tensor, Tensor> o;
+  {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    o = rot_forward(q, k, positions, turns, axis, {qw, kw, qb, kb}, c, false);
+  }
+  auto n = make_node<RotNode>(torch::autograd::collect_next_edges(q, or_undefined(k), or_undefined(qw), or_undefined(kw),
+                                                                  or_undefined(qb), or_undefined(kb)));
+  const OptTensor pos = positions, tu = turns, ax = axis;
+  const OptTensor* ts[9] = {&qo, &k, &pos, &tu, &ax, &qw, &kw, &qb, &kb};
+  for (int i = 0; i < 9; ++i) n->in[i] = saved(*ts[i]);
+  n->c = c;
+  torch::autograd::set_history(o.first, n);
+  if (has(k)) torch::autograd::set_history(o.second, n);
+  return {o.first, opt(o.second)};
 }
 
 std::tuple<Tensor, Tensor> rot_fwd_op(const Tensor& q, const OptTensor& k, const Tensor& positions, const Tensor& turns,
