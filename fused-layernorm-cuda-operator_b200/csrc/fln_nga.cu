@@ -2,8 +2,6 @@
 // and alignment (element loads, the row read once per pass), and the sum of the partial rows.
 // Rows of whole 16-byte vectors that fit a CTA's registers go to fln_nga_rows.cuh.  The formulas
 // stand in fln_nga.cuh.
-#include <stdlib.h>
-
 #include <initializer_list>
 
 #include "fln_nga_rows.cuh"
@@ -274,103 +272,115 @@ __global__ void __launch_bounds__(256) nga_bwd_columns_kernel(const NgaParams p)
 }
 
 // ----------------------------------------------------------------------------------------
-// Sums of the partial rows.  blockIdx.y < groups: the gradients that belong to one group each
-// (dgate of a gate per group, dweight / dbias per group); blockIdx.y == groups: those of the
-// vectors shared by all rows.  32 columns x 16 lanes; lane l adds partial rows l, l + 16, ... and
-// the lanes are added in order.  `rep` partial rows per slot.
+// Sums of the partial rows.  Job y < grouped: the gradients that belong to one group each (dgate of
+// a gate per group, dweight / dbias per group); job y == grouped: those of the vectors shared by all
+// rows.  A CTA takes LANES x (256 / LANES) columns of a job: lane l adds partial rows l, l + LANES,
+// ... of all the sums that the job needs, and the lanes are added in order.  One lane where a group
+// has few partial rows (32 samples x 9 slots of 2048 columns: 16 lanes with a pass per sum took
+// 29 us), 16 where all of them are added for a few hundred columns. 
 // ----------------------------------------------------------------------------------------
-constexpr int kFinalLanes = 16;
-template <typename T>
-__global__ void __launch_bounds__(32 * kFinalLanes) nga_finalize_kernel(const NgaParams p, const NgaGrads g, int rep, int groups) {
+template <typename T, int LANES>
+__global__ void __launch_bounds__(256) nga_finalize_kernel(const NgaParams p, const NgaGrads g, int grouped) {
   constexpr bool EXACT = sizeof(T) == 4;
-  __shared__ float tile[kFinalLanes][33];
-  const int tx = threadIdx.x & 31, lane = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 32 + tx;
+  constexpr int COLS = 256 / LANES;
+  __shared__ float tile[LANES > 1 ? 4 : 1][LANES][LANES > 1 ? COLS + 1 : 1];
+  const int tx = threadIdx.x % COLS, lane = threadIdx.x / COLS;
+  const int64_t c = (int64_t)blockIdx.x * COLS + tx;
   const bool ok = c < p.cols;
-  const int64_t per_group = p.slots_per_group * rep;
+  const int64_t per_group = p.slots_per_group;
   const bool gate_grouped = p.gate_mode == FLN_GATE_GROUP, gate_vec = p.gate_mode == FLN_GATE_VECTOR;
-  // the sum of one accumulator over partial rows [from, to); with `scaled` each partial row is
-  // multiplied by act(gate) of its group first
-  auto total = [&](int which, int64_t from, int64_t to, bool scaled) {
-    const int k = __popc(p.acc & (which - 1));
-    float t = 0.f;
-    if (ok) {
-      const float* src = p.partials + (int64_t)k * p.cols + c;
-      const int64_t pitch = (int64_t)p.nacc * p.cols;
-      if (scaled) {
-        for (int64_t r = from + lane; r < to; r += kFinalLanes) {
-          const float gv = Cvt<T>::to_f(reinterpret_cast<const T*>(p.gate)[(r / per_group) * p.cols + c]);
-          t = fmaf(gate_act<EXACT>(gv, p.act), src[r * pitch], t);
-        }
-      } else {
-        int64_t r = from + lane;
-        for (; r + 7 * kFinalLanes < to; r += 8 * kFinalLanes) {
-          float v[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = __ldcg(src + (r + j * kFinalLanes) * pitch);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) t += v[j];
-        }
-        for (; r < to; r += kFinalLanes) t += __ldcg(src + r * pitch);
-      }
-    }
-    __syncthreads();
-    tile[lane][tx] = t;
-    __syncthreads();
-    t = 0.f;
-#pragma unroll
-    for (int i = 0; i < kFinalLanes; ++i) t += tile[i][tx];
-    return t;
-  };
-  const bool writer = ok && lane == 0;
+  const int64_t pitch = (int64_t)p.nacc * p.cols;
+  const T* gate = reinterpret_cast<const T*>(p.gate);
   auto dgate_of = [&](float P, float Q, int64_t at) {
     float a, da;
-    gate_act_grad<EXACT>(Cvt<T>::to_f(reinterpret_cast<const T*>(p.gate)[at]), p.act, &a, &da);
+    gate_act_grad<EXACT>(Cvt<T>::to_f(gate[at]), p.act, &a, &da);
     float w = 1.f;
     if (p.w1 != nullptr) w = p.woff + Cvt<T>::to_f(reinterpret_cast<const T*>(p.w1)[c]);
     float n = w * P;
     if (p.b1 != nullptr) n = fmaf(Cvt<T>::to_f(reinterpret_cast<const T*>(p.b1)[c]), Q, n);
     reinterpret_cast<T*>(g.dgate)[at] = Cvt<T>::from_f(n * da);
   };
-  for (int64_t y = blockIdx.y; y <= groups; y += gridDim.y) {
-    if (y < groups) {  // one group
-      const int64_t from = y * per_group, to = from + per_group;
+  auto put = [&](void* out, int64_t at, float v) {
+    if (out != nullptr) reinterpret_cast<T*>(out)[at] = Cvt<T>::from_f(v);
+  };
+  const int64_t jobs = p.groups + 1;
+  for (int64_t y = (int64_t)blockIdx.y + (grouped ? 0 : p.groups); y < jobs; y += gridDim.y) {
+    const bool all = y == p.groups;
+    // the sums this job needs (bits as in p.acc), and whether P and Q are weighted with act(gate) of
+    // their group
+    int want = 0;
+    if (all) {
+      if (g.dw1 != nullptr || (gate_vec && g.dgate != nullptr)) want |= kAccP;
+      if (g.db1 != nullptr || (gate_vec && g.dgate != nullptr && p.b1 != nullptr)) want |= kAccQ;
+      if (!p.affine_grouped) want |= (g.dw2 != nullptr ? kAccU : 0) | (g.db2 != nullptr ? kAccV : 0);
+    } else {
+      if (gate_grouped && g.dgate != nullptr) want |= kAccP | (p.b1 != nullptr ? kAccQ : 0);
+      if (p.affine_grouped) want |= (g.dw2 != nullptr ? kAccU : 0) | (g.db2 != nullptr ? kAccV : 0);
+    }
+    if (want == 0) continue;
+    const bool weighted = all && gate_grouped;
+    const int64_t from = all ? 0 : y * per_group, to = all ? p.slots : from + per_group;
+    float t[4] = {0.f, 0.f, 0.f, 0.f};
+    if (ok) {
+      const float* src[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) src[i] = p.partials + (int64_t)__popc(p.acc & ((1 << i) - 1)) * p.cols + c;
+      int64_t r = from + lane;
+      for (; r + 3 * LANES < to; r += 4 * LANES) {
+        float v[4][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[j][i] = (want >> i) & 1 ? __ldcg(src[i] + (r + j * LANES) * pitch) : 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (weighted) {
+            const float a = gate_act<EXACT>(Cvt<T>::to_f(gate[(r + j * LANES) / per_group * p.cols + c]), p.act);
+            v[j][0] *= a;
+            v[j][1] *= a;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) t[i] += v[j][i];
+        }
+      }
+      for (; r < to; r += LANES) {
+        float a = 1.f;
+        if (weighted) a = gate_act<EXACT>(Cvt<T>::to_f(gate[r / per_group * p.cols + c]), p.act);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if ((want >> i) & 1) t[i] = fmaf(i < 2 ? a : 1.f, __ldcg(src[i] + r * pitch), t[i]);
+      }
+    }
+    if (LANES > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tile[i][lane][tx] = t[i];
+      __syncthreads();
+      if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          t[i] = 0.f;
+#pragma unroll
+          for (int l = 0; l < LANES; ++l) t[i] += tile[LANES > 1 ? i : 0][l][LANES > 1 ? tx : 0];
+        }
+      }
+    }
+    if (!ok || lane != 0) continue;
+    if (!all) {
       const int64_t at = y * p.cols + c;
-      if (gate_grouped && g.dgate != nullptr) {
-        const float P = total(kAccP, from, to, false);
-        const float Q = p.b1 != nullptr ? total(kAccQ, from, to, false) : 0.f;
-        if (writer) dgate_of(P, Q, at);
-      }
+      if (gate_grouped && g.dgate != nullptr) dgate_of(t[0], t[1], at);
       if (p.affine_grouped) {
-        if (g.dw2 != nullptr) {
-          const float v = total(kAccU, from, to, false);
-          if (writer) reinterpret_cast<T*>(g.dw2)[at] = Cvt<T>::from_f(v);
-        }
-        if (g.db2 != nullptr) {
-          const float v = total(kAccV, from, to, false);
-          if (writer) reinterpret_cast<T*>(g.db2)[at] = Cvt<T>::from_f(v);
-        }
+        put(g.dw2, at, t[2]);
+        put(g.db2, at, t[3]);
       }
-    } else {  // vectors shared by all rows
-      const int64_t to = p.slots * rep;
-      const float a = gate_vec && ok ? gate_act<EXACT>(Cvt<T>::to_f(reinterpret_cast<const T*>(p.gate)[c]), p.act) : 1.f;
-      float P = 0.f, Q = 0.f;
-      if (g.dw1 != nullptr || (gate_vec && g.dgate != nullptr)) P = total(kAccP, 0, to, gate_grouped);
-      if (g.db1 != nullptr || (gate_vec && g.dgate != nullptr && p.b1 != nullptr)) Q = total(kAccQ, 0, to, gate_grouped);
-      if (writer) {
-        if (g.dw1 != nullptr) reinterpret_cast<T*>(g.dw1)[c] = Cvt<T>::from_f(a * P);
-        if (g.db1 != nullptr) reinterpret_cast<T*>(g.db1)[c] = Cvt<T>::from_f(a * Q);
-        if (gate_vec && g.dgate != nullptr) dgate_of(P, Q, c);
-      }
+    } else {
+      const float a = gate_vec ? gate_act<EXACT>(Cvt<T>::to_f(gate[c]), p.act) : 1.f;
+      put(g.dw1, c, a * t[0]);
+      put(g.db1, c, a * t[1]);
+      if (gate_vec && g.dgate != nullptr) dgate_of(t[0], t[1], c);
       if (!p.affine_grouped) {
-        if (g.dw2 != nullptr) {
-          const float v = total(kAccU, 0, to, false);
-          if (writer) reinterpret_cast<T*>(g.dw2)[c] = Cvt<T>::from_f(v);
-        }
-        if (g.db2 != nullptr) {
-          const float v = total(kAccV, 0, to, false);
-          if (writer) reinterpret_cast<T*>(g.db2)[c] = Cvt<T>::from_f(v);
-        }
+        put(g.dw2, c, t[2]);
+        put(g.db2, c, t[3]);
       }
     }
   }
@@ -444,9 +454,6 @@ static int threads_per_row(int nv, int K) {
 
 static bool row_vectors(const NgaParams& p, int es) { return p.cols % (16 / es) == 0 && p.cols <= (1 << 20); }
 
-// tuning (temporary)
-static int env(const char* n, int d) { const char* v = getenv(n); return v ? atoi(v) : d; }
-
 // rows per CTA: rows of 128 threads and more one at a time, shorter ones until there are 256 threads
 static void rows_per_cta(NgaGeom* g) {
   g->R = g->tpr >= 128 ? 1 : (g->tpr > 32 ? 2 : 256 / g->tpr);
@@ -467,21 +474,27 @@ static int plan_forward(const NgaParams& p, int es, NgaGeom* g) {
   if (threads_per_row(nv, E / vec) > 512) return 0;
   const int K = E / vec;
   g->tpr = threads_per_row(nv, K);
+  if (E == 16 && K * g->tpr != nv && nga_ragged_tpr(g->tpr) != 0) g->tpr = nga_ragged_tpr(g->tpr);
   rows_per_cta(g);
   const int tensors = 1 + (p.res != nullptr) + (p.gate_mode == FLN_GATE_ELEMENT);
-  g->stages = env("NGA_FS", 3);
+  g->stages = 3;
   g->smem = 512 + (size_t)g->stages * tensors * K * g->threads * 16;
   while (g->smem > 220 * 1024) {
     if (--g->stages < 2) return 0;
     g->smem = 512 + (size_t)g->stages * tensors * K * g->threads * 16;
   }
+  // Rows per CTA: about eight row steps, so that a CTA's coefficients and the start of its ring are
+  // paid for, and one wave of CTAs where there are fewer rows than that.  16384 x 8192 bf16: 170 us
+  // with 8 steps, 176 with 16, 182 with 32.  Resident CTAs: some 64 .. 84 registers without biases and
+  // means, up to 119 with them.
   const int64_t groups = p.rows / p.group_rows;
-  const int64_t slots = (int64_t)sm_count() * (768 / g->threads > 0 ? 768 / g->threads : 1);
-  int64_t chunk = p.rows / (slots * env("NGA_FW", 6));
-  const int64_t cap = env("NGA_FC", 16);
-  if (chunk > cap * g->R) chunk = cap * g->R;
-  chunk = (chunk + g->R - 1) / g->R * g->R;
-  if (chunk < g->R) chunk = g->R;
+  int64_t resident = (nga_general(p) ? 512 : 768) / g->threads;
+  const int64_t by_smem = (int64_t)(227 * 1024 / (g->smem + 1024));
+  if (resident > by_smem) resident = by_smem;
+  if (resident < 1) resident = 1;
+  const int64_t slots = (int64_t)sm_count() * resident * g->R, steps = nga_general(p) ? 12 : 8;
+  const int64_t waves = (p.rows + slots * steps - 1) / (slots * steps);
+  int64_t chunk = (p.rows + slots * waves - 1) / (slots * waves) * g->R;
   if (chunk > p.group_rows) chunk = p.group_rows;
   g->per_group = (p.group_rows + chunk - 1) / chunk;
   g->chunk = (p.group_rows + g->per_group - 1) / g->per_group;
@@ -508,27 +521,38 @@ static int plan_backward(NgaParams* p, int es, NgaGeom* g) {
   if (threads_per_row(g->nv, E / vec) > most(E)) return 0;
   const int K = E / vec;
   g->tpr = threads_per_row(g->nv, K);
+  const int set = nga_set_of(*p);
+  if (set == 1 && E == (nga_general(*p) ? 8 : 16) && K * g->tpr != g->nv && nga_ragged_tpr(g->tpr) != 0 && g->tpr > 96)
+    g->tpr = nga_ragged_tpr(g->tpr);
   rows_per_cta(g);
   g->rep = g->tpr < 32 ? g->threads / 32 : g->R;
   const size_t unit = (size_t)K * g->threads * 16;
   int ctas = most(E) / g->threads;
   if (ctas < 1) ctas = 1;
+  // as many CTAs as the registers allow if two rows each fit, else fewer; then dsum past the ring,
+  // then the coefficients out of it, and a ring of one row last
   bool fits = false;
-  for (; ctas >= 1 && !fits; --ctas) {
+  auto fit = [&](int ctas, int csm, int direct, int rows) {
     const size_t per = (size_t)227 * 1024 / ctas - 1024;  // the runtime keeps 1 KB of every CTA
-    for (int csm = 1; csm >= 0 && !fits; --csm) {
-      const NgaBwdLayout l = nga_bwd_layout(*p, es, csm != 0, nga_general(*p));
-      const size_t fixed = kNgaBwdHeader + (size_t)l.coefs * unit, stage = (size_t)l.tensors * unit;
-      if (fixed + 2 * stage > per) continue;
-      int s = (int)((per - fixed) / stage);
-      const int cap = env("NGA_BS", 4);
-      if (s > cap) s = cap;
-      g->csm = csm;
-      g->stages = s;
-      g->smem = fixed + (size_t)s * stage;
-      fits = true;
-    }
+    const NgaBwdLayout l = nga_bwd_layout(*p, es, csm != 0, nga_general(*p), direct != 0);
+    const size_t joint = g->rep > 1 ? (size_t)g->rep * g->tpr * vec * 4 : 0;
+    const size_t fixed = kNgaBwdHeader + (size_t)l.coefs * unit + joint, stage = (size_t)l.tensors * unit;
+    if (fixed + rows * stage > per) return false;
+    int s = (int)((per - fixed) / stage);
+    if (s > 3) s = 3;
+    g->csm = csm;
+    g->direct = direct;
+    g->stages = s;
+    g->smem = fixed + (size_t)s * stage;
+    return true;
+  };
+  for (; ctas >= 1 && !fits; --ctas) {
+    fits = fit(ctas, 1, 0, 2);
     if (fits) break;
+  }
+  if (!fits) {
+    ctas = 1;
+    fits = (set == 1 && fit(1, 1, 1, 2)) || fit(1, 0, 0, 2) || (set == 1 && fit(1, 0, 1, 2)) || fit(1, 1, 0, 1) || fit(1, 0, 0, 1);
   }
   if (!fits) return 0;
   // Slots: as many per group as give every CTA the same number of row steps, nearly; a slot's own
@@ -562,10 +586,18 @@ static int plan_backward(NgaParams* p, int es, NgaGeom* g) {
 static size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 template <typename T>
-static int finalize(const NgaParams& p, const NgaGrads& g, int rep, cudaStream_t st) {
-  const int64_t groups = p.rows / p.group_rows;
-  const dim3 fg((unsigned)((p.cols + 31) / 32), (unsigned)(groups + 1 < 65535 ? groups + 1 : 65535));
-  nga_finalize_kernel<T><<<fg, 32 * kFinalLanes, 0, st>>>(p, g, rep, (int)groups);
+static int finalize(NgaParams p, const NgaGrads& g, cudaStream_t st) {
+  p.groups = p.rows / p.group_rows;
+  const bool grouped = (p.gate_mode == FLN_GATE_GROUP && g.dgate != nullptr) ||
+                       (p.affine_grouped && (g.dw2 != nullptr || g.db2 != nullptr));
+  const bool shared = g.dw1 != nullptr || g.db1 != nullptr || (p.gate_mode == FLN_GATE_VECTOR && g.dgate != nullptr) ||
+                      (!p.affine_grouped && (g.dw2 != nullptr || g.db2 != nullptr));
+  // 16 lanes wherever the shared vectors are among the outputs or a group has many partial rows
+  const bool wide = shared || p.slots_per_group > 32;
+  const int64_t jobs = grouped ? p.groups + (shared ? 1 : 0) : 1;
+  const dim3 grid((unsigned)((p.cols + (wide ? 16 : 256) - 1) / (wide ? 16 : 256)), (unsigned)(jobs < 65535 ? jobs : 65535));
+  if (wide) nga_finalize_kernel<T, 16><<<grid, 256, 0, st>>>(p, g, grouped ? 1 : 0);
+  else nga_finalize_kernel<T, 1><<<grid, 256, 0, st>>>(p, g, grouped ? 1 : 0);
   FLN_CHECK_LAUNCH();
   return FLN_OK;
 }
@@ -580,7 +612,7 @@ static int run_backward(NgaParams p, const NgaGrads& g, bool aligned, cudaStream
       q.partials = p.row_c;  // the whole workspace: the row scalars are not kept
       const int rc = nga_bwd_rows<T>(q, geom, K, st);
       if (rc != FLN_OK || q.acc == 0) return rc;
-      return finalize<T>(q, g, geom.rep, st);
+      return finalize<T>(q, g, st);
     }
   }
   plan_slots(&p);
@@ -591,7 +623,7 @@ static int run_backward(NgaParams p, const NgaGrads& g, bool aligned, cudaStream
     const dim3 cg((unsigned)((p.cols + 31) / 32), (unsigned)(p.slots < 65535 ? p.slots : 65535));
     nga_bwd_columns_kernel<T><<<cg, 256, 0, st>>>(p);
     FLN_CHECK_LAUNCH();
-    return finalize<T>(p, g, 1, st);
+    return finalize<T>(p, g, st);
   }
   return FLN_OK;
 }
@@ -675,7 +707,7 @@ extern "C" size_t fln_norm_gate_add_norm_workspace_bytes(const fln_nga_args* a) 
       q.dy = (grads & 1) != 0 && a->kind != FLN_NO_NORM ? a->x : nullptr;
       q.ds = (grads & 2) != 0 ? a->x : nullptr;
       if (plan_backward(&q, a->dtype == FLN_F32 ? 4 : 2, &g) == 0) continue;
-      const size_t n = (size_t)q.slots * g.rep * row;
+      const size_t n = (size_t)q.slots * row;
       if (n > most) most = n;
     }
   }

@@ -65,6 +65,7 @@ struct NgaParams {
   int64_t chunk;           // rows per slot
   int64_t slots_per_group;
   int64_t slots;
+  int64_t groups;  // set for the last kernel
 };
 constexpr int kAccP = 1, kAccQ = 2, kAccU = 4, kAccV = 8;
 
@@ -72,7 +73,7 @@ constexpr int kAccP = 1, kAccQ = 2, kAccU = 4, kAccV = 8;
 // exponential and reciprocal, relative error about 2^-21, far below the type's 2^-9.
 template <bool EXACT>
 __device__ __forceinline__ float sigmoid_of(float v) {
-  if (EXACT) return 1.0f / (1.0f + expf(-v));
+  if (EXACT) return rcp_approx(1.0f + expf(-v));  // (the reciprocal is good to one unit in the last place)
   return rcp_approx(1.0f + ex2_approx(-1.4426950408889634f * v));
 }
 template <bool EXACT>

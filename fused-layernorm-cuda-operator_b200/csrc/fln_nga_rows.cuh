@@ -33,16 +33,18 @@ struct NgaGeom {
   int nv;       // vectors per row
   int threads;  // per CTA: R * tpr
   int stages;   // backward: rows on their way per row group
-  int rep;      // backward: partial rows a CTA leaves per slot
+  int rep;      // backward: row groups (or warps of several) whose sums a CTA joins
   int64_t grid;
   size_t smem;
   int csm;      // backward: coefficients in shared memory
+  int direct;   // backward: dsum past the ring
   int64_t chunk, per_group;  // forward: rows per CTA, CTAs per group
 };
 
-// Rows per CTA where the threads per row are known at compile time (TPR != 0: the row is whole,
-// cols == TPR * K * vector; every offset is then a constant): 48 -> 34 -> xx instructions per
-// element of the bf16 forward at 4096 columns.
+// Where the threads per row are known at compile time (TPR != 0) every offset in shared memory and
+// between a thread's vectors is a constant, and where the row is whole as well (cols == TPR * K *
+// vector, !RAG) nothing is predicated: 34 -> 22 instructions per element of the bf16 forward at
+// 4096 columns, 51 -> 28 of the backward.  Rows per CTA of these:
 __host__ __device__ constexpr int fixed_rows(int tpr) { return tpr >= 128 ? 1 : (tpr > 32 ? 2 : 256 / tpr); }
 
 // ----------------------------------------------------------------------------------------
@@ -57,7 +59,7 @@ struct RowGroup {
   float2* red; // [2 buffers][32 warps]
   int flip;
 };
-template <int TPR>
+template <int TPR, bool FULL>
 __device__ __forceinline__ RowGroup row_group(const NgaGeom& g, int K, int vec, float2* red) {
   RowGroup r;
   const int tpr = TPR ? TPR : g.tpr;
@@ -67,10 +69,10 @@ __device__ __forceinline__ RowGroup row_group(const NgaGeom& g, int K, int vec, 
   r.red = red;
   r.flip = 0;
   auto count = [&](int w) {  // elements of the row in its warp w
-    if (TPR) return (float)(K * 32 * vec);
+    if (FULL) return (float)(K * 32 * vec);
     int n = 0;
     for (int k = 0; k < K; ++k) {
-      int left = g.nv - (k * g.tpr + w * 32);
+      int left = g.nv - (k * tpr + w * 32);
       left = left < 0 ? 0 : (left > 32 ? 32 : left);
       n += left;
     }
@@ -187,10 +189,10 @@ __device__ __forceinline__ void cp_async16(void* smem, const void* src) {
                : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void cp_async_wait_behind(int ahead) {  // at most `ahead` groups still on their way
+__device__ __forceinline__ void cp_async_wait_behind(int ahead) {  // at most `ahead` groups (0, 1, 2) still on their way
   if (ahead == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
   else if (ahead == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
-  else asm volatile("cp.async.wait_group 3;" ::: "memory");
+  else asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 // v, or zeros (not v times zero, which would be NaN where v is infinite)
 __device__ __forceinline__ float2 f2only(bool on, float2 v) { return make_float2(on ? v.x : 0.f, on ? v.y : 0.f); }
@@ -267,17 +269,17 @@ __device__ __forceinline__ void coef2(const NgaParams& p, int64_t at, float2 (&c
 // GATE 0: none, 1: shared by rows, 2: an element each.  HOLD: the coefficients stay in registers
 // over the chunk, else they are made again for every row (rows too long for that).
 // ----------------------------------------------------------------------------------------
-template <typename T, int K, int GATE, bool GEN, bool HOLD, int TPR>
+template <typename T, int K, int GATE, bool GEN, bool HOLD, int TPR, bool RAG>
 __global__ void __launch_bounds__(512) nga_fwd_rows_kernel(const NgaParams p, const NgaGeom g) {
   constexpr bool EXACT = sizeof(T) == 4;
   constexpr int VEC = 16 / (int)sizeof(T), V2 = VEC / 2;
   extern __shared__ __align__(128) unsigned char smem[];
-  constexpr bool FULL = TPR != 0;
-  const int tpr = FULL ? TPR : g.tpr;
-  const int R = FULL ? fixed_rows(TPR) : g.R;
-  const int threads = FULL ? TPR * fixed_rows(TPR) : g.threads;
+  constexpr bool FULL = TPR != 0 && !RAG;
+  const int tpr = TPR ? TPR : g.tpr;
+  const int R = TPR ? fixed_rows(TPR) : g.R;
+  const int threads = TPR ? TPR * fixed_rows(TPR) : g.threads;
   const int cols = FULL ? TPR * K * VEC : p.cols;
-  RowGroup rg = row_group<TPR>(g, K, VEC, reinterpret_cast<float2*>(smem));
+  RowGroup rg = row_group<TPR, FULL>(g, K, VEC, reinterpret_cast<float2*>(smem));
   const int tid = threadIdx.x;
   const int r_in = tid / tpr, lane = tid - r_in * tpr;
   const float inv_n = 1.0f / (float)cols;
@@ -420,7 +422,8 @@ __global__ void __launch_bounds__(512) nga_fwd_rows_kernel(const NgaParams p, co
 // backward: persistent CTAs; CTA b takes slots b, b + grid, ...  Rows are staged as in the forward,
 // the column sums stay in registers over a slot.  CSM: the coefficients lie in shared memory, in 32
 // bits, each thread's own; else (no room) they are made again where they are used.
-// SET: which tensors there are, 1: x, residual, dy and dsum, 2: x and dsum, 0: found out at run time.
+// SET: which tensors there are, 1: x, residual, dy and dsum, 2: x and dsum, 0: found out at run time;
+// 3: like 1, dsum fetched into registers (rows whose ring would not fit otherwise).
 // ----------------------------------------------------------------------------------------
 constexpr int kNgaBwdHeader = 512;
 
@@ -457,8 +460,8 @@ __host__ __device__ constexpr NgaBwdLayout nga_layout(int es, bool csm, bool bia
   return l;
 }
 // (GEN kernels keep a place for B1 whether there is one or not)
-inline __host__ __device__ NgaBwdLayout nga_bwd_layout(const NgaParams& p, int es, bool csm, bool gen) {
-  return nga_layout(es, csm, gen, p.res != nullptr && p.dy != nullptr, p.dy != nullptr, p.ds != nullptr,
+inline NgaBwdLayout nga_bwd_layout(const NgaParams& p, int es, bool csm, bool gen, bool direct) {
+  return nga_layout(es, csm, gen, p.res != nullptr && p.dy != nullptr, p.dy != nullptr, p.ds != nullptr && !direct,
                     p.gate_mode == FLN_GATE_ELEMENT);
 }
 inline int nga_set_of(const NgaParams& p) {
@@ -467,22 +470,23 @@ inline int nga_set_of(const NgaParams& p) {
   return 0;
 }
 
-template <typename T, int K, int GATE, bool GEN, bool CSM, int TPR, int SET>
+template <typename T, int K, int GATE, bool GEN, bool CSM, int TPR, bool RAG, int SET>
 __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_bwd_rows_kernel(const NgaParams p, const NgaGeom g) {
   constexpr bool EXACT = sizeof(T) == 4;
   constexpr int VEC = 16 / (int)sizeof(T), V2 = VEC / 2;
   extern __shared__ __align__(128) unsigned char smem[];
-  const bool has_dy = SET == 1 || (SET == 0 && p.dy != nullptr);
+  constexpr bool DIRECT = SET == 3;
+  const bool has_dy = SET == 1 || DIRECT || (SET == 0 && p.dy != nullptr);
   const bool has_ds = SET != 0 || p.ds != nullptr;
-  const bool has_res = SET == 1 || (SET == 0 && has_dy && p.res != nullptr);
-  const NgaBwdLayout l = nga_layout((int)sizeof(T), CSM, GEN, has_res, has_dy, has_ds, GATE == 2);
-  constexpr bool FULL = TPR != 0;
-  const int tpr = FULL ? TPR : g.tpr;
-  const int R = FULL ? fixed_rows(TPR) : g.R;
-  const int threads = FULL ? TPR * fixed_rows(TPR) : g.threads;
+  const bool has_res = SET == 1 || DIRECT || (SET == 0 && has_dy && p.res != nullptr);
+  const NgaBwdLayout l = nga_layout((int)sizeof(T), CSM, GEN, has_res, has_dy, has_ds && !DIRECT, GATE == 2);
+  constexpr bool FULL = TPR != 0 && !RAG;
+  const int tpr = TPR ? TPR : g.tpr;
+  const int R = TPR ? fixed_rows(TPR) : g.R;
+  const int threads = TPR ? TPR * fixed_rows(TPR) : g.threads;
   const int cols = FULL ? TPR * K * VEC : p.cols;
-  constexpr bool ONE = FULL && fixed_rows(FULL ? TPR : 1) == 1;  // one row at a time: never behind the slot
-  RowGroup rg = row_group<TPR>(g, K, VEC, reinterpret_cast<float2*>(smem));
+  constexpr bool ONE = TPR != 0 && fixed_rows(TPR ? TPR : 1) == 1;  // one row at a time: never behind the slot
+  RowGroup rg = row_group<TPR, FULL>(g, K, VEC, reinterpret_cast<float2*>(smem));
   const int tid = threadIdx.x;
   const int r_in = ONE ? 0 : tid / tpr, lane = tid - r_in * tpr;
   const float inv_n = 1.0f / (float)cols;
@@ -536,7 +540,7 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
         cp_async16(d, reinterpret_cast<const T*>(p.x) + o);
         if (has_res) cp_async16(d + l.res * unit, reinterpret_cast<const T*>(p.res) + o);
         if (has_dy) cp_async16(d + l.dy * unit, reinterpret_cast<const T*>(p.dy) + o);
-        if (has_ds) cp_async16(d + l.ds * unit, reinterpret_cast<const T*>(p.ds) + o);
+        if (has_ds && !DIRECT) cp_async16(d + l.ds * unit, reinterpret_cast<const T*>(p.ds) + o);
         if (GATE == 2) cp_async16(d + l.gate * unit, reinterpret_cast<const T*>(p.gate) + o);
       }
       step(ahead);
@@ -643,6 +647,11 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
     drain += stage_bytes;
     if (drain == ring_bytes) drain = 0;
 
+    Pack<T, VEC> ds_now[DIRECT ? K : 1];
+    if (DIRECT) {  // used behind the first row sum
+#pragma unroll
+      for (int k = 0; k < K; ++k) ds_now[DIRECT ? k : 0] = ld_stream<T, VEC>(reinterpret_cast<const T*>(p.ds) + base + col[k]);
+    }
     float2 xh[K][V2], sh[K][V2], g2[K][V2];
     float2 r0 = f2(0.f), r1 = f2(0.f);
     {
@@ -709,7 +718,9 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
         const bool ok = live && vok[k];
         const unsigned char* st_k = st + k * kstep;
         float2 d[V2], c[V2], b[V2];
-        if (has_ds) {
+        if (DIRECT) {
+          unpack2<T, VEC>(ds_now[DIRECT ? k : 0], d);
+        } else if (has_ds) {
           take<T>(st_k + l.ds * unit, d);
         } else {
 #pragma unroll
@@ -788,32 +799,48 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
       }
     }
     if (opened) {
-      // the slot's sums: one partial row per row group, or per warp where a warp holds several
+      // the slot's sums; several row groups are joined in the CTA first, in their order
       if (p.acc != 0) {
         const int who = tpr < 32 ? tid >> 5 : r_in;
-        float* out = p.partials + ((int64_t)slot * g.rep + who) * (int64_t)p.nacc * cols;
-        auto leave = [&](float2 (&acc)[V2], int k, int which, float scale) {
+        float* out = p.partials + (int64_t)slot * p.nacc * cols;
+        float* joint = reinterpret_cast<float*>(smem + kNgaBwdHeader + (uint32_t)l.coefs * unit + ring_bytes);
+        auto leave = [&](float2 (&acc)[K][V2], int which, float scale) {
           if (!(p.acc & which)) return;
-          for (int off = 16; off >= tpr; off >>= 1) {
+          float* dst = out + (int64_t)__popc(p.acc & (which - 1)) * cols;
 #pragma unroll
-            for (int e = 0; e < V2; ++e) {
-              acc[e].x += __shfl_xor_sync(0xffffffffu, acc[e].x, off);
-              acc[e].y += __shfl_xor_sync(0xffffffffu, acc[e].y, off);
+          for (int k = 0; k < K; ++k) {
+            for (int off = 16; off >= tpr; off >>= 1) {
+#pragma unroll
+              for (int e = 0; e < V2; ++e) {
+                acc[k][e].x += __shfl_xor_sync(0xffffffffu, acc[k][e].x, off);
+                acc[k][e].y += __shfl_xor_sync(0xffffffffu, acc[k][e].y, off);
+              }
+            }
+            const bool mine = vok[k] && (tpr >= 32 || (tid & 31) < tpr);
+            const bool join = !ONE && g.rep > 1;
+            float* q = join ? joint + (who * tpr + lane) * VEC : dst + col[k];
+            if (mine || join) {
+#pragma unroll
+              for (int e = 0; e < V2; e += 2)
+                *reinterpret_cast<float4*>(q + 2 * e) =
+                    make_float4(acc[k][e].x * scale, acc[k][e].y * scale, acc[k][e + 1].x * scale, acc[k][e + 1].y * scale);
+            }
+            if (join) {
+              __syncthreads();
+              for (int i = tid; i < tpr * VEC; i += threads) {
+                float v = 0.f;
+                for (int r = 0; r < g.rep; ++r) v += joint[r * tpr * VEC + i];
+                if (k * tpr * VEC + i < cols) dst[k * tpr * VEC + i] = v;
+              }
+              __syncthreads();
             }
           }
-          if (!vok[k] || (tpr < 32 && (tid & 31) >= tpr)) return;
-          float* q = out + (int64_t)__popc(p.acc & (which - 1)) * cols + col[k];
-#pragma unroll
-          for (int e = 0; e < V2; e += 2)
-            *reinterpret_cast<float4*>(q + 2 * e) =
-                make_float4(acc[e].x * scale, acc[e].y * scale, acc[e + 1].x * scale, acc[e + 1].y * scale);
         };
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-          leave(acc_p[k], k, kAccP, p.ba);
-          if (GEN) leave(acc_q[GEN ? k : 0], k, kAccQ, p.ba);
-          leave(acc_u[k], k, kAccU, 1.f);
-          if (GEN) leave(acc_v[GEN ? k : 0], k, kAccV, 1.f);
+        leave(acc_p, kAccP, p.ba);
+        leave(acc_u, kAccU, 1.f);
+        if constexpr (GEN) {
+          leave(acc_q, kAccQ, p.ba);
+          leave(acc_v, kAccV, 1.f);
         }
       }
       clear();
@@ -846,62 +873,95 @@ static int nga_launch(F kern, const NgaParams& p, const NgaGeom& g, cudaStream_t
   FLN_CHECK_LAUNCH();
   return FLN_OK;
 }
-// the compile-time rows: 16 elements per thread, 128 to 8192 columns (powers of two)
-template <typename T, int K, int GATE, int TPR>
+// Threads per row of the compile-time kernels for rows that are not whole: the next of these where
+// that leaves at most a sixth of the threads idle, else 0 (everything found out at run time).
+inline int nga_ragged_tpr(int tpr) {
+  const int list[] = {128, 192, 256, 320, 384, 512};
+  for (int t : list)
+    if (t >= tpr && (t - tpr) * 6 <= t) return t;
+  return 0;
+}
+template <typename T, int K, int GATE, int TPR, bool RAG>
 static int nga_fwd_rows_t(const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
   constexpr bool HOLD = K * 16 / (int)sizeof(T) <= 16;
-  return nga_general(p) ? nga_launch(nga_fwd_rows_kernel<T, K, GATE, true, HOLD, TPR>, p, g, st)
-                        : nga_launch(nga_fwd_rows_kernel<T, K, GATE, false, HOLD, TPR>, p, g, st);
+  return nga_general(p) ? nga_launch(nga_fwd_rows_kernel<T, K, GATE, true, HOLD, TPR, RAG>, p, g, st)
+                        : nga_launch(nga_fwd_rows_kernel<T, K, GATE, false, HOLD, TPR, RAG>, p, g, st);
 }
 template <typename T, int K, int GATE>
 static int nga_fwd_rows_k(const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
+  // compile-time rows: 16 elements per thread
   if constexpr (K * 16 / (int)sizeof(T) == 16) {
     if (g.nv == K * g.tpr) {
       switch (g.tpr) {
         case 8:
-          return nga_fwd_rows_t<T, K, GATE, 8>(p, g, st);
+          return nga_fwd_rows_t<T, K, GATE, 8, false>(p, g, st);
         case 64:
-          return nga_fwd_rows_t<T, K, GATE, 64>(p, g, st);
+          return nga_fwd_rows_t<T, K, GATE, 64, false>(p, g, st);
         case 128:
-          return nga_fwd_rows_t<T, K, GATE, 128>(p, g, st);
+          return nga_fwd_rows_t<T, K, GATE, 128, false>(p, g, st);
         case 256:
-          return nga_fwd_rows_t<T, K, GATE, 256>(p, g, st);
+          return nga_fwd_rows_t<T, K, GATE, 256, false>(p, g, st);
         case 512:
-          return nga_fwd_rows_t<T, K, GATE, 512>(p, g, st);
+          return nga_fwd_rows_t<T, K, GATE, 512, false>(p, g, st);
       }
     }
+    switch (g.tpr) {
+      case 128:
+        return nga_fwd_rows_t<T, K, GATE, 128, true>(p, g, st);
+      case 192:
+        return nga_fwd_rows_t<T, K, GATE, 192, true>(p, g, st);
+      case 256:
+        return nga_fwd_rows_t<T, K, GATE, 256, true>(p, g, st);
+      case 320:
+        return nga_fwd_rows_t<T, K, GATE, 320, true>(p, g, st);
+      case 384:
+        return nga_fwd_rows_t<T, K, GATE, 384, true>(p, g, st);
+      case 512:
+        return nga_fwd_rows_t<T, K, GATE, 512, true>(p, g, st);
+    }
   }
-  return nga_fwd_rows_t<T, K, GATE, 0>(p, g, st);
+  return nga_fwd_rows_t<T, K, GATE, 0, false>(p, g, st);
 }
 template <typename T, int K, int GATE, bool GEN>
 static int nga_bwd_rows_g(const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
+  if (g.direct)
+    return g.csm ? nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 3>, p, g, st)
+                 : nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, false, 0, false, 3>, p, g, st);
+  if (!g.csm) return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, false, 0, false, 0>, p, g, st);
   const int set = nga_set_of(p);
-  if (!g.csm) return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, false, 0, 0>, p, g, st);
   // compile-time rows where the registers allow: 16 elements per thread, 8 of the general form
   if constexpr (K * 16 / (int)sizeof(T) == (GEN ? 8 : 16)) {
+#define FLN_NGA_BWD(TPR, RAG, SET) \
+  case TPR:                        \
+    return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, TPR, RAG, SET>, p, g, st);
     if (g.nv == K * g.tpr && set == 1) {
       switch (g.tpr) {
-        case 64:
-          return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 64, 1>, p, g, st);
-        case 128:
-          return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 128, 1>, p, g, st);
-        case 256:
-          return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 256, 1>, p, g, st);
-        case 512:
-          return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 512, 1>, p, g, st);
+        FLN_NGA_BWD(64, false, 1)
+        FLN_NGA_BWD(128, false, 1)
+        FLN_NGA_BWD(256, false, 1)
+        FLN_NGA_BWD(512, false, 1)
       }
     }
     if (g.nv == K * g.tpr && set == 2) {
       switch (g.tpr) {
-        case 8:
-          return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 8, 2>, p, g, st);
-        case 16:
-          return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 16, 2>, p, g, st);
+        FLN_NGA_BWD(8, false, 2)
+        FLN_NGA_BWD(16, false, 2)
       }
     }
+    if (set == 1) {
+      switch (g.tpr) {
+        FLN_NGA_BWD(128, true, 1)
+        FLN_NGA_BWD(192, true, 1)
+        FLN_NGA_BWD(256, true, 1)
+        FLN_NGA_BWD(320, true, 1)
+        FLN_NGA_BWD(384, true, 1)
+        FLN_NGA_BWD(512, true, 1)
+      }
+    }
+#undef FLN_NGA_BWD
   }
-  if (set == 1) return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, 1>, p, g, st);
-  return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, 0>, p, g, st);
+  if (set == 1) return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 1>, p, g, st);
+  return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 0>, p, g, st);
 }
 template <typename T, int K, int GATE>
 static int nga_bwd_rows_k(const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
