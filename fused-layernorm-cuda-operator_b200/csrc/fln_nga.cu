@@ -433,6 +433,7 @@ static NgaParams base_params(const fln_nga_args* a) {
 
 // Slots of the loop kernels: 64 rows, more when that would make over a thousand of them.
 static void plan_slots(NgaParams* p) {
+  p->period = 1;
   const int64_t groups = p->rows / p->group_rows;
   int64_t most = 1024 / groups;
   if (most < 1) most = 1;
@@ -452,7 +453,29 @@ static int threads_per_row(int nv, int K) {
   return w;
 }
 
-static bool row_vectors(const NgaParams& p, int es) { return p.cols % (16 / es) == 0 && p.cols <= (1 << 20); }
+// Places of a 16-byte vector that the rows start at in turn, and with them p's classes.
+static bool row_vectors(NgaParams* p, int es) {
+  if (p->cols > (1 << 20)) return false;
+  const int vec = 16 / es;
+  p->period = vec;
+  for (int c = p->cols; p->period > 1 && c % 2 == 0; c /= 2) p->period /= 2;
+  p->classes = p->group_rows < p->period ? (int)p->group_rows : p->period;
+  p->pieces = 1;
+  return true;
+}
+// Cuts every class of a group into about `want` slots, none of them empty.
+static void cut_classes(NgaParams* p, int64_t want) {
+  const int64_t most = p->group_rows / p->period;
+  p->pieces = want > most ? most : want;
+  if (p->pieces < 1) p->pieces = 1;
+  p->slots_per_group = p->classes * p->pieces;
+  p->slots = p->slots_per_group * (p->rows / p->group_rows);
+}
+// vectors that cover a row, wherever it starts
+static int row_vector_count(const NgaParams& p, int es) {
+  const int vec = 16 / es;
+  return p.period == 1 ? p.cols / vec : (p.cols + 2 * (vec - 1)) / vec;
+}
 
 // rows per CTA: rows of 128 threads and more one at a time, shorter ones until there are 256 threads
 static void rows_per_cta(NgaGeom* g) {
@@ -461,9 +484,10 @@ static void rows_per_cta(NgaGeom* g) {
 }
 
 // The forward's plan.  K = 0: not for the row kernels.
-static int plan_forward(const NgaParams& p, int es, NgaGeom* g) {
-  if (!row_vectors(p, es)) return 0;
-  const int nv = p.cols * es / 16, vec = 16 / es;
+static int plan_forward(NgaParams* pp, int es, NgaGeom* g) {
+  if (!row_vectors(pp, es)) return 0;
+  const NgaParams& p = *pp;
+  const int nv = row_vector_count(p, es), vec = 16 / es;
   g->nv = nv;
   int E = 16;  // elements per thread
   int fK = 0, ftpr = 0;
@@ -474,7 +498,7 @@ static int plan_forward(const NgaParams& p, int es, NgaGeom* g) {
   if (threads_per_row(nv, E / vec) > 512) return 0;
   const int K = E / vec;
   g->tpr = threads_per_row(nv, K);
-  if (E == 16 && K * g->tpr != nv && nga_ragged_tpr(g->tpr) != 0) g->tpr = nga_ragged_tpr(g->tpr);
+  if (p.period == 1 && E == 16 && K * g->tpr != nv && nga_ragged_tpr(g->tpr) != 0) g->tpr = nga_ragged_tpr(g->tpr);
   rows_per_cta(g);
   const int tensors = 1 + (p.res != nullptr) + (p.gate_mode == FLN_GATE_ELEMENT);
   g->stages = 3;
@@ -500,6 +524,10 @@ static int plan_forward(const NgaParams& p, int es, NgaGeom* g) {
   g->chunk = (p.group_rows + g->per_group - 1) / g->per_group;
   g->chunk = (g->chunk + g->R - 1) / g->R * g->R;
   g->per_group = (p.group_rows + g->chunk - 1) / g->chunk;
+  if (p.period > 1) {
+    cut_classes(pp, (g->per_group + p.period - 1) / p.period);
+    g->per_group = p.slots_per_group;
+  }
   g->grid = g->per_group * groups;
   if (g->grid > 0x7fffffff) return 0;
   return K;
@@ -509,9 +537,9 @@ static int plan_forward(const NgaParams& p, int es, NgaGeom* g) {
 // kernels' registers allow (640 with 8 elements per thread, 512 with 16), at least two rows on
 // their way per row group.  Fills p's slots.  K = 0: not for the row kernels.
 static int plan_backward(NgaParams* p, int es, NgaGeom* g) {
-  if (!row_vectors(*p, es)) return 0;
+  if (!row_vectors(p, es)) return 0;
   const int vec = 16 / es;
-  g->nv = p->cols * es / 16;
+  g->nv = row_vector_count(*p, es);
   auto most = [&](int e) { return e <= 8 ? 640 : 512; };
   int E = nga_general(*p) ? 8 : 16;
   int fK = 0, ftpr = 0;
@@ -521,7 +549,7 @@ static int plan_backward(NgaParams* p, int es, NgaGeom* g) {
   if (threads_per_row(g->nv, E / vec) > most(E)) return 0;
   const int K = E / vec;
   g->tpr = threads_per_row(g->nv, K);
-  const int set = nga_set_of(*p);
+  const int set = p->period == 1 ? nga_set_of(*p) : 0;  // (0: dsum never past the ring)
   if (set == 1 && E == (nga_general(*p) ? 8 : 16) && K * g->tpr != g->nv && nga_ragged_tpr(g->tpr) != 0 && g->tpr > 96)
     g->tpr = nga_ragged_tpr(g->tpr);
   rows_per_cta(g);
@@ -560,6 +588,11 @@ static int plan_backward(NgaParams* p, int es, NgaGeom* g) {
   const int64_t groups = p->rows / p->group_rows, T = p->group_rows;
   const int64_t slots_max = (T + g->R - 1) / g->R;
   const int64_t cta = (int64_t)usable_sms() * ctas;
+  if (p->period > 1) {
+    cut_classes(p, (cta + groups * p->classes - 1) / (groups * p->classes));
+    g->grid = p->slots < cta ? p->slots : cta;
+    return p->slots > 0x7fffffff - g->grid ? 0 : K;
+  }
   int64_t best = -1, best_cost = 0;
   auto consider = [&](int64_t spg) {
     if (spg < 1) spg = 1;
@@ -668,7 +701,7 @@ extern "C" int fln_norm_gate_add_norm_forward(const fln_nga_args* a, void* y, vo
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (all_aligned({a->x, a->residual, a->gate, a->post_weight, a->post_bias, a->weight, a->bias, y, sum})) {
     NgaGeom g = {};
-    const int K = plan_forward(p, a->dtype == FLN_F32 ? 4 : 2, &g);
+    const int K = plan_forward(&p, a->dtype == FLN_F32 ? 4 : 2, &g);
     if (K != 0) {
       if (a->dtype == FLN_F32) return nga_fwd_rows<float>(p, g, K, st);
       if (a->dtype == FLN_BF16) return nga_fwd_rows<__nv_bfloat16>(p, g, K, st);

@@ -66,6 +66,11 @@ struct NgaParams {
   int64_t slots_per_group;
   int64_t slots;
   int64_t groups;  // set for the last kernel
+  // Rows that are not whole 16-byte vectors start at one of `period` places of a vector in turn.  A
+  // slot then holds rows of one such class (every period-th row of the group), `classes` of them per
+  // group, cut into `pieces` slots each.  period 1: whole vectors, slots of `chunk` rows.
+  int period, classes;
+  int64_t pieces;
 };
 constexpr int kAccP = 1, kAccQ = 2, kAccU = 4, kAccV = 8;
 
@@ -131,13 +136,20 @@ __device__ __forceinline__ void cta_sum(float (&v)[NV], float* red, int& flip) {
 
 // the rows of slot `slot`
 struct SlotRows {
-  int64_t group, first, last;  // rows [first, last)
+  int64_t group, first, last;  // rows first, first + p.period, ... below last; last - 1 is one of them
 };
 __device__ __forceinline__ SlotRows slot_rows(const NgaParams& p, int64_t slot) {
   SlotRows s;
   s.group = slot / p.slots_per_group;
   const int64_t j = slot - s.group * p.slots_per_group;
   const int64_t g0 = s.group * p.group_rows;
+  if (p.period > 1) {
+    const int64_t c = j % p.classes, piece = j / p.classes;
+    const int64_t n = (p.group_rows - c + p.period - 1) / p.period;  // rows of the class, at least `pieces`
+    s.first = g0 + c + piece * n / p.pieces * p.period;
+    s.last = g0 + c + ((piece + 1) * n / p.pieces - 1) * p.period + 1;
+    return s;
+  }
   s.first = g0 + j * p.chunk;
   s.last = s.first + p.chunk < g0 + p.group_rows ? s.first + p.chunk : g0 + p.group_rows;
   return s;

@@ -19,6 +19,14 @@
 // The unfolded form on single floats took 48 (forward) and 84 (backward) instructions per element
 // at 16384 x 4096 bf16: 127 and 248 us.
 //
+// SHIFT: rows that are not whole 16-byte vectors (tensors that start on a 16-byte boundary, row length
+// not a multiple of a vector).  Such a row starts at one of 2, 4 or 8 places of a vector, by its
+// number; a CTA takes rows of one class at a time (fln_nga.cuh), for which a column always lies at
+// the same place of the same thread's vectors.  So all that is above holds: the row is staged as
+// the vectors that cover it, what belongs to the neighbouring rows in its first and last vector is
+// set to zero, and only those two are stored element by element.  (Rows held element by element
+// instead: 16384 x 2777 bf16 at 190 us forward and 546 us backward.)
+//
 // GEN = false: both norms RMSNorm or none and no bias, which is what most blocks have; no means, no
 // Q and V.  GEN = true: everything.
 #pragma once
@@ -59,8 +67,9 @@ struct RowGroup {
   float2* red; // [2 buffers][32 warps]
   int flip;
 };
+// (the row lies at elements [shift, shift + cols) of its nv vectors)
 template <int TPR, bool FULL>
-__device__ __forceinline__ RowGroup row_group(const NgaGeom& g, int K, int vec, float2* red) {
+__device__ __forceinline__ RowGroup row_group(const NgaGeom& g, int K, int vec, int nv, int shift, int cols, float2* red) {
   RowGroup r;
   const int tpr = TPR ? TPR : g.tpr;
   r.width = tpr < 32 ? tpr : 32;
@@ -72,15 +81,15 @@ __device__ __forceinline__ RowGroup row_group(const NgaGeom& g, int K, int vec, 
     if (FULL) return (float)(K * 32 * vec);
     int n = 0;
     for (int k = 0; k < K; ++k) {
-      int left = g.nv - (k * tpr + w * 32);
-      left = left < 0 ? 0 : (left > 32 ? 32 : left);
-      n += left;
+      const int v0 = k * tpr + w * 32, v1 = v0 + 32 < nv ? v0 + 32 : nv;
+      const int e0 = v0 * vec > shift ? v0 * vec : shift, e1 = v1 * vec < shift + cols ? v1 * vec : shift + cols;
+      n += e1 > e0 ? e1 - e0 : 0;
     }
-    return (float)(n * vec);
+    return (float)n;
   };
   const int lane = threadIdx.x & 31;
   r.cnt = lane < r.wpr ? count(lane) : 0.f;
-  r.mine = r.wpr == 1 ? (float)(g.nv * vec) : count((int)(threadIdx.x >> 5) - r.warp0);
+  r.mine = r.wpr == 1 ? (float)cols : count((int)(threadIdx.x >> 5) - r.warp0);
   return r;
 }
 template <int NV>
@@ -132,8 +141,9 @@ __device__ __forceinline__ void row_sum2(RowGroup& g, float& a, float& b) {
 // Mean and reciprocal deviation of the row held in v (zeros behind it).  LayerNorm: the spread is
 // taken about the mean of the warp, and the warps' spreads are joined with that of their means
 // about the row's, so one barrier is enough and nothing cancels.
-template <int K, int V2, bool GEN>
-__device__ __forceinline__ void row_stats(RowGroup& g, int kind, const float2 (&v)[K][V2], const bool (&ok)[K], float inv_n,
+// only(k, e, d): d where the two elements belong to the row, else zeros.
+template <int K, int V2, bool GEN, typename Only>
+__device__ __forceinline__ void row_stats(RowGroup& g, int kind, const float2 (&v)[K][V2], const Only& only, float inv_n,
                                           float eps, float& mean, float& rstd) {
   float q = 0.f;
   mean = 0.f;
@@ -157,12 +167,10 @@ __device__ __forceinline__ void row_stats(RowGroup& g, int kind, const float2 (&
     t = f2(0.f);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (ok[k]) {
 #pragma unroll
-        for (int e = 0; e < V2; ++e) {
-          const float2 d = f2add(v[k][e], f2(-m));
-          t = f2fma(d, d, t);
-        }
+      for (int e = 0; e < V2; ++e) {
+        const float2 d = only(k, e, f2add(v[k][e], f2(-m)));
+        t = f2fma(d, d, t);
       }
     }
     float d2[1] = {t.x + t.y};
@@ -194,6 +202,58 @@ __device__ __forceinline__ void cp_async_wait_behind(int ahead) {  // at most `a
   else if (ahead == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
   else asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
+__device__ __forceinline__ void cp_async16_part(void* smem, const void* src, int bytes) {  // the rest zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(smem)), "l"(src),
+               "r"(bytes)
+               : "memory");
+}
+// Where a thread's vectors lie in the row.  at[k]: column of the first element (below zero in the
+// first vector of a shifted row); a vector behind the row is replaced by the row's last one and
+// ok[k] is false; [lo, hi): the elements of an edge vector that belong to the row.
+template <int K, int VEC, bool FULL, bool SHIFT>
+struct Places {
+  int at[K];
+  bool ok[K], edge[SHIFT ? K : 1];
+  int lo[SHIFT ? K : 1], hi[SHIFT ? K : 1];
+  __device__ __forceinline__ void set(int lane, int tpr, int nv, int cols, int shift) {
+    if (SHIFT) nv = (shift + cols + VEC - 1) / VEC;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int v = lane + k * tpr;
+      ok[k] = FULL || (!SHIFT && K == 2 && k == 0) || v < nv;  // (tpr <= nv where K is 2)
+      at[k] = (ok[k] ? v : nv - 1) * VEC - (SHIFT ? shift : 0);
+      if (SHIFT) {
+        lo[SHIFT ? k : 0] = at[k] < 0 ? -at[k] : 0;
+        hi[SHIFT ? k : 0] = cols - at[k] < VEC ? cols - at[k] : VEC;
+        edge[SHIFT ? k : 0] = at[k] < 0 || at[k] + VEC > cols;
+      }
+    }
+  }
+  // a pair of the vector where it belongs to the row, else zeros (not v times zero, which would be
+  // NaN where v is infinite)
+  __device__ __forceinline__ float2 only(int k, int e, float2 v) const {
+    if (FULL) return v;
+    if (SHIFT) {
+      const int l = lo[SHIFT ? k : 0], h = hi[SHIFT ? k : 0];
+      return make_float2(ok[k] && 2 * e >= l && 2 * e < h ? v.x : 0.f, ok[k] && 2 * e + 1 >= l && 2 * e + 1 < h ? v.y : 0.f);
+    }
+    return make_float2(ok[k] ? v.x : 0.f, ok[k] ? v.y : 0.f);
+  }
+  // what the neighbouring rows have in an edge vector, set to zero
+  __device__ __forceinline__ void trim(int k, float2 (&v)[VEC / 2]) const {
+    if (SHIFT && edge[SHIFT ? k : 0]) {
+#pragma unroll
+      for (int e = 0; e < VEC / 2; ++e) {
+        const int l = lo[SHIFT ? k : 0], h = hi[SHIFT ? k : 0];
+        v[e] = make_float2(2 * e >= l && 2 * e < h ? v[e].x : 0.f, 2 * e + 1 >= l && 2 * e + 1 < h ? v[e].y : 0.f);
+      }
+    }
+  }
+};
+// the first column of a row in its first vector
+__device__ __forceinline__ int row_shift(int64_t row, int cols, int vec) {
+  return (int)((uint32_t)(row & (vec - 1)) * (uint32_t)(cols & (vec - 1)) & (uint32_t)(vec - 1));
+}
 // v, or zeros (not v times zero, which would be NaN where v is infinite)
 __device__ __forceinline__ float2 f2only(bool on, float2 v) { return make_float2(on ? v.x : 0.f, on ? v.y : 0.f); }
 template <typename T>
@@ -208,13 +268,36 @@ __device__ __forceinline__ void give(T* p, const float2 (&f)[8 / sizeof(T)]) {
   pack2<T, 16 / sizeof(T)>(f, v);
   st_stream<T, 16 / sizeof(T)>(p, v);
 }
-template <typename T>
-__device__ __forceinline__ void param2(const void* p, int64_t at, float2 (&f)[8 / sizeof(T)]) {
-  unpack2<T, 16 / sizeof(T)>(ld_param<T, 16 / sizeof(T)>(reinterpret_cast<const T*>(p) + at), f);
+// a vector of a row at `row`, whole or only what belongs to the row
+template <typename T, int K, bool FULL, bool SHIFT>
+__device__ __forceinline__ void give_row(T* row, const Places<K, 16 / (int)sizeof(T), FULL, SHIFT>& w, int k,
+                                         const float2 (&f)[8 / sizeof(T)]) {
+  if (SHIFT && w.edge[SHIFT ? k : 0]) {
+#pragma unroll
+    for (int e = 0; e < 8 / (int)sizeof(T); ++e) {
+      const int l = w.lo[SHIFT ? k : 0], h = w.hi[SHIFT ? k : 0];
+      if (2 * e >= l && 2 * e < h) row[w.at[k] + 2 * e] = Cvt<T>::from_f(f[e].x);
+      if (2 * e + 1 >= l && 2 * e + 1 < h) row[w.at[k] + 2 * e + 1] = Cvt<T>::from_f(f[e].y);
+    }
+    return;
+  }
+  give<T>(row + w.at[k], f);
+}
+// a vector of a parameter; SHIFT: element by element, the nearest there is for those beside the row
+template <typename T, bool SHIFT>
+__device__ __forceinline__ void param2(const void* p, int64_t off, int col, int cols, float2 (&f)[8 / sizeof(T)]) {
+  const T* q = reinterpret_cast<const T*>(p) + off;
+  if (!SHIFT) {
+    unpack2<T, 16 / sizeof(T)>(ld_param<T, 16 / sizeof(T)>(q + col), f);
+    return;
+  }
+  auto one = [&](int c) { return Cvt<T>::to_f(__ldg(q + (c < 0 ? 0 : (c < cols ? c : cols - 1)))); };
+#pragma unroll
+  for (int e = 0; e < 8 / (int)sizeof(T); ++e) f[e] = make_float2(one(col + 2 * e), one(col + 2 * e + 1));
 }
 
 // C1 and B1 of a vector of columns; `goff` is where the group's gate vector starts
-template <typename T, int GATE>
+template <typename T, int GATE, bool SHIFT>
 __device__ __forceinline__ void coef1(const NgaParams& p, int col, int64_t goff, float2 (&c)[8 / sizeof(T)],
                                       float2 (&b)[8 / sizeof(T)]) {
   constexpr int V2 = 8 / (int)sizeof(T);
@@ -224,16 +307,16 @@ __device__ __forceinline__ void coef1(const NgaParams& p, int col, int64_t goff,
     b[e] = f2(0.f);
   }
   if (p.w1 != nullptr) {
-    param2<T>(p.w1, col, c);
+    param2<T, SHIFT>(p.w1, 0, col, p.cols, c);
 #pragma unroll
     for (int e = 0; e < V2; ++e) c[e] = f2add(c[e], f2(p.woff));
   }
-  if (p.b1 != nullptr) param2<T>(p.b1, col, b);
+  if (p.b1 != nullptr) param2<T, SHIFT>(p.b1, 0, col, p.cols, b);
   float2 a[V2];
 #pragma unroll
   for (int e = 0; e < V2; ++e) a[e] = f2(1.f);
   if (GATE == 1) {
-    param2<T>(p.gate, goff + col, a);
+    param2<T, SHIFT>(p.gate, goff, col, p.cols, a);
 #pragma unroll
     for (int e = 0; e < V2; ++e)
       a[e] = make_float2(gate_act<sizeof(T) == 4>(a[e].x, p.act), gate_act<sizeof(T) == 4>(a[e].y, p.act));
@@ -245,8 +328,8 @@ __device__ __forceinline__ void coef1(const NgaParams& p, int col, int64_t goff,
     b[e] = f2mul(b[e], a[e]);
   }
 }
-template <typename T>
-__device__ __forceinline__ void coef2(const NgaParams& p, int64_t at, float2 (&c)[8 / sizeof(T)], float2 (&b)[8 / sizeof(T)]) {
+template <typename T, bool SHIFT>
+__device__ __forceinline__ void coef2(const NgaParams& p, int col, int64_t aoff, float2 (&c)[8 / sizeof(T)], float2 (&b)[8 / sizeof(T)]) {
   constexpr int V2 = 8 / (int)sizeof(T);
 #pragma unroll
   for (int e = 0; e < V2; ++e) {
@@ -254,11 +337,11 @@ __device__ __forceinline__ void coef2(const NgaParams& p, int64_t at, float2 (&c
     b[e] = f2(0.f);
   }
   if (p.w2 != nullptr) {
-    param2<T>(p.w2, at, c);
+    param2<T, SHIFT>(p.w2, aoff, col, p.cols, c);
 #pragma unroll
     for (int e = 0; e < V2; ++e) c[e] = f2add(c[e], f2(p.woff));
   }
-  if (p.b2 != nullptr) param2<T>(p.b2, at, b);
+  if (p.b2 != nullptr) param2<T, SHIFT>(p.b2, aoff, col, p.cols, b);
 }
 
 // ----------------------------------------------------------------------------------------
@@ -269,7 +352,7 @@ __device__ __forceinline__ void coef2(const NgaParams& p, int64_t at, float2 (&c
 // GATE 0: none, 1: shared by rows, 2: an element each.  HOLD: the coefficients stay in registers
 // over the chunk, else they are made again for every row (rows too long for that).
 // ----------------------------------------------------------------------------------------
-template <typename T, int K, int GATE, bool GEN, bool HOLD, int TPR, bool RAG>
+template <typename T, int K, int GATE, bool GEN, bool HOLD, int TPR, bool RAG, bool SHIFT>
 __global__ void __launch_bounds__(512) nga_fwd_rows_kernel(const NgaParams p, const NgaGeom g) {
   constexpr bool EXACT = sizeof(T) == 4;
   constexpr int VEC = 16 / (int)sizeof(T), V2 = VEC / 2;
@@ -279,7 +362,6 @@ __global__ void __launch_bounds__(512) nga_fwd_rows_kernel(const NgaParams p, co
   const int R = TPR ? fixed_rows(TPR) : g.R;
   const int threads = TPR ? TPR * fixed_rows(TPR) : g.threads;
   const int cols = FULL ? TPR * K * VEC : p.cols;
-  RowGroup rg = row_group<TPR, FULL>(g, K, VEC, reinterpret_cast<float2*>(smem));
   const int tid = threadIdx.x;
   const int r_in = tid / tpr, lane = tid - r_in * tpr;
   const float inv_n = 1.0f / (float)cols;
@@ -288,20 +370,29 @@ __global__ void __launch_bounds__(512) nga_fwd_rows_kernel(const NgaParams p, co
   const int has_res = p.res != nullptr ? 1 : 0;
   const uint32_t stage_bytes = (uint32_t)(1 + has_res + (GATE == 2 ? 1 : 0)) * unit;
   const uint32_t gate_off = (uint32_t)(1 + has_res) * unit;
-  const int64_t group = blockIdx.x / g.per_group;
-  const int64_t first = group * p.group_rows + (blockIdx.x - group * g.per_group) * g.chunk;
-  int64_t last = (group + 1) * p.group_rows;
-  if (first + g.chunk < last) last = first + g.chunk;
+  int64_t group, first, last;
+  if (SHIFT) {
+    const SlotRows sr = slot_rows(p, blockIdx.x);
+    group = sr.group;
+    first = sr.first;
+    last = sr.last;
+  } else {
+    group = blockIdx.x / g.per_group;
+    first = group * p.group_rows + (blockIdx.x - group * g.per_group) * g.chunk;
+    last = (group + 1) * p.group_rows;
+    if (first + g.chunk < last) last = first + g.chunk;
+  }
+  const int64_t apart = SHIFT ? p.period : 1;  // from one row to the next
   const int64_t goff = p.gate_mode == FLN_GATE_GROUP ? group * cols : 0;
   const int64_t aoff = p.affine_grouped ? group * cols : 0;
-  bool vok[K];
-#pragma unroll
-  for (int k = 0; k < K; ++k) vok[k] = FULL || (K == 2 && k == 0) || lane + k * tpr < g.nv;  // (tpr <= nv where K is 2)
   // A lane whose last vectors lie behind the row works on the row's last vector instead; what goes
   // into the sums is set to zero there and nothing is stored, so the arithmetic has no branches.
-  int col[K];
-#pragma unroll
-  for (int k = 0; k < K; ++k) col[k] = (vok[k] ? lane + k * tpr : g.nv - 1) * VEC;
+  Places<K, VEC, FULL, SHIFT> w;
+  const int shift = SHIFT ? row_shift(first, cols, VEC) : 0;
+  w.set(lane, tpr, g.nv, cols, shift);
+  RowGroup rg = row_group<TPR, FULL>(g, K, VEC, SHIFT ? (shift + cols + VEC - 1) / VEC : g.nv, shift, cols,
+                                     reinterpret_cast<float2*>(smem));
+  auto only = [&](int k, int e, float2 v) { return w.only(k, e, v); };
 
   // row groups behind the last row work on the last row once more (and write the same values), so
   // that nothing below depends on it
@@ -309,16 +400,26 @@ __global__ void __launch_bounds__(512) nga_fwd_rows_kernel(const NgaParams p, co
   int in_stage = 0;
   auto fetch = [&]() {
     if (ahead < last) {
-      const int64_t o = (ahead + r_in < last ? ahead + r_in : last - 1) * (int64_t)cols;
+      const int64_t mine = ahead + r_in * apart;
+      const int64_t o = (mine < last ? mine : last - 1) * (int64_t)cols;
       unsigned char* st = stages + (uint32_t)in_stage * stage_bytes;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         unsigned char* d = st + (uint32_t)(k * threads) * 16u;
-        cp_async16(d, reinterpret_cast<const T*>(p.x) + o + col[k]);
-        if (has_res) cp_async16(d + unit, reinterpret_cast<const T*>(p.res) + o + col[k]);
-        if (GATE == 2) cp_async16(d + gate_off, reinterpret_cast<const T*>(p.gate) + o + col[k]);
+        const int64_t q = o + w.at[k];
+        auto bring = [&](unsigned char* to, const void* from) {
+          if (SHIFT) {  // the last vector of the last row may reach behind the tensor
+            const int64_t left = (p.rows * cols - q) * (int)sizeof(T);
+            cp_async16_part(to, reinterpret_cast<const T*>(from) + q, left < 16 ? (int)left : 16);
+          } else {
+            cp_async16(to, reinterpret_cast<const T*>(from) + q);
+          }
+        };
+        bring(d, p.x);
+        if (has_res) bring(d + unit, p.res);
+        if (GATE == 2) bring(d + gate_off, p.gate);
       }
-      ahead += R;
+      ahead += R * apart;
     }
     cp_async_commit();
     in_stage = in_stage + 1 == g.stages ? 0 : in_stage + 1;
@@ -329,15 +430,15 @@ __global__ void __launch_bounds__(512) nga_fwd_rows_kernel(const NgaParams p, co
   if (HOLD) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      coef1<T, GATE>(p, col[k], goff, c1[HOLD ? k : 0], b1[HOLD && GEN ? k : 0]);
-      coef2<T>(p, aoff + col[k], c2[HOLD ? k : 0], b2[HOLD && GEN ? k : 0]);
+      coef1<T, GATE, SHIFT>(p, w.at[k], goff, c1[HOLD ? k : 0], b1[HOLD && GEN ? k : 0]);
+      coef2<T, SHIFT>(p, w.at[k], aoff, c2[HOLD ? k : 0], b2[HOLD && GEN ? k : 0]);
     }
   }
   const float2 ra = f2(p.ra);
   int stage = 0;
-  for (int64_t row0 = first; row0 < last; row0 += R) {
+  for (int64_t row0 = first; row0 < last; row0 += R * apart) {
     fetch();
-    const int64_t row = row0 + r_in < last ? row0 + r_in : last - 1;
+    const int64_t row = row0 + r_in * apart < last ? row0 + r_in * apart : last - 1;
     cp_async_wait_behind(g.stages - 1);
     const unsigned char* st = stages + (uint32_t)stage * stage_bytes;
     stage = stage + 1 == g.stages ? 0 : stage + 1;
@@ -347,18 +448,18 @@ __global__ void __launch_bounds__(512) nga_fwd_rows_kernel(const NgaParams p, co
       take<T>(st + (uint32_t)(k * threads) * 16u, s[k]);
       if (!FULL) {
 #pragma unroll
-        for (int e = 0; e < V2; ++e) s[k][e] = f2only(vok[k], s[k][e]);
+        for (int e = 0; e < V2; ++e) s[k][e] = w.only(k, e, s[k][e]);
       }
     }
     float mean1 = 0.f, rstd1 = 1.f;
-    if (p.post_kind != FLN_NO_NORM) row_stats<K, V2, GEN>(rg, p.post_kind, s, vok, inv_n, p.eps1, mean1, rstd1);
+    if (p.post_kind != FLN_NO_NORM) row_stats<K, V2, GEN>(rg, p.post_kind, s, only, inv_n, p.eps1, mean1, rstd1);
     T* sum = reinterpret_cast<T*>(p.sum) + row * (int64_t)cols;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       {
         const unsigned char* d = st + (uint32_t)(k * threads) * 16u;
         float2 tc[V2], tb[V2];
-        if (!HOLD) coef1<T, GATE>(p, col[k], goff, tc, tb);
+        if (!HOLD) coef1<T, GATE, SHIFT>(p, w.at[k], goff, tc, tb);
 #pragma unroll
         for (int e = 0; e < V2; ++e) {
           // (x - mean) * rstd: without a norm mean is 0 and rstd 1, and x passes as it is
@@ -381,22 +482,22 @@ __global__ void __launch_bounds__(512) nga_fwd_rows_kernel(const NgaParams p, co
 #pragma unroll
           for (int e = 0; e < V2; ++e) s[k][e] = f2fma(r[e], ra, s[k][e]);
         }
-        if (vok[k]) give<T>(sum + col[k], s[k]);
+        if (w.ok[k]) give_row<T, K, FULL, SHIFT>(sum, w, k, s[k]);
         if (!FULL) {
 #pragma unroll
-          for (int e = 0; e < V2; ++e) s[k][e] = f2only(vok[k], s[k][e]);
+          for (int e = 0; e < V2; ++e) s[k][e] = w.only(k, e, s[k][e]);
         }
       }
     }
     float mean2 = 0.f, rstd2 = 1.f;
     if (p.kind != FLN_NO_NORM) {
-      row_stats<K, V2, GEN>(rg, p.kind, s, vok, inv_n, p.eps2, mean2, rstd2);
+      row_stats<K, V2, GEN>(rg, p.kind, s, only, inv_n, p.eps2, mean2, rstd2);
       T* y = reinterpret_cast<T*>(p.y) + row * (int64_t)cols;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         {
           float2 tc[V2], tb[V2];
-          if (!HOLD) coef2<T>(p, aoff + col[k], tc, tb);
+          if (!HOLD) coef2<T, SHIFT>(p, w.at[k], aoff, tc, tb);
 #pragma unroll
           for (int e = 0; e < V2; ++e) {
             if (GEN) s[k][e] = f2add(s[k][e], f2(-mean2));
@@ -405,7 +506,7 @@ __global__ void __launch_bounds__(512) nga_fwd_rows_kernel(const NgaParams p, co
             const float2 b = HOLD ? b2[HOLD && GEN ? k : 0][e] : tb[e];
             s[k][e] = GEN ? f2fma(s[k][e], c, b) : f2mul(s[k][e], c);
           }
-          if (vok[k]) give<T>(y + col[k], s[k]);
+          if (w.ok[k]) give_row<T, K, FULL, SHIFT>(y, w, k, s[k]);
         }
       }
     }
@@ -470,7 +571,7 @@ inline int nga_set_of(const NgaParams& p) {
   return 0;
 }
 
-template <typename T, int K, int GATE, bool GEN, bool CSM, int TPR, bool RAG, int SET>
+template <typename T, int K, int GATE, bool GEN, bool CSM, int TPR, bool RAG, int SET, bool SHIFT>
 __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_bwd_rows_kernel(const NgaParams p, const NgaGeom g) {
   constexpr bool EXACT = sizeof(T) == 4;
   constexpr int VEC = 16 / (int)sizeof(T), V2 = VEC / 2;
@@ -486,7 +587,7 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
   const int threads = TPR ? TPR * fixed_rows(TPR) : g.threads;
   const int cols = FULL ? TPR * K * VEC : p.cols;
   constexpr bool ONE = TPR != 0 && fixed_rows(TPR ? TPR : 1) == 1;  // one row at a time: never behind the slot
-  RowGroup rg = row_group<TPR, FULL>(g, K, VEC, reinterpret_cast<float2*>(smem));
+  RowGroup rg = row_group<TPR, FULL>(g, K, VEC, g.nv, 0, cols, reinterpret_cast<float2*>(smem));
   const int tid = threadIdx.x;
   const int r_in = ONE ? 0 : tid / tpr, lane = tid - r_in * tpr;
   const float inv_n = 1.0f / (float)cols;
@@ -496,14 +597,11 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
   unsigned char* stages = coefs + (uint32_t)l.coefs * unit;
   const uint32_t stage_bytes = (uint32_t)l.tensors * unit;
   const uint32_t ring_bytes = (uint32_t)g.stages * stage_bytes;
-  bool vok[K];
-#pragma unroll
-  for (int k = 0; k < K; ++k) vok[k] = FULL || (K == 2 && k == 0) || lane + k * tpr < g.nv;  // (tpr <= nv where K is 2)
   // Lanes behind the row work on its last vector, row groups behind the slot on its last row; what
   // goes into the sums is set to zero there and nothing is stored, so the arithmetic has no branches.
-  int col[K];
-#pragma unroll
-  for (int k = 0; k < K; ++k) col[k] = (vok[k] ? lane + k * tpr : g.nv - 1) * VEC;
+  Places<K, VEC, FULL, SHIFT> w;
+  if (!SHIFT) w.set(lane, tpr, g.nv, cols, 0);
+  const int apart = SHIFT ? p.period : 1;  // from one row to the next
 
   // The row sequence of this CTA: slot after slot, R rows at a time; one walker runs ahead.
   struct Walker {
@@ -518,13 +616,13 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
     }
   };
   auto step = [&](Walker& w) {
-    w.row += R;
+    w.row += R * apart;
     if (w.row >= w.last) {
       w.slot += grid;
       open(w);
     }
   };
-  auto my_row = [&](const Walker& w) { return ONE ? w.row : (w.row + r_in < w.last ? w.row + r_in : w.last - 1); };
+  auto my_row = [&](const Walker& w) { return ONE ? w.row : (w.row + r_in * apart < w.last ? w.row + r_in * apart : w.last - 1); };
   Walker ahead{(int)blockIdx.x, 0, 0};
   open(ahead);
   Walker cur = ahead;
@@ -532,16 +630,26 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
   auto fetch = [&]() {
     if (ahead.slot < nslots) {
       unsigned char* st = stages + fill;
-      const int64_t at = (int64_t)my_row(ahead) * cols;
+      const int64_t row_at = (int64_t)my_row(ahead) * cols;
+      Places<K, VEC, FULL, SHIFT> wa = w;
+      if (SHIFT) wa.set(lane, tpr, g.nv, cols, row_shift(ahead.row, cols, VEC));
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         unsigned char* d = st + k * kstep;
-        const int64_t o = at + col[k];
-        cp_async16(d, reinterpret_cast<const T*>(p.x) + o);
-        if (has_res) cp_async16(d + l.res * unit, reinterpret_cast<const T*>(p.res) + o);
-        if (has_dy) cp_async16(d + l.dy * unit, reinterpret_cast<const T*>(p.dy) + o);
-        if (has_ds && !DIRECT) cp_async16(d + l.ds * unit, reinterpret_cast<const T*>(p.ds) + o);
-        if (GATE == 2) cp_async16(d + l.gate * unit, reinterpret_cast<const T*>(p.gate) + o);
+        const int64_t o = row_at + wa.at[k];
+        auto bring = [&](unsigned char* to, const void* from) {
+          if (SHIFT) {  // the last vector of the last row may reach behind the tensor
+            const int64_t left = (p.rows * cols - o) * (int)sizeof(T);
+            cp_async16_part(to, reinterpret_cast<const T*>(from) + o, left < 16 ? (int)left : 16);
+          } else {
+            cp_async16(to, reinterpret_cast<const T*>(from) + o);
+          }
+        };
+        bring(d, p.x);
+        if (has_res) bring(d + l.res * unit, p.res);
+        if (has_dy) bring(d + l.dy * unit, p.dy);
+        if (has_ds && !DIRECT) bring(d + l.ds * unit, p.ds);
+        if (GATE == 2) bring(d + l.gate * unit, p.gate);
       }
       step(ahead);
     }
@@ -600,14 +708,15 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
       coef(l.c1, k, c);
       if (GEN) coef(l.b1, k, b);
     } else {
-      coef1<T, GATE>(p, col[k], goff, c, b);
+      coef1<T, GATE, SHIFT>(p, w.at[k], goff, c, b);
     }
   };
   while (cur.slot < nslots) {
     if (opened) {
       const int64_t grp = cur.slot / p.slots_per_group;
-      if (grp != group) {  // coefficients of a new group
-        const bool first = group < 0;
+      if (SHIFT) w.set(lane, tpr, g.nv, cols, row_shift(cur.row, cols, VEC));
+      if (SHIFT || grp != group) {  // coefficients of a new group, or for another place of the row
+        const bool first = SHIFT || group < 0;
         group = grp;
         goff = p.gate_mode == FLN_GATE_GROUP ? grp * cols : 0;
         aoff = p.affine_grouped ? grp * cols : 0;
@@ -622,12 +731,12 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
                     make_float4(v[e].x, v[e].y, v[e + 1].x, v[e + 1].y);
             };
             if (first || p.gate_mode == FLN_GATE_GROUP) {
-              coef1<T, GATE>(p, col[k], goff, c, b);
+              coef1<T, GATE, SHIFT>(p, w.at[k], goff, c, b);
               put(l.c1, c);
               if (GEN) put(l.b1, b);
             }
             if (has_dy && (first || p.affine_grouped)) {
-              coef2<T>(p, aoff + col[k], c, b);
+              coef2<T, SHIFT>(p, w.at[k], aoff, c, b);
               put(l.c2, c);
             }
           }
@@ -636,7 +745,8 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
     }
     fetch();
     const int slot = cur.slot;
-    const bool live = ONE || cur.row + r_in < cur.last;
+    const int slot_shift = SHIFT ? row_shift(cur.row, cols, VEC) : 0;
+    const bool live = ONE || cur.row + r_in * apart < cur.last;
     const int64_t base = (int64_t)my_row(cur) * cols;
     const Scalars sc = sc_next;
     step(cur);
@@ -650,7 +760,7 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
     Pack<T, VEC> ds_now[DIRECT ? K : 1];
     if (DIRECT) {  // used behind the first row sum
 #pragma unroll
-      for (int k = 0; k < K; ++k) ds_now[DIRECT ? k : 0] = ld_stream<T, VEC>(reinterpret_cast<const T*>(p.ds) + base + col[k]);
+      for (int k = 0; k < K; ++k) ds_now[DIRECT ? k : 0] = ld_stream<T, VEC>(reinterpret_cast<const T*>(p.ds) + base + w.at[k]);
     }
     float2 xh[K][V2], sh[K][V2], g2[K][V2];
     float2 r0 = f2(0.f), r1 = f2(0.f);
@@ -659,6 +769,7 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
       for (int k = 0; k < K; ++k) {
         const unsigned char* d = st + k * kstep;
         take<T>(d, xh[k]);
+        w.trim(k, xh[k]);
 #pragma unroll
         for (int e = 0; e < V2; ++e) {
           if (GEN) xh[k][e] = f2add(xh[k][e], f2(-sc.mean1));
@@ -680,13 +791,15 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
 #pragma unroll
             for (int e = 0; e < V2; ++e) sh[k][e] = f2fma(c[e], ra, sh[k][e]);
           }
+          w.trim(k, sh[k]);
           take<T>(d + l.dy * unit, g2[k]);
+          w.trim(k, g2[k]);
           if (!(FULL && ONE)) {
 #pragma unroll
-            for (int e = 0; e < V2; ++e) g2[k][e] = f2only(live && vok[k], g2[k][e]);
+            for (int e = 0; e < V2; ++e) g2[k][e] = f2only(live && w.ok[k], g2[k][e]);
           }
           if (CSM) coef(l.c2, k, c);
-          else coef2<T>(p, aoff + col[k], c, b);
+          else coef2<T, SHIFT>(p, w.at[k], aoff, c, b);
 #pragma unroll
           for (int e = 0; e < V2; ++e) {
             if (GEN) sh[k][e] = f2add(sh[k][e], f2(-sc.mean2));
@@ -715,7 +828,7 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
       T* dgate = reinterpret_cast<T*>(p.dgate) + base;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const bool ok = live && vok[k];
+        const bool ok = live && w.ok[k];
         const unsigned char* st_k = st + k * kstep;
         float2 d[V2], c[V2], b[V2];
         if (DIRECT) {
@@ -736,16 +849,18 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
         if (!(FULL && ONE)) {
 #pragma unroll
           for (int e = 0; e < V2; ++e) d[e] = f2only(ok, d[e]);
+          w.trim(k, d);
         }
         if (p.dres != nullptr) {
 #pragma unroll
           for (int e = 0; e < V2; ++e) c[e] = f2mul(d[e], ra);
-          if (ok) give<T>(dres + col[k], c);
+          if (ok) give_row<T, K, FULL, SHIFT>(dres, w, k, c);
         }
         first_coefs(k, c, b);
         if (GATE == 2) {
           float2 gv[V2];
           take<T>(st_k + l.gate * unit, gv);
+          w.trim(k, gv);
           if (p.dgate != nullptr) {
             float2 o[V2];
 #pragma unroll
@@ -757,7 +872,7 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
               o[e] = f2mul(f2mul(d[e], n), da);
               d[e] = f2mul(d[e], a);
             }
-            if (ok) give<T>(dgate + col[k], o);
+            if (ok) give_row<T, K, FULL, SHIFT>(dgate, w, k, o);
           } else {
 #pragma unroll
             for (int e = 0; e < V2; ++e)
@@ -794,7 +909,7 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
               g2[k][e] = f2mul(q, f2(sc.rstd1));
             }
           }
-          if (live && vok[k]) give<T>(dx + col[k], g2[k]);
+          if (live && w.ok[k]) give_row<T, K, FULL, SHIFT>(dx, w, k, g2[k]);
         }
       }
     }
@@ -816,10 +931,19 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
                 acc[k][e].y += __shfl_xor_sync(0xffffffffu, acc[k][e].y, off);
               }
             }
-            const bool mine = vok[k] && (tpr >= 32 || (tid & 31) < tpr);
+            const bool mine = w.ok[k] && (tpr >= 32 || (tid & 31) < tpr);
             const bool join = !ONE && g.rep > 1;
-            float* q = join ? joint + (who * tpr + lane) * VEC : dst + col[k];
-            if (mine || join) {
+            float* q = join ? joint + (who * tpr + lane) * VEC : dst + w.at[k];
+            if (SHIFT && !join) {
+              if (mine) {
+#pragma unroll
+                for (int e = 0; e < V2; ++e) {
+                  const int lo = w.lo[SHIFT ? k : 0], hi = w.hi[SHIFT ? k : 0];
+                  if (2 * e >= lo && 2 * e < hi) q[2 * e] = acc[k][e].x * scale;
+                  if (2 * e + 1 >= lo && 2 * e + 1 < hi) q[2 * e + 1] = acc[k][e].y * scale;
+                }
+              }
+            } else if (mine || join) {
 #pragma unroll
               for (int e = 0; e < V2; e += 2)
                 *reinterpret_cast<float4*>(q + 2 * e) =
@@ -830,7 +954,8 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
               for (int i = tid; i < tpr * VEC; i += threads) {
                 float v = 0.f;
                 for (int r = 0; r < g.rep; ++r) v += joint[r * tpr * VEC + i];
-                if (k * tpr * VEC + i < cols) dst[k * tpr * VEC + i] = v;
+                const int c = k * tpr * VEC + i - (SHIFT ? slot_shift : 0);
+                if (c >= 0 && c < cols) dst[c] = v;
               }
               __syncthreads();
             }
@@ -881,14 +1006,15 @@ inline int nga_ragged_tpr(int tpr) {
     if (t >= tpr && (t - tpr) * 6 <= t) return t;
   return 0;
 }
-template <typename T, int K, int GATE, int TPR, bool RAG>
+template <typename T, int K, int GATE, int TPR, bool RAG, bool SHIFT = false>
 static int nga_fwd_rows_t(const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
   constexpr bool HOLD = K * 16 / (int)sizeof(T) <= 16;
-  return nga_general(p) ? nga_launch(nga_fwd_rows_kernel<T, K, GATE, true, HOLD, TPR, RAG>, p, g, st)
-                        : nga_launch(nga_fwd_rows_kernel<T, K, GATE, false, HOLD, TPR, RAG>, p, g, st);
+  return nga_general(p) ? nga_launch(nga_fwd_rows_kernel<T, K, GATE, true, HOLD, TPR, RAG, SHIFT>, p, g, st)
+                        : nga_launch(nga_fwd_rows_kernel<T, K, GATE, false, HOLD, TPR, RAG, SHIFT>, p, g, st);
 }
 template <typename T, int K, int GATE>
 static int nga_fwd_rows_k(const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
+  if (p.period > 1) return nga_fwd_rows_t<T, K, GATE, 0, false, true>(p, g, st);
   // compile-time rows: 16 elements per thread
   if constexpr (K * 16 / (int)sizeof(T) == 16) {
     if (g.nv == K * g.tpr) {
@@ -924,16 +1050,21 @@ static int nga_fwd_rows_k(const NgaParams& p, const NgaGeom& g, cudaStream_t st)
 }
 template <typename T, int K, int GATE, bool GEN>
 static int nga_bwd_rows_g(const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
+  if (p.period > 1) {
+    if (!g.csm) return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, false, 0, false, 0, true>, p, g, st);
+    return nga_set_of(p) == 1 ? nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 1, true>, p, g, st)
+                              : nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 0, true>, p, g, st);
+  }
   if (g.direct)
-    return g.csm ? nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 3>, p, g, st)
-                 : nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, false, 0, false, 3>, p, g, st);
-  if (!g.csm) return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, false, 0, false, 0>, p, g, st);
+    return g.csm ? nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 3, false>, p, g, st)
+                 : nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, false, 0, false, 3, false>, p, g, st);
+  if (!g.csm) return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, false, 0, false, 0, false>, p, g, st);
   const int set = nga_set_of(p);
   // compile-time rows where the registers allow: 16 elements per thread, 8 of the general form
   if constexpr (K * 16 / (int)sizeof(T) == (GEN ? 8 : 16)) {
 #define FLN_NGA_BWD(TPR, RAG, SET) \
   case TPR:                        \
-    return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, TPR, RAG, SET>, p, g, st);
+    return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, TPR, RAG, SET, false>, p, g, st);
     if (g.nv == K * g.tpr && set == 1) {
       switch (g.tpr) {
         FLN_NGA_BWD(64, false, 1)
@@ -960,8 +1091,8 @@ static int nga_bwd_rows_g(const NgaParams& p, const NgaGeom& g, cudaStream_t st)
     }
 #undef FLN_NGA_BWD
   }
-  if (set == 1) return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 1>, p, g, st);
-  return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 0>, p, g, st);
+  if (set == 1) return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 1, false>, p, g, st);
+  return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 0, false>, p, g, st);
 }
 template <typename T, int K, int GATE>
 static int nga_bwd_rows_k(const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
