@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "fln_b200.h"
@@ -537,6 +538,24 @@ Plan make_plan(bool backward, int64_t rows, int cols, int elem_bytes, bool align
 void plan_override(int* K, int* tpr);
 
 inline bool is_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Lets KERN be launched with `bytes` of dynamic shared memory on the current device; the runtime is
+// asked once per kernel and device (the call costs about a microsecond).
+template <auto KERN>
+inline bool allow_smem(size_t bytes) {
+  if (bytes <= 48 * 1024) return true;
+  static std::atomic<unsigned long long> done{0};  // bit per device, for the largest size there is
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const unsigned long long bit = dev >= 0 && dev < 64 ? 1ull << dev : 0ull;
+  if (bit != 0 && (done.load(std::memory_order_relaxed) & bit) != 0) return true;
+  if (cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
 
 #define FLN_CHECK_LAUNCH()                                   \
   do {                                                       \

@@ -541,7 +541,10 @@ static int plan_backward(NgaParams* p, int es, NgaGeom* g) {
   const int vec = 16 / es;
   g->nv = row_vector_count(*p, es);
   auto most = [&](int e) { return e <= 8 ? 640 : 512; };
-  int E = nga_general(*p) ? 8 : 16;
+  // 16 elements per thread, 8 with four column sums and for fp32 (whose staged rows leave room for
+  // one CTA of either: 8192 x 4096, 145 us with 512 threads, 165 with 256)
+  const bool eight = nga_general(*p) || es == 4;
+  int E = eight ? 8 : 16;
   int fK = 0, ftpr = 0;
   plan_override(&fK, &ftpr);
   if (fK == 1 || fK == 2) E = 8 * fK;
@@ -550,7 +553,7 @@ static int plan_backward(NgaParams* p, int es, NgaGeom* g) {
   const int K = E / vec;
   g->tpr = threads_per_row(g->nv, K);
   const int set = p->period == 1 ? nga_set_of(*p) : 0;  // (0: dsum never past the ring)
-  if (set == 1 && E == (nga_general(*p) ? 8 : 16) && K * g->tpr != g->nv && nga_ragged_tpr(g->tpr) != 0 && g->tpr > 96)
+  if (set == 1 && E == (eight ? 8 : 16) && K * g->tpr != g->nv && nga_ragged_tpr(g->tpr) != 0 && g->tpr > 96)
     g->tpr = nga_ragged_tpr(g->tpr);
   rows_per_cta(g);
   g->rep = g->tpr < 32 ? g->threads / 32 : g->R;
@@ -589,7 +592,17 @@ static int plan_backward(NgaParams* p, int es, NgaGeom* g) {
   const int64_t slots_max = (T + g->R - 1) / g->R;
   const int64_t cta = (int64_t)usable_sms() * ctas;
   if (p->period > 1) {
-    cut_classes(p, (cta + groups * p->classes - 1) / (groups * p->classes));
+    const int64_t n = (T + p->period - 1) / p->period, per = groups * p->classes;
+    int64_t best = 1, best_cost = -1;
+    for (int64_t w = 1; w <= 8; ++w) {
+      cut_classes(p, w * cta / per);
+      const int64_t cost = (p->slots + cta - 1) / cta * (((n + p->pieces - 1) / p->pieces + g->R - 1) / g->R + 1);
+      if (best_cost < 0 || cost < best_cost) {
+        best = p->pieces;
+        best_cost = cost;
+      }
+    }
+    cut_classes(p, best);
     g->grid = p->slots < cta ? p->slots : cta;
     return p->slots > 0x7fffffff - g->grid ? 0 : K;
   }

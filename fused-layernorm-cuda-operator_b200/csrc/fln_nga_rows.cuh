@@ -987,14 +987,10 @@ inline bool nga_general(const NgaParams& p) {
          (p.acc & (kAccQ | kAccV)) != 0;
 }
 
-template <typename F>
-static int nga_launch(F kern, const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
-  if (g.smem > 48 * 1024 &&
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)g.smem) != cudaSuccess) {
-    cudaGetLastError();
-    return FLN_ERR_LAUNCH;
-  }
-  kern<<<(unsigned)g.grid, g.threads, g.smem, st>>>(p, g);
+template <auto KERN>
+static int nga_launch(const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
+  if (!allow_smem<KERN>(g.smem)) return FLN_ERR_LAUNCH;
+  KERN<<<(unsigned)g.grid, g.threads, g.smem, st>>>(p, g);
   FLN_CHECK_LAUNCH();
   return FLN_OK;
 }
@@ -1009,8 +1005,8 @@ inline int nga_ragged_tpr(int tpr) {
 template <typename T, int K, int GATE, int TPR, bool RAG, bool SHIFT = false>
 static int nga_fwd_rows_t(const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
   constexpr bool HOLD = K * 16 / (int)sizeof(T) <= 16;
-  return nga_general(p) ? nga_launch(nga_fwd_rows_kernel<T, K, GATE, true, HOLD, TPR, RAG, SHIFT>, p, g, st)
-                        : nga_launch(nga_fwd_rows_kernel<T, K, GATE, false, HOLD, TPR, RAG, SHIFT>, p, g, st);
+  return nga_general(p) ? nga_launch<nga_fwd_rows_kernel<T, K, GATE, true, HOLD, TPR, RAG, SHIFT>>(p, g, st)
+                        : nga_launch<nga_fwd_rows_kernel<T, K, GATE, false, HOLD, TPR, RAG, SHIFT>>(p, g, st);
 }
 template <typename T, int K, int GATE>
 static int nga_fwd_rows_k(const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
@@ -1051,20 +1047,20 @@ static int nga_fwd_rows_k(const NgaParams& p, const NgaGeom& g, cudaStream_t st)
 template <typename T, int K, int GATE, bool GEN>
 static int nga_bwd_rows_g(const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
   if (p.period > 1) {
-    if (!g.csm) return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, false, 0, false, 0, true>, p, g, st);
-    return nga_set_of(p) == 1 ? nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 1, true>, p, g, st)
-                              : nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 0, true>, p, g, st);
+    if (!g.csm) return nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, false, 0, false, 0, true>>(p, g, st);
+    return nga_set_of(p) == 1 ? nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 1, true>>(p, g, st)
+                              : nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 0, true>>(p, g, st);
   }
   if (g.direct)
-    return g.csm ? nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 3, false>, p, g, st)
-                 : nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, false, 0, false, 3, false>, p, g, st);
-  if (!g.csm) return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, false, 0, false, 0, false>, p, g, st);
+    return g.csm ? nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 3, false>>(p, g, st)
+                 : nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, false, 0, false, 3, false>>(p, g, st);
+  if (!g.csm) return nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, false, 0, false, 0, false>>(p, g, st);
   const int set = nga_set_of(p);
-  // compile-time rows where the registers allow: 16 elements per thread, 8 of the general form
-  if constexpr (K * 16 / (int)sizeof(T) == (GEN ? 8 : 16)) {
+  // compile-time rows where the registers allow: 16 elements per thread, 8 of the general form and of fp32
+  if constexpr (K * 16 / (int)sizeof(T) == (GEN || sizeof(T) == 4 ? 8 : 16)) {
 #define FLN_NGA_BWD(TPR, RAG, SET) \
   case TPR:                        \
-    return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, TPR, RAG, SET, false>, p, g, st);
+    return nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, true, TPR, RAG, SET, false>>(p, g, st);
     if (g.nv == K * g.tpr && set == 1) {
       switch (g.tpr) {
         FLN_NGA_BWD(64, false, 1)
@@ -1091,8 +1087,8 @@ static int nga_bwd_rows_g(const NgaParams& p, const NgaGeom& g, cudaStream_t st)
     }
 #undef FLN_NGA_BWD
   }
-  if (set == 1) return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 1, false>, p, g, st);
-  return nga_launch(nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 0, false>, p, g, st);
+  if (set == 1) return nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 1, false>>(p, g, st);
+  return nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 0, false>>(p, g, st);
 }
 template <typename T, int K, int GATE>
 static int nga_bwd_rows_k(const NgaParams& p, const NgaGeom& g, cudaStream_t st) {

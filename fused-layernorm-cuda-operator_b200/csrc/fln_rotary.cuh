@@ -53,6 +53,10 @@ struct RotParams {
 };
 
 constexpr int kRotThreads = 256;
+// CTAs per SM that the registers are cut for, by the pairs a lane holds of a row
+__host__ __device__ constexpr int rot_blocks(int pairs, bool backward) {
+  return pairs <= 8 ? (backward ? 2 : 3) : (pairs <= 12 ? 2 : 1);
+}
 
 // first columns of a unit's two vectors; hi < 0: the second vector does not exist
 template <int V, bool HALF>
@@ -294,14 +298,8 @@ struct RotLane {
 // (and so more loads) be in flight.
 // GEN: layer norm or bias.  LL >= 0: log2 of the lanes per row, known at compile time.
 // ----------------------------------------------------------------------------------------
-#ifndef ROT_FMB
-#define ROT_FMB 3
-#endif
-#ifndef ROT_NBF
-#define ROT_NBF 2
-#endif
 template <typename T, int V, int U, bool HALF, int NB, bool GEN, int LL>
-__global__ void __launch_bounds__(kRotThreads, V * U <= 8 ? ROT_FMB : 1) rotary_fwd_kernel(const RotParams p) {
+__global__ void __launch_bounds__(kRotThreads, rot_blocks(V * U, false)) rotary_fwd_kernel(const RotParams p) {
   RotLane<V, U, HALF> r;
   r.template init<LL>(p);
   extern __shared__ __align__(16) float tables[];
@@ -431,7 +429,7 @@ __global__ void __launch_bounds__(kRotThreads, V * U <= 8 ? ROT_FMB : 1) rotary_
 // order at its end, so a CTA works for one tensor only.
 // ----------------------------------------------------------------------------------------
 template <typename T, int V, int U, bool HALF, int NB, bool GEN, int LL>
-__global__ void __launch_bounds__(kRotThreads, V * U <= 8 ? 2 : 1) rotary_bwd_kernel(const RotParams p) {
+__global__ void __launch_bounds__(kRotThreads, rot_blocks(V * U, true)) rotary_bwd_kernel(const RotParams p) {
   extern __shared__ __align__(16) float sacc[];  // the tables; at the end [warps][2][dim]
   const RotTables tab = rot_tables<T, V, GEN>(p, sacc);
   constexpr bool WHOLE = LL >= 0;
@@ -630,7 +628,7 @@ template <typename T, int V, int U, bool HALF, bool GEN, int LL>
 static int rotary_launch_one(const RotParams& p, bool backward, unsigned grid, cudaStream_t st) {
   // rows in flight per row group: 128 bytes of each tensor per lane where the registers allow it
   constexpr int W = 2 * V * U * (int)sizeof(T);
-  constexpr int NBF = W <= 32 ? ROT_NBF : (W <= 64 ? 2 : 1);
+  constexpr int NBF = W <= 64 ? 2 : 1;
   constexpr int NBB = W <= 32 ? 2 : 1;
   size_t smem = rot_tables_floats(p.units, V, p.dim, GEN) * sizeof(float);
   if (!backward) {
