@@ -455,7 +455,8 @@ static int threads_per_row(int nv, int K) {
 
 // Places of a 16-byte vector that the rows start at in turn, and with them p's classes.
 static bool row_vectors(NgaParams* p, int es) {
-  if (p->cols > (1 << 20)) return false;
+  // (the kernels count rows in 32 bits, a few steps past the last one)
+  if (p->cols > (1 << 20) || p->rows > 0x7fff0000) return false;
   const int vec = 16 / es;
   p->period = vec;
   for (int c = p->cols; p->period > 1 && c % 2 == 0; c /= 2) p->period /= 2;
@@ -549,10 +550,14 @@ static int plan_backward(NgaParams* p, int es, NgaGeom* g) {
   plan_override(&fK, &ftpr);
   if (fK == 1 || fK == 2) E = 8 * fK;
   if (threads_per_row(g->nv, E / vec) > most(E)) E = 16;
-  if (threads_per_row(g->nv, E / vec) > most(E)) return 0;
   const int K = E / vec;
   g->tpr = threads_per_row(g->nv, K);
-  const int set = p->period == 1 ? nga_set_of(*p) : 0;  // (0: dsum never past the ring)
+  if (g->tpr > most(E)) {  // E is 16 here
+    g->pair = 1;
+    g->tpr = threads_per_row((g->nv + 1) / 2, K);
+    if (g->tpr > 512) return 0;
+  }
+  const int set = p->period == 1 && !g->pair ? nga_set_of(*p) : 0;  // (0: dsum never past the ring)
   if (set == 1 && E == (eight ? 8 : 16) && K * g->tpr != g->nv && nga_ragged_tpr(g->tpr) != 0 && g->tpr > 96)
     g->tpr = nga_ragged_tpr(g->tpr);
   rows_per_cta(g);
@@ -590,7 +595,8 @@ static int plan_backward(NgaParams* p, int es, NgaGeom* g) {
   // cost (its partial rows) counts as one more step.
   const int64_t groups = p->rows / p->group_rows, T = p->group_rows;
   const int64_t slots_max = (T + g->R - 1) / g->R;
-  const int64_t cta = (int64_t)usable_sms() * ctas;
+  const int64_t cta = g->pair ? usable_sms() / 2 : (int64_t)usable_sms() * ctas;  // (or pairs of them)
+  if (cta < 1) return 0;
   if (p->period > 1) {
     const int64_t n = (T + p->period - 1) / p->period, per = groups * p->classes;
     int64_t best = 1, best_cost = -1;
@@ -603,7 +609,7 @@ static int plan_backward(NgaParams* p, int es, NgaGeom* g) {
       }
     }
     cut_classes(p, best);
-    g->grid = p->slots < cta ? p->slots : cta;
+    g->grid = (p->slots < cta ? p->slots : cta) * (g->pair ? 2 : 1);
     return p->slots > 0x7fffffff - g->grid ? 0 : K;
   }
   int64_t best = -1, best_cost = 0;
@@ -624,7 +630,7 @@ static int plan_backward(NgaParams* p, int es, NgaGeom* g) {
   p->chunk = ((T + best - 1) / best + g->R - 1) / g->R * g->R;
   p->slots_per_group = (T + p->chunk - 1) / p->chunk;
   p->slots = p->slots_per_group * groups;
-  g->grid = p->slots < cta ? p->slots : cta;
+  g->grid = (p->slots < cta ? p->slots : cta) * (g->pair ? 2 : 1);
   if (p->slots > 0x7fffffff - g->grid) return 0;
   return K;
 }
@@ -704,6 +710,9 @@ extern "C" int fln_norm_gate_add_norm_forward(const fln_nga_args* a, void* y, vo
   if (a->rows == 0) return FLN_OK;
   if (a->x == nullptr || sum == nullptr) return FLN_ERR_NULL;
   if (a->kind != FLN_NO_NORM && y == nullptr) return FLN_ERR_NULL;
+  for (const void* q : {(const void*)y, (const void*)sum})
+    if (q != nullptr && (q == a->x || q == a->residual || q == a->gate)) return FLN_ERR_ARG;
+  if (y == sum) return FLN_ERR_ARG;
   NgaParams p = base_params(a);
   p.y = y;
   p.sum = sum;
@@ -783,6 +792,8 @@ extern "C" int fln_norm_gate_add_norm_backward(const fln_nga_args* a, const floa
   if (a->x == nullptr) return FLN_ERR_NULL;
   if (dy != nullptr && (rstd == nullptr || (a->kind == FLN_LAYERNORM && mean == nullptr)))
     return FLN_ERR_NULL;
+  for (const void* q : {(const void*)dx, (const void*)dresidual, (const void*)dgate})
+    if (q != nullptr && (q == a->x || q == a->residual || q == a->gate || q == dy || q == dsum)) return FLN_ERR_ARG;
   if (a->post_kind != FLN_NO_NORM && (post_rstd == nullptr || (a->post_kind == FLN_LAYERNORM && post_mean == nullptr)))
     return FLN_ERR_NULL;
   NgaParams p = base_params(a);

@@ -17,7 +17,8 @@
 //     C2 = w2, B2 = b2            y  = sh * C2 + B2,                    g2 = dy * C2
 // The column sums P and Q are kept of ds (times a) and multiplied by ba when they are left.
 // The unfolded form on single floats took 48 (forward) and 84 (backward) instructions per element
-// at 16384 x 4096 bf16: 127 and 248 us.
+// at 16384 x 4096 bf16: 127 and 248 us.  As it is: 22 and 28, 90 and 147 us; 16384 x 8192: 170 us (6.3
+// TB/s of the 8 bytes per element) and 262 us (6.1 TB/s of 12), where HBM is the bound.
 //
 // SHIFT: rows that are not whole 16-byte vectors (tensors that start on a 16-byte boundary, row length
 // not a multiple of a vector).  Such a row starts at one of 2, 4 or 8 places of a vector, by its
@@ -25,13 +26,19 @@
 // the same place of the same thread's vectors.  So all that is above holds: the row is staged as
 // the vectors that cover it, what belongs to the neighbouring rows in its first and last vector is
 // set to zero, and only those two are stored element by element.  (Rows held element by element
-// instead: 16384 x 2777 bf16 at 190 us forward and 546 us backward.)
+// instead: 16384 x 2777 bf16 at 190 us forward and 546 us backward; this way 123 and 205.)
+//
+// PAIR (backward): a row is shared by the two CTAs of a cluster, half of its vectors each, where one
+// CTA's registers do not hold it.  The row sums go through the shared memory of both and the
+// cluster's barrier takes the place of the CTA's; both add the same values in the same order.
+// 4096 x 12288 bf16, 12 bytes per element: 235 us, 1590 with the looping kernels.
 //
 // GEN = false: both norms RMSNorm or none and no bias, which is what most blocks have; no means, no
 // Q and V.  GEN = true: everything.
 #pragma once
 
 #include "fln_nga.cuh"
+#include "fln_pipeline.cuh"  // thread-block cluster helpers
 
 namespace fln {
 
@@ -46,6 +53,7 @@ struct NgaGeom {
   size_t smem;
   int csm;      // backward: coefficients in shared memory
   int direct;   // backward: dsum past the ring
+  int pair;     // backward: a row is shared by the two CTAs of a cluster
   int64_t chunk, per_group;  // forward: rows per CTA, CTAs per group
 };
 
@@ -66,6 +74,7 @@ struct RowGroup {
   float mine;  // elements of the row that my warp holds
   float2* red; // [2 buffers][32 warps]
   int flip;
+  int rank;    // in the cluster that shares the row, -1 where there is none
 };
 // (the row lies at elements [shift, shift + cols) of its nv vectors)
 template <int TPR, bool FULL>
@@ -77,6 +86,7 @@ __device__ __forceinline__ RowGroup row_group(const NgaGeom& g, int K, int vec, 
   r.warp0 = tpr <= 32 ? (int)(threadIdx.x >> 5) : (int)(threadIdx.x / tpr) * r.wpr;
   r.red = red;
   r.flip = 0;
+  r.rank = -1;
   auto count = [&](int w) {  // elements of the row in its warp w
     if (FULL) return (float)(K * 32 * vec);
     int n = 0;
@@ -117,20 +127,41 @@ __device__ __forceinline__ float2 warp_exchange(RowGroup& g, float2 mine) {
   const int lane = threadIdx.x & 31;
   return lane < g.wpr ? r[g.warp0 + lane] : make_float2(0.f, 0.f);
 }
+// the same over the two CTAs of a cluster: 16 warps at most of each
+__device__ __forceinline__ float2 pair_exchange(RowGroup& g, float2 mine) {
+  float2* r = g.red + g.flip * 32;
+  g.flip ^= 1;
+  if ((threadIdx.x & 31) == 0) {
+    float2* place = r + g.rank * 16 + (threadIdx.x >> 5);
+    *place = mine;
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(map_to_cta(place, (uint32_t)(g.rank ^ 1))), "f"(mine.x),
+                 "f"(mine.y)
+                 : "memory");
+  }
+  __syncwarp();
+  cluster_sync_all();
+  const int lane = threadIdx.x & 31;
+  return (lane & 15) < g.wpr ? r[lane] : make_float2(0.f, 0.f);
+}
+template <bool PAIR = false>
 __device__ __forceinline__ void row_sum1(RowGroup& g, float& a) {
   float v[1] = {a};
   warp_sum<1>(v, g.width);
-  if (g.wpr > 1) {
+  if (PAIR) {
+    v[0] = pair_exchange(g, make_float2(v[0], 0.f)).x;
+    warp_sum<1>(v, 32);
+  } else if (g.wpr > 1) {
     v[0] = warp_exchange(g, make_float2(v[0], 0.f)).x;
     warp_sum<1>(v, 32);
   }
   a = v[0];
 }
+template <bool PAIR = false>
 __device__ __forceinline__ void row_sum2(RowGroup& g, float& a, float& b) {
   float v[2] = {a, b};
   warp_sum<2>(v, g.width);
-  if (g.wpr > 1) {
-    const float2 o = warp_exchange(g, make_float2(v[0], v[1]));
+  if (PAIR || g.wpr > 1) {
+    const float2 o = PAIR ? pair_exchange(g, make_float2(v[0], v[1])) : warp_exchange(g, make_float2(v[0], v[1]));
     v[0] = o.x;
     v[1] = o.y;
     warp_sum<2>(v, 32);
@@ -215,12 +246,13 @@ struct Places {
   int at[K];
   bool ok[K], edge[SHIFT ? K : 1];
   int lo[SHIFT ? K : 1], hi[SHIFT ? K : 1];
-  __device__ __forceinline__ void set(int lane, int tpr, int nv, int cols, int shift) {
+  // (v0, v1: the vectors of this CTA where two share the row)
+  __device__ __forceinline__ void set(int lane, int tpr, int nv, int cols, int shift, bool pair = false, int v0 = 0, int v1 = 0) {
     if (SHIFT) nv = (shift + cols + VEC - 1) / VEC;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int v = lane + k * tpr;
-      ok[k] = FULL || (!SHIFT && K == 2 && k == 0) || v < nv;  // (tpr <= nv where K is 2)
+      const int v = lane + k * tpr + (pair ? v0 : 0);
+      ok[k] = FULL || (!SHIFT && !pair && K == 2 && k == 0) || (v < nv && (!pair || v < v1));  // (tpr <= nv where K is 2)
       at[k] = (ok[k] ? v : nv - 1) * VEC - (SHIFT ? shift : 0);
       if (SHIFT) {
         lo[SHIFT ? k : 0] = at[k] < 0 ? -at[k] : 0;
@@ -571,7 +603,7 @@ inline int nga_set_of(const NgaParams& p) {
   return 0;
 }
 
-template <typename T, int K, int GATE, bool GEN, bool CSM, int TPR, bool RAG, int SET, bool SHIFT>
+template <typename T, int K, int GATE, bool GEN, bool CSM, int TPR, bool RAG, int SET, bool SHIFT, bool PAIR = false>
 __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_bwd_rows_kernel(const NgaParams p, const NgaGeom g) {
   constexpr bool EXACT = sizeof(T) == 4;
   constexpr int VEC = 16 / (int)sizeof(T), V2 = VEC / 2;
@@ -586,7 +618,7 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
   const int R = TPR ? fixed_rows(TPR) : g.R;
   const int threads = TPR ? TPR * fixed_rows(TPR) : g.threads;
   const int cols = FULL ? TPR * K * VEC : p.cols;
-  constexpr bool ONE = TPR != 0 && fixed_rows(TPR ? TPR : 1) == 1;  // one row at a time: never behind the slot
+  constexpr bool ONE = PAIR || (TPR != 0 && fixed_rows(TPR ? TPR : 1) == 1);  // one row at a time: never behind the slot
   RowGroup rg = row_group<TPR, FULL>(g, K, VEC, g.nv, 0, cols, reinterpret_cast<float2*>(smem));
   const int tid = threadIdx.x;
   const int r_in = ONE ? 0 : tid / tpr, lane = tid - r_in * tpr;
@@ -599,15 +631,21 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
   const uint32_t ring_bytes = (uint32_t)g.stages * stage_bytes;
   // Lanes behind the row work on its last vector, row groups behind the slot on its last row; what
   // goes into the sums is set to zero there and nothing is stored, so the arithmetic has no branches.
+  const int rank = PAIR ? (int)cluster_ctarank() : 0;
+  const int half = (g.nv + 1) / 2, v0 = rank * half, v1 = v0 + half;
+  if (PAIR) {
+    rg.rank = rank;
+    cluster_sync_all();  // the other CTA is there before anything is written into its shared memory
+  }
   Places<K, VEC, FULL, SHIFT> w;
-  if (!SHIFT) w.set(lane, tpr, g.nv, cols, 0);
+  if (!SHIFT) w.set(lane, tpr, g.nv, cols, 0, PAIR, v0, v1);
   const int apart = SHIFT ? p.period : 1;  // from one row to the next
 
   // The row sequence of this CTA: slot after slot, R rows at a time; one walker runs ahead.
   struct Walker {
     int slot, row, last;  // row: of the CTA's first row group
   };
-  const int nslots = (int)p.slots, grid = (int)gridDim.x;
+  const int nslots = (int)p.slots, grid = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
   auto open = [&](Walker& w) {
     if (w.slot < nslots) {
       const SlotRows sr = slot_rows(p, w.slot);
@@ -623,7 +661,7 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
     }
   };
   auto my_row = [&](const Walker& w) { return ONE ? w.row : (w.row + r_in * apart < w.last ? w.row + r_in * apart : w.last - 1); };
-  Walker ahead{(int)blockIdx.x, 0, 0};
+  Walker ahead{PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x, 0, 0};
   open(ahead);
   Walker cur = ahead;
   uint32_t fill = 0;  // byte offset of the stage the walker fills next
@@ -632,7 +670,7 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
       unsigned char* st = stages + fill;
       const int64_t row_at = (int64_t)my_row(ahead) * cols;
       Places<K, VEC, FULL, SHIFT> wa = w;
-      if (SHIFT) wa.set(lane, tpr, g.nv, cols, row_shift(ahead.row, cols, VEC));
+      if (SHIFT) wa.set(lane, tpr, g.nv, cols, row_shift(ahead.row, cols, VEC), PAIR, v0, v1);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         unsigned char* d = st + k * kstep;
@@ -714,7 +752,7 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
   while (cur.slot < nslots) {
     if (opened) {
       const int64_t grp = cur.slot / p.slots_per_group;
-      if (SHIFT) w.set(lane, tpr, g.nv, cols, row_shift(cur.row, cols, VEC));
+      if (SHIFT) w.set(lane, tpr, g.nv, cols, row_shift(cur.row, cols, VEC), PAIR, v0, v1);
       if (SHIFT || grp != group) {  // coefficients of a new group, or for another place of the row
         const bool first = SHIFT || group < 0;
         group = grp;
@@ -816,8 +854,8 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
     float c1 = 0.f, c2 = 0.f;
     if (has_dy) {
       float a = r0.x + r0.y, b = r1.x + r1.y;
-      if (GEN) row_sum2(rg, a, b);
-      else row_sum1(rg, a);
+      if (GEN) row_sum2<PAIR>(rg, a, b);
+      else row_sum1<PAIR>(rg, a);
       c1 = a * inv_n;
       c2 = GEN && p.kind == FLN_LAYERNORM ? b * inv_n : 0.f;
     }
@@ -893,8 +931,8 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
       float d1 = 0.f, d2 = 0.f;
       if (p.post_kind != FLN_NO_NORM) {
         float a = r0.x + r0.y, b = r1.x + r1.y;
-        if (GEN) row_sum2(rg, a, b);
-        else row_sum1(rg, a);
+        if (GEN) row_sum2<PAIR>(rg, a, b);
+        else row_sum1<PAIR>(rg, a);
         d1 = a * inv_n;
         d2 = GEN && p.post_kind == FLN_LAYERNORM ? b * inv_n : 0.f;
       }
@@ -987,6 +1025,29 @@ inline bool nga_general(const NgaParams& p) {
          (p.acc & (kAccQ | kAccV)) != 0;
 }
 
+// clusters of two CTAs
+template <auto KERN>
+static int nga_launch_pair(const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
+  if (!allow_smem<KERN>(g.smem)) return FLN_ERR_LAUNCH;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)g.grid);
+  cfg.blockDim = dim3((unsigned)g.threads);
+  cfg.dynamicSmemBytes = g.smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 2;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, KERN, p, g) != cudaSuccess) {
+    cudaGetLastError();
+    return FLN_ERR_LAUNCH;
+  }
+  FLN_CHECK_LAUNCH();
+  return FLN_OK;
+}
 template <auto KERN>
 static int nga_launch(const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
   if (!allow_smem<KERN>(g.smem)) return FLN_ERR_LAUNCH;
@@ -1046,6 +1107,16 @@ static int nga_fwd_rows_k(const NgaParams& p, const NgaGeom& g, cudaStream_t st)
 }
 template <typename T, int K, int GATE, bool GEN>
 static int nga_bwd_rows_g(const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
+  if (g.pair) {
+    if constexpr (K * 16 / (int)sizeof(T) == 16) {
+      if (p.period > 1)
+        return g.csm ? nga_launch_pair<nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 0, true, true>>(p, g, st)
+                     : nga_launch_pair<nga_bwd_rows_kernel<T, K, GATE, GEN, false, 0, false, 0, true, true>>(p, g, st);
+      return g.csm ? nga_launch_pair<nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 0, false, true>>(p, g, st)
+                   : nga_launch_pair<nga_bwd_rows_kernel<T, K, GATE, GEN, false, 0, false, 0, false, true>>(p, g, st);
+    }
+    return FLN_ERR_UNSUPPORTED;
+  }
   if (p.period > 1) {
     if (!g.csm) return nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, false, 0, false, 0, true>>(p, g, st);
     return nga_set_of(p) == 1 ? nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 1, true>>(p, g, st)

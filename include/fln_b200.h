@@ -428,7 +428,8 @@ typedef struct {
   float branch_scale, residual_scale, weight_offset, post_eps, eps;
 } fln_nga_args;
 
-/* y may be NULL when kind is FLN_NO_NORM, and only then.  The statistics (fp32 [rows], each may
+/* y may be NULL when kind is FLN_NO_NORM, and only then.  Outputs may not overlap inputs (a row can
+ * be read again after it was written).  The statistics (fp32 [rows], each may
  * be NULL) are what the backward reads: post_mean / mean of a LayerNorm, post_rstd / rstd of
  * either norm. */
 int fln_norm_gate_add_norm_forward(const fln_nga_args* a, void* y, void* sum, float* post_mean, float* post_rstd,

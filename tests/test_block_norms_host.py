@@ -29,11 +29,16 @@ def test_norm_gate_add_norm_argument_errors():
                    (dict(), 3)):
         assert fwd(nga(**kw)) == st, kw
     assert fwd(nga(rows=0)) == 0
+    # outputs may not be inputs
+    for y, total in ((64, 128), (128, 64), (128, 128)):
+        a = nga(x=64, residual=64)
+        assert L.fln_norm_gate_add_norm_forward(C.byref(a), y, total, *[None] * 5) == 8
     bwd = lambda a, p, n=0: L.fln_norm_gate_add_norm_backward(C.byref(a), *p, n, None)
     none = [None] * 14
     assert bwd(nga(), none) == 3  # no gradient arrives
     assert bwd(nga(), none[:8] + [64] + none[9:]) == 8  # dgate without a gate
     assert bwd(nga(x=64), [64] * 6 + [None] * 5 + [64] + [None] * 2) == 4  # dweight without scratch
+    assert bwd(nga(x=64), [64] * 6 + [64] + [None] * 7) == 8  # dx over x
     assert L.fln_norm_gate_add_norm_workspace_bytes(C.byref(nga(kind=7))) == 0
     assert L.fln_norm_gate_add_norm_workspace_bytes(C.byref(nga())) > 0
 

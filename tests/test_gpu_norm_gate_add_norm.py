@@ -102,6 +102,35 @@ def test_groups_of_every_length(dtype, affine, gate):
                          act="tanh" if gate != "none" else "none", off=1.0, seed=i))
 
 
+@pytest.mark.parametrize("shape,dtype", [((3, 8200), F32), ((2, 11, 9984), F16), ((200, 10007), BF16), ((2, 90, 16384), BF16),
+                                         ((5, 16383), F32), ((3, 16392), F16)], ids=lambda v: str(v).replace("torch.", ""))
+def test_long_rows(shape, dtype):
+    """Rows that two CTAs share in the backward, and rows beyond those; whole vectors and not."""
+    for i in range(6):
+        check_case(*make(shape, dtype, **KINDS[i], **GATES[(i + len(shape)) % 6], off=float(i % 2), seed=i, ba=0.7))
+
+
+@pytest.mark.parametrize("h", [1, 2, 3, 5, 9, 31, 65, 130, 257, 333, 511, 1001, 2050, 2777, 4100, 5121, 6007, 7998])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_rows_that_start_anywhere_in_a_vector(h, dtype):
+    """Row lengths that are not whole vectors: every class of starting places, groups shorter than
+    the number of classes, neighbours with infinities in the same vectors."""
+    i = h % 6
+    for b, n in ((1, 67), (5, 3), (9, 1)):
+        check_case(*make((b, n, h), dtype, **KINDS[i], **GATES[(i + n) % 6], off=float(h % 2), seed=h + n))
+    t, dy, ds, conf = make((33, h), dtype, post="layernorm", norm="layernorm", bias=True)
+    want = call(t, conf)
+    grads = lambda v: torch.autograd.grad(call(v, conf), [v["input"], v["residual"]], [dy, ds])
+    leaves = lambda v: {k: (None if x is None else x.detach().requires_grad_(True)) for k, x in v.items()}
+    g = grads(leaves(t))
+    bad = {k: (None if v is None else v.clone()) for k, v in t.items()}
+    bad["input"][1::2] = float("inf")
+    bad["residual"][1::2] = float("nan")
+    got, gb = call(bad, conf), grads(leaves(bad))
+    for a, b in zip((*got, *gb), (*want, *g)):
+        assert torch.equal(a[::2], b[::2])
+
+
 def test_more_groups_than_partial_rows_and_many_rows():
     check_case(*make((1500, 2, 72), BF16, gate="group", affine="group", seed=3))
     check_case(*make((70001, 16), F32, bias=True, post="layernorm", norm="layernorm", seed=4))
@@ -308,6 +337,37 @@ def test_two_graphs_replayed_in_turn():
         for g, leaves, out, step in graphs:
             for a, b in zip(out, step()):
                 assert torch.equal(a, b)
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2**31 elements in each tensor: the last rows and the sums over all rows."""
+    rows, h = 262200, 8200  # 2.15e9 elements
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.empty(rows, h, dtype=BF16, device="cuda").normal_(generator=g)
+    r = torch.empty(rows, h, dtype=BF16, device="cuda").normal_(generator=g)
+    w1, w2 = (torch.randn(h, device="cuda", generator=g).to(BF16) for _ in range(2))
+    leaves = [v.requires_grad_(True) for v in (x, r, w1, w2)]
+    y, s = fl.fused_norm_gate_add_norm(x, r, None, w1, None, w2, post_eps=R.EPS1, eps=R.EPS2)
+    one = torch.ones((), dtype=BF16, device="cuda").expand_as(y)
+    dx, dr, dw1, dw2 = torch.autograd.grad([y], leaves, [one])
+    for part in (slice(0, 2), slice(rows // 2, rows // 2 + 2), slice(rows - 2, rows)):
+        t = dict.fromkeys(R.NAMES)
+        t.update(input=x[part], residual=r[part], post_weight=w1, weight=w2)
+        conf = dict(post_norm="rmsnorm", norm="rmsnorm", gate_activation="none", branch_scale=1.0, residual_scale=1.0, weight_offset=0.0)
+        want = bounds(t, one[part], None, conf)
+        R.check(y[part], want["y"], "y"), R.check(s[part], want["sum"], "sum")
+        R.check(dx[part], want["grads"]["input"], "dx"), R.check(dr[part], want["grads"]["residual"], "dresidual")
+    # dweight = sum of sh: |sh| sums to about 0.8 rows, each term is good to 2**-14 (e24 of the bounds
+    # at this row length), the sum's rounding is half a step of bf16
+    total = torch.zeros(h, dtype=torch.float64, device="cuda")
+    size = torch.zeros_like(total)
+    with torch.no_grad():
+        for i in range(0, rows, 8740):
+            v = R.norm_of(x[i:i + 8740].double(), "rmsnorm", w1.double(), None, 0.0, R.EPS1)[0] + r[i:i + 8740].double()
+            sh = v / torch.sqrt((v * v).mean(-1, keepdim=True) + R.EPS2)
+            total += sh.sum(0)
+            size += sh.abs().sum(0)
+    R.check(dw2, (total, R.u_of(BF16) * total.abs() + (2.0 ** -14 + (64 + rows / 64) * 2.0 ** -24) * size), "dweight")
 
 
 def test_refusals():

@@ -164,6 +164,24 @@ def test_far_positions_are_exact():
     assert torch.equal(fl.fused_qk_norm_rotary(q[:5], None, small.int(), rot, norm="none")[0], out[:5])
 
 
+def test_offsets_beyond_32_bits():
+    """Tokens of a packed projection that lie past 2**31 elements, and dx past them."""
+    n, hq, hk, dim = 210000, 70, 10, 128  # 90 heads of 128 in a row of the projection: 2.4e9 elements
+    rot = fl.RotaryAxes(dim, (16, 24, 24))
+    qkv = torch.empty(n, hq + 2 * hk, dim, dtype=BF16, device="cuda").normal_()
+    q, k = qkv[:, :hq].detach().requires_grad_(True), qkv[:, hq:hq + hk].detach().requires_grad_(True)
+    pos = positions((n,), 3)
+    qo, ko = fl.fused_qk_norm_rotary(q, k, pos, rot, eps=EPS)
+    dq, dk = torch.empty_like(qo).normal_(), torch.empty_like(ko).normal_()
+    gq, gk = torch.autograd.grad([qo, ko], [q, k], [dq, dk])
+    for part in (slice(0, 3), slice(n - 3, n)):
+        t = {"q": q[part].detach(), "k": k[part].detach(), "dq": dq[part], "dk": dk[part],
+             **dict.fromkeys(("q_weight", "k_weight", "q_bias", "k_bias"))}
+        for s, o, gr in (("q", qo, gq), ("k", ko, gk)):
+            want = bounds(t, pos[:, part], rot, "rmsnorm", 0.0, s)
+            R.check(o[part], want["value"], s), R.check(gr[part], want["dx"], "d" + s)
+
+
 def test_position_shapes():
     t = make((3, 10), 2, 1, 64, F32)
     one, three = fl.RotaryAxes(64, 32), fl.RotaryAxes(64, (8, 12, 12))
