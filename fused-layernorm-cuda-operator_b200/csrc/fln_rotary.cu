@@ -14,12 +14,13 @@ int rotary_launch<__nv_bfloat16>(const RotParams&, const RotPlan&, bool, unsigne
 template <>
 int rotary_launch<__half>(const RotParams&, const RotPlan&, bool, unsigned, cudaStream_t);
 
-// One CTA per 32 columns of one output row; 8 lanes take the partial rows in turn, the lanes are
+// One CTA per 32 columns of one output row; 32 lanes take the partial rows in turn, the lanes are
 // added in order.
+constexpr int kRotFinalLanes = 32;
 template <typename T>
-__global__ void __launch_bounds__(256) rotary_finalize_kernel(const float* p0, int n0, const float* p1, int n1, int dim,
+__global__ void __launch_bounds__(32 * kRotFinalLanes) rotary_finalize_kernel(const float* p0, int n0, const float* p1, int n1, int dim,
                                                               T* dw0, T* db0, T* dw1, T* db1) {
-  __shared__ float tile[8][33];
+  __shared__ float tile[kRotFinalLanes][33];
   const int which = blockIdx.y >> 1, bias = blockIdx.y & 1;
   T* out = which == 0 ? (bias ? db0 : dw0) : (bias ? db1 : dw1);
   if (out == nullptr) return;
@@ -30,22 +31,20 @@ __global__ void __launch_bounds__(256) rotary_finalize_kernel(const float* p0, i
   float v = 0.f;
   if (c < dim) {
     const float* s = src + bias * dim + c;
-    int r = lane;
-    for (; r + 56 < n; r += 64) {
-      float q[8];
+    for (int r = lane; r < n; r += 4 * kRotFinalLanes) {
+      float q[4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) q[j] = __ldcg(s + (int64_t)(r + j * 8) * 2 * dim);
+      for (int j = 0; j < 4; ++j) q[j] = r + j * kRotFinalLanes < n ? __ldcg(s + (int64_t)(r + j * kRotFinalLanes) * 2 * dim) : 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v += q[j];
+      for (int j = 0; j < 4; ++j) v += q[j];
     }
-    for (; r < n; r += 8) v += __ldcg(s + (int64_t)r * 2 * dim);
   }
   tile[lane][tx] = v;
   __syncthreads();
   if (lane == 0 && c < dim) {
     v = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v += tile[i][tx];
+    for (int i = 0; i < kRotFinalLanes; ++i) v += tile[i][tx];
     out[c] = Cvt<T>::from_f(v);
   }
 }
@@ -157,21 +156,6 @@ static RotParams base_params(const fln_rotary_args* a) {
   return p;
 }
 
-// Heads per item: all of them (the angles are made once per token) unless that leaves warps
-// without work; then fewer, down to one per row group.
-static void split_heads(int tokens, int heads, int groups, int64_t warps, int* splits, int* per) {
-  int n = 1;
-  const int most = (heads + groups - 1) / groups;
-  while (n < most && (int64_t)tokens * n < warps) n <<= 1;
-  if (n > most) n = most;
-  if (n < 1) n = 1;
-  int each = (heads + n - 1) / n;
-  each = (each + groups - 1) / groups * groups;
-  if (each < 1) each = 1;
-  *per = each;
-  *splits = heads > 0 ? (heads + each - 1) / each : 1;
-}
-
 static int launch(int dtype, const RotParams& p, const RotPlan& plan, bool backward, unsigned grid, cudaStream_t st) {
   switch (dtype) {
     case FLN_F32:
@@ -186,10 +170,13 @@ static int launch(int dtype, const RotParams& p, const RotPlan& plan, bool backw
 constexpr int kRotBwdCtasPerSm = 2;
 
 // CTAs of the backward for q and for k: in proportion to their heads, at least one for a tensor
-// that has any
+// that has any, and not more than one per eight rows
 static void bwd_grid(const fln_rotary_args* a, int* n0, int* n1) {
   const int h0 = a->t[0].heads, h1 = a->t[1].heads;
-  const int all = sm_count() * kRotBwdCtasPerSm;
+  int64_t most = (a->batch * a->seq * (h0 + h1) + 7) / 8;
+  if (most < 2) most = 2;
+  int all = sm_count() * kRotBwdCtasPerSm;
+  if (all > most) all = (int)most;
   int q = (int)((int64_t)all * h0 / (h0 + h1));
   if (h0 > 0 && q < 1) q = 1;
   if (h1 > 0 && q > all - 1) q = all - 1;
@@ -210,12 +197,7 @@ extern "C" int fln_qk_norm_rotary_forward(const fln_rotary_args* a, void* stream
   if (rc != FLN_OK) return rc;
   RotParams p = base_params(a);
   const RotPlan plan = make_rot_plan(a, nullptr, &p);
-  const int64_t warps = (int64_t)sm_count() * 32;
-  split_heads(p.tokens, p.t[0].heads + p.t[1].heads, 32 >> p.log2_l, warps, &p.splits[0], &p.per_split[0]);
-  const int64_t items = (int64_t)p.tokens * p.splits[0];
-  int64_t grid = (items + kRotThreads / 32 - 1) / (kRotThreads / 32);
-  if (grid > 0x7fffffff) grid = 0x7fffffff;
-  return launch(a->dtype, p, plan, false, (unsigned)grid, reinterpret_cast<cudaStream_t>(stream));
+  return launch(a->dtype, p, plan, false, 0, reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" size_t fln_qk_norm_rotary_workspace_bytes(const fln_rotary_args* a) {
@@ -264,15 +246,13 @@ extern "C" int fln_qk_norm_rotary_backward(const fln_rotary_args* a, void* const
     p.t[i].partials = (dweight[i] != nullptr || dbias[i] != nullptr) && p.t[i].heads > 0
                           ? ws + (i == 0 ? 0 : (int64_t)n0 * 2 * p.dim)
                           : nullptr;
-    const int64_t warps = (int64_t)(i == 0 ? n0 : n1) * (kRotThreads / 32);
-    split_heads(p.tokens, p.t[i].heads, 32 >> p.log2_l, warps, &p.splits[i], &p.per_split[i]);
   }
   rc = launch(a->dtype, p, plan, true, (unsigned)(n0 + n1), st);
   if (rc != FLN_OK || !sums) return rc;
   const dim3 grid((unsigned)((p.dim + 31) / 32), 4);
   auto own = [&](int i, void* q) { return p.t[i].heads > 0 ? q : nullptr; };
 #define FLN_FIN(T)                                                                                                     \
-  rotary_finalize_kernel<T><<<grid, 256, 0, st>>>(p.t[0].partials, n0, p.t[1].partials, n1, p.dim,                     \
+  rotary_finalize_kernel<T><<<grid, 32 * kRotFinalLanes, 0, st>>>(p.t[0].partials, n0, p.t[1].partials, n1, p.dim,                     \
                                                   reinterpret_cast<T*>(own(0, dweight[0])),                            \
                                                   reinterpret_cast<T*>(own(0, dbias[0])),                              \
                                                   reinterpret_cast<T*>(own(1, dweight[1])),                            \

@@ -45,10 +45,7 @@ struct RotParams {
   int log2_l;            // lanes per row
   int pos64, kind;
   float woff, eps, mag;
-  // forward: items = tokens * splits, each a run of `per_split` heads of the q heads followed by
-  // the k heads.  backward: the first nb0 CTAs take q, the others k; items of `per_split` heads.
-  int splits[2], per_split[2];
-  int nb0;
+  int nb0;      // backward: the first nb0 CTAs take q, the others k
   int want_db;  // a bias gradient is asked for
 };
 
@@ -290,12 +287,14 @@ struct RotLane {
 };
 
 // ----------------------------------------------------------------------------------------
-// forward: a warp takes items (token, run of heads); each of its 32 / L row groups takes every
-// (32 / L)-th head of the run, NB of them at a time so that NB rows are on their way from memory
-// together.  All lanes of a warp make the same number of turns, so the shuffles are whole.  The
-// rows stay packed as they came; they are unpacked once for the sums and once more for the
-// result, which costs an instruction per element and saves the registers that let more warps
-// (and so more loads) be in flight.
+// forward: the work is one sequence of steps, token after token; a step is NB heads of q or of k for
+// each of a warp's 32 / L row groups, so that NB rows per group are on their way from memory
+// together.  The warps of as many CTAs as are resident at once take equal runs of it (with a token
+// per warp and its CTA's tables made for eight tokens, 8192 x 48 x 128 bf16 took 44 us, 40 so); a run
+// that starts inside a token makes that token's angles again.  All lanes of a warp take part in
+// every step, so the shuffles are whole.  The rows stay packed as they came; they are unpacked once
+// for the sums and once more for the result, which costs an instruction per element and saves the
+// registers that let more warps (and so more loads) be in flight.
 // GEN: layer norm or bias.  LL >= 0: log2 of the lanes per row, known at compile time.
 // ----------------------------------------------------------------------------------------
 template <typename T, int V, int U, bool HALF, int NB, bool GEN, int LL>
@@ -306,115 +305,112 @@ __global__ void __launch_bounds__(kRotThreads, rot_blocks(V * U, false)) rotary_
   const RotTables tab = rot_tables<T, V, GEN>(p, tables);
   constexpr bool WHOLE = LL >= 0;
   const float inv_d = 1.0f / (float)p.dim;
-  const int splits = p.splits[0], per = p.per_split[0];
-  const int64_t items = (int64_t)p.tokens * splits;
-  const int64_t stride = (int64_t)gridDim.x * (kRotThreads / 32);
-  const int q_heads = p.t[0].heads, heads_all = q_heads + p.t[1].heads;
-  for (int64_t it = (int64_t)blockIdx.x * (kRotThreads / 32) + (threadIdx.x >> 5); it < items; it += stride) {
-    int token, h0 = 0, h1 = heads_all;
-    if (splits == 1) {
-      token = (int)it;
-    } else {
-      token = (int)(it / splits);
-      h0 = (int)(it - (int64_t)token * splits) * per;
-      h1 = h0 + per < heads_all ? h0 + per : heads_all;
+  const int q_heads = p.t[0].heads, turn = r.groups * NB;
+  const int q_steps = (q_heads + turn - 1) / turn, steps = q_steps + (p.t[1].heads + turn - 1) / turn;
+  const int64_t total = (int64_t)p.tokens * steps, warps = (int64_t)gridDim.x * (kRotThreads / 32);
+  const int64_t me = (int64_t)blockIdx.x * (kRotThreads / 32) + (threadIdx.x >> 5);
+  const int64_t lo = total * me / warps, hi = total * (me + 1) / warps;
+  int token = (int)(lo / steps), step = (int)(lo - (int64_t)token * steps);
+  int b = 0, s = 0;
+  bool fresh = true;
+#pragma unroll 1
+  for (int64_t i = lo; i < hi; ++i) {
+    if (fresh) {
+      b = p.tokens == p.seq ? 0 : token / p.seq;
+      s = token - b * p.seq;
     }
-    const int b = p.tokens == p.seq ? 0 : token / p.seq, s = token - b * p.seq;
-    bool angles = false;
-#pragma unroll 1
-    for (int which = 0; which < 2; ++which) {
-      const RotTensor& t = p.t[which];
-      const int first = which == 0 ? h0 : (h0 > q_heads ? h0 - q_heads : 0);
-      const int end = which == 0 ? (h1 < q_heads ? h1 : q_heads) : h1 - q_heads;
-      if (first >= end) continue;
-      const T* in = reinterpret_cast<const T*>(t.in) + (int64_t)b * t.in_batch + (int64_t)s * t.in_seq;
-      T* out = reinterpret_cast<T*>(t.out) + (int64_t)b * t.out_batch + (int64_t)s * t.out_seq;
-#pragma unroll 1
-      for (int h = first; h < end; h += r.groups * NB) {
-        UnitPack<T, V> x[NB][U];
+    const int which = step >= q_steps ? 1 : 0;
+    const RotTensor& t = p.t[which];
+    const int h = (step - (which == 0 ? 0 : q_steps)) * turn, end = t.heads;
+    const T* in = reinterpret_cast<const T*>(t.in) + (int64_t)b * t.in_batch + (int64_t)s * t.in_seq;
+    T* out = reinterpret_cast<T*>(t.out) + (int64_t)b * t.out_batch + (int64_t)s * t.out_seq;
+    UnitPack<T, V> x[NB][U];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      // (row groups behind the last head take it once more and store nothing)
+      const int hh = min(h + n * r.groups + r.grp, end - 1);
+      const T* row = in + (int64_t)hh * t.in_head;
+#pragma unroll
+      for (int k = 0; k < U; ++k) x[n][k] = unit_load<T, V, WHOLE>(row, r.lo[k], r.hi[k], r.lo_ok[k], r.hi_ok[k]);
+    }
+    if (fresh) {  // behind the loads, so that both wait for memory together
+      fresh = false;
+      token_angles(p, tab, b, s);
+    }
+    float mean[NB], rstd[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      mean[n] = 0.f;
+      rstd[n] = 1.f;
+    }
+    if (p.kind != FLN_NO_NORM) {
+      float v[NB];
+      if (GEN && p.kind == FLN_LAYERNORM) {
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-          // (row groups behind the last head take it once more and store nothing)
-          const int hh = min(h + n * r.groups + r.grp, end - 1);
-          const T* row = in + (int64_t)hh * t.in_head;
-#pragma unroll
-          for (int k = 0; k < U; ++k) x[n][k] = unit_load<T, V, WHOLE>(row, r.lo[k], r.hi[k], r.lo_ok[k], r.hi_ok[k]);
-        }
-        if (!angles) {  // behind the first loads, so that both wait for memory together
-          angles = true;
-          token_angles(p, tab, b, s);
-        }
-        float mean[NB], rstd[NB];
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          mean[n] = 0.f;
-          rstd[n] = 1.f;
-        }
-        if (p.kind != FLN_NO_NORM) {
-          float v[NB];
-          if (GEN && p.kind == FLN_LAYERNORM) {
-#pragma unroll
-            for (int n = 0; n < NB; ++n) {
-              float2 a = f2(0.f);
-#pragma unroll
-              for (int k = 0; k < U; ++k) {
-                float2 f[V];
-                unit_unpack<T, V>(x[n][k], f);
-#pragma unroll
-                for (int j = 0; j < V; ++j) a = f2add(a, f[j]);
-              }
-              v[n] = a.x + a.y;
-            }
-            lane_sum<NB, LL>(v, p.log2_l);
-#pragma unroll
-            for (int n = 0; n < NB; ++n) mean[n] = v[n] * inv_d;
-          }
-#pragma unroll
-          for (int n = 0; n < NB; ++n) {
-            float2 a = f2(0.f);
-#pragma unroll
-            for (int k = 0; k < U; ++k) {
-              float2 f[V];
-              unit_unpack<T, V>(x[n][k], f);
-#pragma unroll
-              for (int j = 0; j < V; ++j) {
-                if (GEN) {
-                  f[j] = f2add(f[j], f2(-mean[n]));
-                  if (!WHOLE) f[j] = in_row<V>(f[j], j, r.lo_ok[k], r.hi_ok[k]);
-                }
-                a = f2fma(f[j], f[j], a);
-              }
-            }
-            v[n] = a.x + a.y;
-          }
-          lane_sum<NB, LL>(v, p.log2_l);
-#pragma unroll
-          for (int n = 0; n < NB; ++n) rstd[n] = rsqrtf(fmaf(v[n], inv_d, p.eps));
-        }
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          const int hh = h + n * r.groups + r.grp;
-          T* row = out + (int64_t)hh * t.out_head;
+          float2 a = f2(0.f);
 #pragma unroll
           for (int k = 0; k < U; ++k) {
-            float2 f[V], w[V], bi[V];
-            float cs[V], sn[V];
+            float2 f[V];
             unit_unpack<T, V>(x[n][k], f);
-            table_unit<V>(tab.w + which * tab.step, r.lo[k], r.hi[k], w);
-            if (GEN) table_unit<V>(tab.b + which * tab.step, r.lo[k], r.hi[k], bi);
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-              if (GEN) f[j] = f2add(f[j], f2(-mean[n]));
-              f[j] = f2mul(f[j], f2(rstd[n]));
-              f[j] = GEN ? f2fma(f[j], w[j], bi[j]) : f2mul(f[j], w[j]);
+            for (int j = 0; j < V; ++j) a = f2add(a, f[j]);
+          }
+          v[n] = a.x + a.y;
+        }
+        lane_sum<NB, LL>(v, p.log2_l);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) mean[n] = v[n] * inv_d;
+      }
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        float2 a = f2(0.f);
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          float2 f[V];
+          unit_unpack<T, V>(x[n][k], f);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            if (GEN) {
+              f[j] = f2add(f[j], f2(-mean[n]));
+              if (!WHOLE) f[j] = in_row<V>(f[j], j, r.lo_ok[k], r.hi_ok[k]);
             }
-            table_take<V>(tab.c + r.at[k], cs);
-            table_take<V>(tab.s + r.at[k], sn);
-            unit_rotate<V, HALF, false>(f, cs, sn);
-            if (hh < end && r.lo_ok[k]) unit_store<T, V>(row, r.lo[k], r.hi[k], r.hi_ok[k], f);
+            a = f2fma(f[j], f[j], a);
           }
         }
+        v[n] = a.x + a.y;
       }
+      lane_sum<NB, LL>(v, p.log2_l);
+#pragma unroll
+      for (int n = 0; n < NB; ++n) rstd[n] = rsqrtf(fmaf(v[n], inv_d, p.eps));
+    }
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const int hh = h + n * r.groups + r.grp;
+      T* row = out + (int64_t)hh * t.out_head;
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        float2 f[V], w[V], bi[V];
+        float cs[V], sn[V];
+        unit_unpack<T, V>(x[n][k], f);
+        table_unit<V>(tab.w + which * tab.step, r.lo[k], r.hi[k], w);
+        if (GEN) table_unit<V>(tab.b + which * tab.step, r.lo[k], r.hi[k], bi);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          if (GEN) f[j] = f2add(f[j], f2(-mean[n]));
+          f[j] = f2mul(f[j], f2(rstd[n]));
+          f[j] = GEN ? f2fma(f[j], w[j], bi[j]) : f2mul(f[j], w[j]);
+        }
+        table_take<V>(tab.c + r.at[k], cs);
+        table_take<V>(tab.s + r.at[k], sn);
+        unit_rotate<V, HALF, false>(f, cs, sn);
+        if (hh < end && r.lo_ok[k]) unit_store<T, V>(row, r.lo[k], r.hi[k], r.hi_ok[k], f);
+      }
+    }
+    if (++step == steps) {
+      step = 0;
+      ++token;
+      fresh = true;
     }
   }
 }
@@ -450,105 +446,69 @@ __global__ void __launch_bounds__(kRotThreads, rot_blocks(V * U, true)) rotary_b
     }
   }
   const float inv_d = 1.0f / (float)p.dim;
-  const int splits = p.splits[which], per = p.per_split[which];
-  const int64_t items = (int64_t)p.tokens * splits;
-  const int64_t stride = (int64_t)ctas * (kRotThreads / 32);
-  for (int64_t it = (int64_t)cta * (kRotThreads / 32) + warp; it < items; it += stride) {
-    int token, h0 = 0, end = t.heads;
-    if (splits == 1) {
-      token = (int)it;
-    } else {
-      token = (int)(it / splits);
-      h0 = (int)(it - (int64_t)token * splits) * per;
-      end = h0 + per < t.heads ? h0 + per : t.heads;
+  const int turn = r.groups * NB, steps = (t.heads + turn - 1) / turn;
+  const int64_t total = (int64_t)p.tokens * steps, warps = (int64_t)ctas * (kRotThreads / 32);
+  const int64_t me = (int64_t)cta * (kRotThreads / 32) + warp;
+  const int64_t lo = total * me / warps, hi = total * (me + 1) / warps;
+  int token = (int)(lo / steps), step = (int)(lo - (int64_t)token * steps);
+  int b = 0, s = 0;
+  bool fresh = true;
+#pragma unroll 1
+  for (int64_t i = lo; i < hi; ++i) {
+    if (fresh) {
+      b = p.tokens == p.seq ? 0 : token / p.seq;
+      s = token - b * p.seq;
     }
-    const int b = p.tokens == p.seq ? 0 : token / p.seq, s = token - b * p.seq;
+    const int h = step * turn, end = t.heads;
     const T* in = reinterpret_cast<const T*>(t.in) + (int64_t)b * t.in_batch + (int64_t)s * t.in_seq;
     const T* go = reinterpret_cast<const T*>(t.out) + (int64_t)b * t.out_batch + (int64_t)s * t.out_seq;
     T* dx = reinterpret_cast<T*>(t.dx) + (int64_t)token * t.heads * p.dim;
-#pragma unroll 1
-    for (int h = h0; h < end; h += r.groups * NB) {
-      UnitPack<T, V> px[NB][U], pg[NB][U];
+    UnitPack<T, V> px[NB][U], pg[NB][U];
 #pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        // (row groups behind the last head read it once more; their gradient is zero)
-        const int hh = min(h + n * r.groups + r.grp, end - 1);
+    for (int n = 0; n < NB; ++n) {
+      // (row groups behind the last head read it once more; their gradient is zero)
+      const int hh = min(h + n * r.groups + r.grp, end - 1);
 #pragma unroll
-        for (int k = 0; k < U; ++k) {
-          px[n][k] = unit_load<T, V, WHOLE>(in + (int64_t)hh * t.in_head, r.lo[k], r.hi[k], r.lo_ok[k], r.hi_ok[k]);
-          pg[n][k] = unit_load<T, V, WHOLE>(go + (int64_t)hh * t.out_head, r.lo[k], r.hi[k], r.lo_ok[k], r.hi_ok[k]);
-        }
+      for (int k = 0; k < U; ++k) {
+        px[n][k] = unit_load<T, V, WHOLE>(in + (int64_t)hh * t.in_head, r.lo[k], r.hi[k], r.lo_ok[k], r.hi_ok[k]);
+        pg[n][k] = unit_load<T, V, WHOLE>(go + (int64_t)hh * t.out_head, r.lo[k], r.hi[k], r.lo_ok[k], r.hi_ok[k]);
       }
-      if (h == h0) token_angles(p, tab, b, s);
-      float mean[NB], rstd[NB], c1[NB], c2[NB];
+    }
+    if (fresh) {
+      fresh = false;
+      token_angles(p, tab, b, s);
+    }
+    float mean[NB], rstd[NB], c1[NB], c2[NB];
 #pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        mean[n] = 0.f;
-        rstd[n] = 1.f;
-        c1[n] = c2[n] = 0.f;
-      }
-      if (p.kind != FLN_NO_NORM) {
-        if (GEN && p.kind == FLN_LAYERNORM) {
-          float v[NB];
-#pragma unroll
-          for (int n = 0; n < NB; ++n) {
-            float2 a = f2(0.f);
-#pragma unroll
-            for (int k = 0; k < U; ++k) {
-              float2 f[V];
-              unit_unpack<T, V>(px[n][k], f);
-#pragma unroll
-              for (int j = 0; j < V; ++j) a = f2add(a, f[j]);
-            }
-            v[n] = a.x + a.y;
-          }
-          lane_sum<NB, LL>(v, p.log2_l);
-#pragma unroll
-          for (int n = 0; n < NB; ++n) mean[n] = v[n] * inv_d;
-        }
-        constexpr int NS = GEN ? 3 : 2;
-        float v[NS * NB];  // the squares, g times the centred row, g
+    for (int n = 0; n < NB; ++n) {
+      mean[n] = 0.f;
+      rstd[n] = 1.f;
+      c1[n] = c2[n] = 0.f;
+    }
+    if (p.kind != FLN_NO_NORM) {
+      if (GEN && p.kind == FLN_LAYERNORM) {
+        float v[NB];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-          float2 a = f2(0.f), gx = f2(0.f), gs = f2(0.f);
+          float2 a = f2(0.f);
 #pragma unroll
           for (int k = 0; k < U; ++k) {
-            float2 x[V], g[V], w[V];
-            float cs[V], sn[V];
-            unit_unpack<T, V>(px[n][k], x);
-            unit_unpack<T, V>(pg[n][k], g);
-            table_take<V>(tab.c + r.at[k], cs);
-            table_take<V>(tab.s + r.at[k], sn);
-            unit_rotate<V, HALF, true>(g, cs, sn);
-            table_unit<V>(tab.w + which * tab.step, r.lo[k], r.hi[k], w);
+            float2 f[V];
+            unit_unpack<T, V>(px[n][k], f);
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-              if (GEN) {
-                x[j] = f2add(x[j], f2(-mean[n]));
-                if (!WHOLE) x[j] = in_row<V>(x[j], j, r.lo_ok[k], r.hi_ok[k]);
-              }
-              const float2 q = f2mul(g[j], w[j]);
-              a = f2fma(x[j], x[j], a);
-              gx = f2fma(q, x[j], gx);
-              if (GEN) gs = f2add(gs, q);
-            }
+            for (int j = 0; j < V; ++j) a = f2add(a, f[j]);
           }
-          v[NS * n] = a.x + a.y;
-          v[NS * n + 1] = gx.x + gx.y;
-          if (GEN) v[NS * n + NS - 1] = gs.x + gs.y;
+          v[n] = a.x + a.y;
         }
-        lane_sum<NS * NB, LL>(v, p.log2_l);
+        lane_sum<NB, LL>(v, p.log2_l);
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          rstd[n] = rsqrtf(fmaf(v[NS * n], inv_d, p.eps));
-          c1[n] = rstd[n] * v[NS * n + 1] * inv_d;
-          if (GEN && p.kind == FLN_LAYERNORM) c2[n] = v[NS * n + NS - 1] * inv_d;
-        }
+        for (int n = 0; n < NB; ++n) mean[n] = v[n] * inv_d;
       }
+      constexpr int NS = GEN ? 3 : 2;
+      float v[NS * NB];  // the squares, g times the centred row, g
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
-        const int hh = h + n * r.groups + r.grp;
-        const bool live = hh < end;
+        float2 a = f2(0.f), gx = f2(0.f), gs = f2(0.f);
 #pragma unroll
         for (int k = 0; k < U; ++k) {
           float2 x[V], g[V], w[V];
@@ -561,22 +521,64 @@ __global__ void __launch_bounds__(kRotThreads, rot_blocks(V * U, true)) rotary_b
           table_unit<V>(tab.w + which * tab.step, r.lo[k], r.hi[k], w);
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            if (GEN) x[j] = f2add(x[j], f2(-mean[n]));
-            x[j] = f2mul(x[j], f2(rstd[n]));
-            if (live) {
-              dw[k][j] = f2fma(g[j], x[j], dw[k][j]);
-              if (GEN) db[GEN ? k : 0][j] = f2add(db[GEN ? k : 0][j], g[j]);
+            if (GEN) {
+              x[j] = f2add(x[j], f2(-mean[n]));
+              if (!WHOLE) x[j] = in_row<V>(x[j], j, r.lo_ok[k], r.hi_ok[k]);
             }
-            g[j] = f2mul(g[j], w[j]);
-            if (p.kind != FLN_NO_NORM) {
-              if (GEN) g[j] = f2add(g[j], f2(-c2[n]));
-              g[j] = f2mul(f2fma(x[j], f2(-c1[n]), g[j]), f2(rstd[n]));
-            }
+            const float2 q = f2mul(g[j], w[j]);
+            a = f2fma(x[j], x[j], a);
+            gx = f2fma(q, x[j], gx);
+            if (GEN) gs = f2add(gs, q);
           }
-          if (t.dx != nullptr && live && r.lo_ok[k])
-            unit_store<T, V>(dx + (int64_t)hh * p.dim, r.lo[k], r.hi[k], r.hi_ok[k], g);
         }
+        v[NS * n] = a.x + a.y;
+        v[NS * n + 1] = gx.x + gx.y;
+        if (GEN) v[NS * n + NS - 1] = gs.x + gs.y;
       }
+      lane_sum<NS * NB, LL>(v, p.log2_l);
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        rstd[n] = rsqrtf(fmaf(v[NS * n], inv_d, p.eps));
+        c1[n] = rstd[n] * v[NS * n + 1] * inv_d;
+        if (GEN && p.kind == FLN_LAYERNORM) c2[n] = v[NS * n + NS - 1] * inv_d;
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const int hh = h + n * r.groups + r.grp;
+      const bool live = hh < end;
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        float2 x[V], g[V], w[V];
+        float cs[V], sn[V];
+        unit_unpack<T, V>(px[n][k], x);
+        unit_unpack<T, V>(pg[n][k], g);
+        table_take<V>(tab.c + r.at[k], cs);
+        table_take<V>(tab.s + r.at[k], sn);
+        unit_rotate<V, HALF, true>(g, cs, sn);
+        table_unit<V>(tab.w + which * tab.step, r.lo[k], r.hi[k], w);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          if (GEN) x[j] = f2add(x[j], f2(-mean[n]));
+          x[j] = f2mul(x[j], f2(rstd[n]));
+          if (live) {
+            dw[k][j] = f2fma(g[j], x[j], dw[k][j]);
+            if (GEN) db[GEN ? k : 0][j] = f2add(db[GEN ? k : 0][j], g[j]);
+          }
+          g[j] = f2mul(g[j], w[j]);
+          if (p.kind != FLN_NO_NORM) {
+            if (GEN) g[j] = f2add(g[j], f2(-c2[n]));
+            g[j] = f2mul(f2fma(x[j], f2(-c1[n]), g[j]), f2(rstd[n]));
+          }
+        }
+        if (t.dx != nullptr && live && r.lo_ok[k])
+          unit_store<T, V>(dx + (int64_t)hh * p.dim, r.lo[k], r.hi[k], r.hi_ok[k], g);
+      }
+    }
+    if (++step == steps) {
+      step = 0;
+      ++token;
+      fresh = true;
     }
   }
   if (t.partials == nullptr) return;
@@ -622,7 +624,7 @@ struct RotPlan {
   bool half;
 };
 template <typename T>
-int rotary_launch(const RotParams& p, const RotPlan& plan, bool backward, unsigned grid, cudaStream_t st);
+int rotary_launch(const RotParams& p, const RotPlan& plan, bool backward, unsigned grid, cudaStream_t st);  // grid: of a backward
 
 template <typename T, int V, int U, bool HALF, bool GEN, int LL>
 static int rotary_launch_one(const RotParams& p, bool backward, unsigned grid, cudaStream_t st) {
@@ -632,6 +634,11 @@ static int rotary_launch_one(const RotParams& p, bool backward, unsigned grid, c
   constexpr int NBB = W <= 32 ? 2 : 1;
   size_t smem = rot_tables_floats(p.units, V, p.dim, GEN) * sizeof(float);
   if (!backward) {
+    // CTAs: those that are resident at once, fewer where there are not steps for all of their warps
+    const int turn = (32 >> p.log2_l) * NBF;
+    const int64_t total = (int64_t)p.tokens * ((p.t[0].heads + turn - 1) / turn + (p.t[1].heads + turn - 1) / turn);
+    const int64_t all = (int64_t)sm_count() * rot_blocks(V * U, false), most = (total + kRotThreads / 32 - 1) / (kRotThreads / 32);
+    grid = (unsigned)(most < all ? most : all);
     rotary_fwd_kernel<T, V, U, HALF, NBF, GEN, LL><<<grid, kRotThreads, smem, st>>>(p);
   } else {
     const size_t sums = (size_t)(kRotThreads / 32) * 2 * p.dim * sizeof(float);
