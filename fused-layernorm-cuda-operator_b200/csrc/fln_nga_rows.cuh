@@ -1084,6 +1084,8 @@ static int nga_fwd_rows_k(const NgaParams& p, const NgaGeom& g, cudaStream_t st)
           return nga_fwd_rows_t<T, K, GATE, 128, false>(p, g, st);
         case 256:
           return nga_fwd_rows_t<T, K, GATE, 256, false>(p, g, st);
+        case 320:
+          return nga_fwd_rows_t<T, K, GATE, 320, false>(p, g, st);
         case 512:
           return nga_fwd_rows_t<T, K, GATE, 512, false>(p, g, st);
       }
@@ -1122,9 +1124,14 @@ static int nga_bwd_rows_g(const NgaParams& p, const NgaGeom& g, cudaStream_t st)
     return nga_set_of(p) == 1 ? nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 1, true>>(p, g, st)
                               : nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 0, true>>(p, g, st);
   }
-  if (g.direct)
+  if (g.direct) {
+    // (fp32 rows of 5120, general form: 84 us at 2047 rows with the threads per row found out at run time, 67 so)
+    if constexpr (sizeof(T) == 4 && K * 16 / (int)sizeof(T) == 8) {
+      if (g.csm && g.nv == K * g.tpr && g.tpr == 640) return nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, true, 640, false, 3, false>>(p, g, st);
+    }
     return g.csm ? nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 3, false>>(p, g, st)
                  : nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, false, 0, false, 3, false>>(p, g, st);
+  }
   if (!g.csm) return nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, false, 0, false, 0, false>>(p, g, st);
   const int set = nga_set_of(p);
   // compile-time rows where the registers allow: 16 elements per thread, 8 of the general form and of fp32
@@ -1137,7 +1144,12 @@ static int nga_bwd_rows_g(const NgaParams& p, const NgaGeom& g, cudaStream_t st)
         FLN_NGA_BWD(64, false, 1)
         FLN_NGA_BWD(128, false, 1)
         FLN_NGA_BWD(256, false, 1)
+        FLN_NGA_BWD(320, false, 1)
         FLN_NGA_BWD(512, false, 1)
+        default:
+          if constexpr (K * 16 / (int)sizeof(T) == 8) {  // (what 640 threads have the registers for)
+            if (g.tpr == 640) return nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, true, 640, false, 1, false>>(p, g, st);
+          }
       }
     }
     if (g.nv == K * g.tpr && set == 2) {
