@@ -108,6 +108,40 @@ __device__ __forceinline__ void gate_act_grad(float v, int act, float* a, float*
     *da = 1.0f;
   }
 }
+template <int V>
+struct Known {
+  static constexpr int value = V;
+};
+// the same of N pairs: which function is asked once for all of them, so that their special-function
+// instructions follow each other instead of each waiting behind a branch (262144 x 128 bf16: forward
+// 42.8 -> 38.5 us, backward 58.7 -> 54.3).  The general backward has no registers left for it and takes
+// one pair after the other (2047 x 5120 fp32: 67 us, 78 all at once).
+template <bool EXACT, int N>
+__device__ __forceinline__ void gate_act_all(float2 (&v)[N], int act) {
+  auto all = [&](auto known) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = make_float2(gate_act<EXACT>(v[e].x, known.value), gate_act<EXACT>(v[e].y, known.value));
+  };
+  if (act == FLN_GATE_ACT_SIGMOID) all(Known<FLN_GATE_ACT_SIGMOID>());
+  else if (act == FLN_GATE_ACT_SILU) all(Known<FLN_GATE_ACT_SILU>());
+  else if (act == FLN_GATE_ACT_TANH) all(Known<FLN_GATE_ACT_TANH>());
+}
+template <bool EXACT, int N>
+__device__ __forceinline__ void gate_act_grad_all(float2 (&v)[N], float2 (&d)[N], int act) {  // v becomes act(v)
+  auto all = [&](auto known) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      float2 a;
+      gate_act_grad<EXACT>(v[e].x, known.value, &a.x, &d[e].x);
+      gate_act_grad<EXACT>(v[e].y, known.value, &a.y, &d[e].y);
+      v[e] = a;
+    }
+  };
+  if (act == FLN_GATE_ACT_SIGMOID) all(Known<FLN_GATE_ACT_SIGMOID>());
+  else if (act == FLN_GATE_ACT_SILU) all(Known<FLN_GATE_ACT_SILU>());
+  else if (act == FLN_GATE_ACT_TANH) all(Known<FLN_GATE_ACT_TANH>());
+  else all(Known<FLN_GATE_ACT_NONE>());
+}
 
 // sum of NV values over the CTA, result in every thread, the same order everywhere; red holds
 // 2 x NV x 32 floats, `flip` alternates so that one barrier per call is enough

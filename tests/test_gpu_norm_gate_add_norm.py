@@ -110,6 +110,15 @@ def test_long_rows(shape, dtype):
         check_case(*make(shape, dtype, **KINDS[i], **GATES[(i + len(shape)) % 6], off=float(i % 2), seed=i, ba=0.7))
 
 
+@pytest.mark.parametrize("shape,dtype", [((2, 39, 5120), BF16), ((2, 39, 5120), F32), ((5, 31, 2560), F32), ((5, 31, 2560), F16),
+                                         ((301, 5120), F32), ((3, 100, 1280), BF16)], ids=lambda v: str(v).replace("torch.", ""))
+def test_whole_rows_of_five_times_a_power_of_two(shape, dtype):
+    """Every pair of norm kinds and every kind of gate, with a residual and with both gradients."""
+    for i in range(6):
+        for j in range(6):
+            check_case(*make(shape, dtype, **KINDS[i], **GATES[j], off=float(i % 2), seed=6 * i + j, ba=0.7))
+
+
 @pytest.mark.parametrize("h", [1, 2, 3, 5, 9, 31, 65, 130, 257, 333, 511, 1001, 2050, 2777, 4100, 5121, 6007, 7998])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_rows_that_start_anywhere_in_a_vector(h, dtype):
