@@ -262,6 +262,7 @@ OptTensor unpacked(const SavedVariable& v) {
   return t.defined() ? OptTensor(t) : std::nullopt;
 }
 Tensor or_undefined(const OptTensor& t) { return has(t) ? *t : Tensor(); }
+// (a dual tensor need not require grad, and no_grad leaves forward mode on: asked before anything else)
 void refuse_forward_mode(std::initializer_list<const OptTensor*> ts, const char* what) {
   for (const OptTensor* t : ts)
     TORCH_CHECK(!has(*t) || !torch::autograd::isFwGradDefined(*t), what, " has no forward-mode derivative");
@@ -314,11 +315,11 @@ std::tuple<OptTensor, Tensor> norm_gate_add_norm(const Tensor& input, const OptT
                                                  const OptTensor& b2, int64_t post_kind, int64_t kind, int64_t act,
                                                  double ba, double ra, double woff, double eps1, double eps2) {
   const OptTensor in = input;
+  refuse_forward_mode({&in, &residual, &gate, &w1, &b1, &w2, &b2}, "fused_norm_gate_add_norm");
   if (!wants_grad({&in, &residual, &gate, &w1, &b1, &w2, &b2})) {
     NgaOut o = nga_forward(input, residual, gate, w1, b1, w2, b2, {post_kind, kind, act, ba, ra, woff, eps1, eps2}, false);
     return {opt(o.y), o.sum};
   }
-  refuse_forward_mode({&in, &residual, &gate, &w1, &b1, &w2, &b2}, "fused_norm_gate_add_norm");
   const NgaConf c{post_kind, kind, act, ba, ra, woff, eps1, eps2};
   NgaOut o;
   {
@@ -649,13 +650,13 @@ std::tuple<Tensor, OptTensor> qk_norm_rotary(const Tensor& q, const OptTensor& k
                                              int64_t axes, int64_t layout, int64_t kind, double eps, double woff,
                                              double mag, bool in_place) {
   const OptTensor qo = q;
+  refuse_forward_mode({&qo, &k, &qw, &kw, &qb, &kb}, "fused_qk_norm_rotary");
   const bool grad = wants_grad({&qo, &k, &qw, &kw, &qb, &kb});
   TORCH_CHECK(!(in_place && grad), "the in-place form records no gradient: use it under torch.no_grad()");
   if (!grad) {
     auto o = rot_forward(q, k, positions, turns, axis, {qw, kw, qb, kb}, {pairs, axes, layout, kind, eps, woff, mag}, in_place);
     return {o.first, opt(o.second)};
   }
-  refuse_forward_mode({&qo, &k, &qw, &kw, &qb, &kb}, "fused_qk_norm_rotary");
   const RotConf c{pairs, axes, layout, kind, eps, woff, mag};
   std::pair<Tensor, Tensor> o;
   {
