@@ -529,17 +529,19 @@ bool elements_apart(const Tensor& t) {
   return true;
 }
 // q and k hold no element in common: their ranges are apart, or become so when the outermost
-// dimensions, which both step through alike, are taken off (views of one packed projection)
+// dimensions, which both step through alike, are taken off (views of one packed projection).  What
+// is left of both together has to fit between two steps of every dimension that was taken off.
 bool tensors_apart(const Tensor& q, const Tensor& k) {
   if (q.numel() == 0 || k.numel() == 0 || !q.is_alias_of(k)) return true;
   const int64_t off = k.storage_offset() - q.storage_offset();
   std::vector<int64_t> dims;
   for (int64_t i = 0; i < q.dim(); ++i) dims.push_back(i);
-  int64_t window = INT64_MAX;  // what the dimensions taken off step over
+  int64_t window = INT64_MAX;  // the step of the dimension taken off last
   while (true) {
     const int64_t sq = span(q, dims), sk = span(k, dims);
     const int64_t lo = std::min<int64_t>(0, off), hi = std::max(sq, off + sk);
-    if (hi - lo <= window && (off >= sq || off + sk <= 0)) return true;
+    if (hi - lo > window) return false;
+    if (off >= sq || off + sk <= 0) return true;
     int64_t best = -1;
     for (int64_t d : dims)
       if (q.size(d) > 1 && (best < 0 || q.stride(d) > q.stride(best))) best = d;
@@ -547,6 +549,17 @@ bool tensors_apart(const Tensor& q, const Tensor& k) {
     window = q.stride(best);
     dims.erase(std::find(dims.begin(), dims.end(), best));
   }
+}
+
+void check_in_place(const Tensor& q, const OptTensor& k, Heads* views) {
+  const Tensor* in[2] = {&q, has(k) ? &*k : nullptr};
+  for (int i = 0; i < 2; ++i) {
+    if (in[i] == nullptr) continue;
+    TORCH_CHECK(in[i]->dim() >= 2, "q and k must be [.., heads, head_dim]");
+    TORCH_CHECK(heads_view(*in[i], &views[i]) && elements_apart(*in[i]),
+                "in place, q and k need a contiguous last dimension, leading dimensions that fold, and no element twice");
+  }
+  TORCH_CHECK(in[1] == nullptr || (k->dim() == q.dim() && tensors_apart(q, *k)), "in place, q and k must not overlap");
 }
 
 // (q', k'); k' undefined without k
@@ -557,14 +570,7 @@ std::pair<Tensor, Tensor> rot_forward(const Tensor& q, const OptTensor& k, const
   Tensor out[2];
   const Tensor* in[2] = {&q, has(k) ? &*k : nullptr};
   Heads keep[4];
-  if (in_place) {
-    for (int i = 0; i < 2; ++i) {
-      if (in[i] == nullptr) continue;
-      TORCH_CHECK(heads_view(*in[i], &keep[i]) && elements_apart(*in[i]),
-                  "in place, q and k need a contiguous last dimension, leading dimensions that fold, and no element twice");
-    }
-    TORCH_CHECK(in[1] == nullptr || tensors_apart(q, *k), "in place, q and k must not overlap");
-  }
+  if (in_place) check_in_place(q, k, keep);
   for (int i = 0; i < 2; ++i) {
     if (in[i] == nullptr) continue;
     if (!in_place) {
@@ -720,4 +726,10 @@ void fln_bind_blocks(pybind11::module& m) {
         py::arg("q"), py::arg("k"), py::arg("positions"), py::arg("turns"), py::arg("axis"), py::arg("q_weight"),
         py::arg("k_weight"), py::arg("q_bias"), py::arg("k_bias"), py::arg("pairs"), py::arg("axes"), py::arg("layout"),
         py::arg("kind"), py::arg("eps"), py::arg("weight_offset"), py::arg("magnitude"), py::arg("in_place"));
+  m.def("check_rotary_in_place",
+        [](const Tensor& q, const OptTensor& k) {
+          Heads views[2];
+          check_in_place(q, k, views);
+        },
+        "raises if qk_norm_rotary could not write over these q and k (of any device)", py::arg("q"), py::arg("k"));
 }
