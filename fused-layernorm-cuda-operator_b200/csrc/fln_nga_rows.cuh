@@ -669,21 +669,23 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
     if (ahead.slot < nslots) {
       unsigned char* st = stages + fill;
       const int64_t row_at = (int64_t)my_row(ahead) * cols;
+      const bool there = ONE || ahead.row + r_in * apart < ahead.last;
       Places<K, VEC, FULL, SHIFT> wa = w;
       if (SHIFT) wa.set(lane, tpr, g.nv, cols, row_shift(ahead.row, cols, VEC), PAIR, v0, v1);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         unsigned char* d = st + k * kstep;
         const int64_t o = row_at + wa.at[k];
+        const int64_t left = SHIFT ? (p.rows * cols - o) * (int)sizeof(T) : 16;
+        const int bytes = left < 16 ? (int)left : 16;  // (the last vector of the last row may reach behind the tensor)
         auto bring = [&](unsigned char* to, const void* from) {
-          if (SHIFT) {  // the last vector of the last row may reach behind the tensor
-            const int64_t left = (p.rows * cols - o) * (int)sizeof(T);
-            cp_async16_part(to, reinterpret_cast<const T*>(from) + o, left < 16 ? (int)left : 16);
-          } else {
-            cp_async16(to, reinterpret_cast<const T*>(from) + o);
-          }
+          if (SHIFT) cp_async16_part(to, reinterpret_cast<const T*>(from) + o, bytes);
+          else cp_async16(to, reinterpret_cast<const T*>(from) + o);
         };
-        bring(d, p.x);
+        // a row group behind the slot takes x as zeros: without a norm in front of it an infinity of the last
+        // row would be multiplied by that group's ds of 0
+        if (ONE) bring(d, p.x);
+        else cp_async16_part(d, reinterpret_cast<const T*>(p.x) + o, there ? bytes : 0);
         if (has_res) bring(d + l.res * unit, p.res);
         if (has_dy) bring(d + l.dy * unit, p.dy);
         if (has_ds && !DIRECT) bring(d + l.ds * unit, p.ds);

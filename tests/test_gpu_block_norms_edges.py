@@ -1,0 +1,40 @@
+"""Edges of the block norms: infinities where a formula keeps them to themselves, angles next to
+quarter turns, work queued on another stream."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+import block_norms_ref as R
+
+if torch.cuda.is_available():
+    import fused_layernorm as fl
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.mark.parametrize("shape", [(1, 3, 64), (2, 5, 128), (3, 67, 96), (4, 1, 128), (2, 9, 33), (1, 201, 256)], ids=str)
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("gate", ["vector", "group"])
+def test_infinite_inputs_in_the_gradient_of_a_shared_gate(shape, dtype, gate):
+    """dgate = act'(gate) * sum of branch_scale * dsum * x without a norm in front: an infinity in the
+    last row of a sample makes an infinity of its column, not NaN, and touches no other column.  The
+    rows do not fill the row groups of a block."""
+    b, n, h = shape
+    g = torch.Generator().manual_seed(h + n)
+    rn = lambda *s: torch.randn(*s, generator=g).to(dtype).cuda()
+    x, r, ds, gt = rn(*shape), rn(*shape), rn(*shape), rn(*((h,) if gate == "vector" else (b, h)))
+    x[-1, -1, 3], x[0, -1, h - 1] = float("inf"), float("-inf")
+    ds[-1, -1, 3], ds[0, -1, h - 1] = 0.5, 1.5
+    leaf = gt.clone().requires_grad_(True)
+    _, s = fl.fused_norm_gate_add_norm(x, r, leaf, post_norm=None, norm=None, gate_activation="sigmoid", branch_scale=0.7)
+    got = torch.autograd.grad(s, leaf, ds)[0]
+    t = dict.fromkeys(R.NAMES)
+    t.update(input=x.double(), residual=r.double(), gate=gt.double())
+    want, tol = R.nga_bounds(t, None, ds.double(), dtype, "none", "none", "sigmoid", 0.7, 1.0, 0.0)["grads"]["gate"]
+    fin = torch.isfinite(want)
+    assert int((~fin).sum()) == 2 and bool((want[~fin].abs() == math.inf).all())
+    assert torch.equal(got[~fin].double(), want[~fin])
+    R.check(got[fin], (want[fin], tol.expand(want.shape)[fin]), "dgate")
