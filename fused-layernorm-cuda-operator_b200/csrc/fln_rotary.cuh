@@ -11,11 +11,10 @@
 // so both members of every pair are in one lane's registers, a rotation needs no exchange, and
 // the row sums take log2(L) shuffles and no barrier.
 //
-// Angles.  position * turns modulo 2^64 is the fraction of a turn as a signed 64-bit number, so
-// the range reduction is the wrap of an integer product: no table of cosines to read, nothing
-// lost at far positions.  sincospi of twice that fraction gives cosine and sine.  A lane makes
-// them once per token and keeps them in registers for all the heads that its warp takes of that
-// token.
+// Angles.  position * turns modulo 2^64 is the fraction of a turn as a 64-bit integer, so the range
+// reduction is the wrap of an integer product: no table of cosines to read, nothing lost at far
+// positions.  sincospi of what is left behind whole quarter turns gives cosine and sine.  A warp
+// makes them once per token, in shared memory, for all the heads that it takes of that token.
 #pragma once
 
 #include "fln_common.cuh"
@@ -68,32 +67,28 @@ __device__ __forceinline__ void unit_columns(const RotParams& p, int u, int& lo,
 }
 
 // Tables in shared memory, in 32 bits.  Every warp keeps the cosines and sines of its token, one
-// entry per pair and 1 / 0 behind them (units of the part that is not rotated): the lanes make the
-// angles between them, P / 32 each, and all row groups of the warp read them.  The CTA keeps
+// entry per pair: the lanes make the angles between them, P / 32 each, and all row groups of the
+// warp read them.  The CTA keeps
 // weight_offset + weight and bias of both tensors.  (With the angles made by every lane for its own
 // unit and held in registers beside the weights, the bf16 forward at 8192 x 48 x 128 ran with 80
 // registers, 16.7 instructions per element, 55 us.)
 struct RotTables {
-  float *c, *s;  // of this warp: [units * V] each
+  float *c, *s;  // of this warp: [rot_units * V] each
   float *w, *b;  // of q; those of k lie `step` behind them
   int step;
 };
-__host__ __device__ constexpr size_t rot_tables_floats(int units, int V, int dim, bool gen) {
-  return (size_t)(kRotThreads / 32) * 2 * units * V + (size_t)(gen ? 4 : 2) * ((dim + 3) & ~3);
+__host__ __device__ constexpr size_t rot_tables_floats(int rot_units, int V, int dim, bool gen) {
+  return (size_t)(kRotThreads / 32) * 2 * rot_units * V + (size_t)(gen ? 4 : 2) * ((dim + 3) & ~3);
 }
 template <typename T, int V, bool GEN>
 __device__ __forceinline__ RotTables rot_tables(const RotParams& p, float* mem) {
   RotTables t;
-  const int n = p.units * V, warp = threadIdx.x >> 5, dim4 = (p.dim + 3) & ~3;
+  const int n = p.rot_units * V, warp = threadIdx.x >> 5, dim4 = (p.dim + 3) & ~3;
   t.c = mem + warp * 2 * n;
   t.s = t.c + n;
   t.w = mem + (kRotThreads / 32) * 2 * n;
   t.b = t.w + dim4;
   t.step = GEN ? 2 * dim4 : dim4;
-  for (int i = threadIdx.x & 31; i < n; i += 32) {
-    t.c[i] = 1.f;
-    t.s[i] = 0.f;
-  }
   for (int i = threadIdx.x; i < 2 * p.dim; i += kRotThreads) {
     const int which = i >= p.dim ? 1 : 0, c = i - which * p.dim;
     const T* w = reinterpret_cast<const T*>(p.t[which].weight);
@@ -107,8 +102,8 @@ __device__ __forceinline__ RotTables rot_tables(const RotParams& p, float* mem) 
   return t;
 }
 // the angles of a token into its warp's table
-__device__ __forceinline__ void token_angles(const RotParams& p, const RotTables& t, int b, int s) {
-  const int64_t at0 = (int64_t)b * p.pos_batch + (int64_t)s * p.pos_seq;
+__device__ __forceinline__ void token_angles(const RotParams& p, const RotTables& t, int batch, int seq) {
+  const int64_t at0 = (int64_t)batch * p.pos_batch + (int64_t)seq * p.pos_seq;
   __syncwarp();  // nobody reads the last token's any more
   for (int i = threadIdx.x & 31; i < p.pairs; i += 32) {
     const int64_t at = at0 + (int64_t)__ldg(p.axis + i) * p.pos_axis;
@@ -234,6 +229,17 @@ __device__ __forceinline__ void unit_rotate(float2 (&f)[V], const float (&c)[V],
   }
 }
 
+// ... by its angles in the table; a unit of the part that is not rotated stays as it is (a rotation
+// by nothing would multiply by zero, and take an infinity to its neighbour as NaN)
+template <int V, bool HALF, bool BACK>
+__device__ __forceinline__ void unit_turn(float2 (&f)[V], const RotTables& tab, int at, bool turn) {
+  if (!turn) return;
+  float c[V], s[V];
+  table_take<V>(tab.c + at, c);
+  table_take<V>(tab.s + at, s);
+  unit_rotate<V, HALF, BACK>(f, c, s);
+}
+
 template <int N, int LL>
 __device__ __forceinline__ void lane_sum(float (&v)[N], int log2_l) {
   if constexpr (LL >= 0) {
@@ -264,6 +270,7 @@ struct RotLane {
   int L, groups, grp, ul;
   int lo[U], hi[U];          // first columns of the unit's vectors (of another vector where there is none)
   int at[U];                 // its first entry in the table of angles
+  bool rot[U];               // it is rotated
   bool lo_ok[U], hi_ok[U];
   template <int LL>
   __device__ __forceinline__ void init(const RotParams& p) {
@@ -280,7 +287,8 @@ struct RotLane {
       unit_columns<V, HALF>(p, lo_ok[k] ? u : 0, lo[k], hi[k]);
       hi_ok[k] = lo_ok[k] && hi[k] >= 0;
       if (hi[k] < 0) hi[k] = lo[k];
-      at[k] = (lo_ok[k] ? u : 0) * V;
+      rot[k] = u < p.rot_units;
+      at[k] = (rot[k] ? u : 0) * V;
       if (LL >= 0) lo_ok[k] = hi_ok[k] = true;  // whole units on every lane
     }
   }
@@ -295,9 +303,11 @@ struct RotLane {
 // every step, so the shuffles are whole.  The rows stay packed as they came; they are unpacked once
 // for the sums and once more for the result, which costs an instruction per element and saves the
 // registers that let more warps (and so more loads) be in flight.
-// GEN: layer norm or bias.  LL >= 0: log2 of the lanes per row, known at compile time.
+// GEN: layer norm or bias.  LL >= 0: log2 of the lanes per row, known at compile time.  PART: there are
+// units that are not rotated (asked for each unit where every one is: 8192 x 48 x 128 bf16, backward
+// 70.8 -> 74.9 us with its sums).
 // ----------------------------------------------------------------------------------------
-template <typename T, int V, int U, bool HALF, int NB, bool GEN, int LL>
+template <typename T, int V, int U, bool HALF, int NB, bool GEN, int LL, bool PART>
 __global__ void __launch_bounds__(kRotThreads, rot_blocks(V * U, false)) rotary_fwd_kernel(const RotParams p) {
   RotLane<V, U, HALF> r;
   r.template init<LL>(p);
@@ -391,7 +401,6 @@ __global__ void __launch_bounds__(kRotThreads, rot_blocks(V * U, false)) rotary_
 #pragma unroll
       for (int k = 0; k < U; ++k) {
         float2 f[V], w[V], bi[V];
-        float cs[V], sn[V];
         unit_unpack<T, V>(x[n][k], f);
         table_unit<V>(tab.w + which * tab.step, r.lo[k], r.hi[k], w);
         if (GEN) table_unit<V>(tab.b + which * tab.step, r.lo[k], r.hi[k], bi);
@@ -401,9 +410,7 @@ __global__ void __launch_bounds__(kRotThreads, rot_blocks(V * U, false)) rotary_
           f[j] = f2mul(f[j], f2(rstd[n]));
           f[j] = GEN ? f2fma(f[j], w[j], bi[j]) : f2mul(f[j], w[j]);
         }
-        table_take<V>(tab.c + r.at[k], cs);
-        table_take<V>(tab.s + r.at[k], sn);
-        unit_rotate<V, HALF, false>(f, cs, sn);
+        unit_turn<V, HALF, false>(f, tab, r.at[k], !PART || r.rot[k]);
         if (hh < end && r.lo_ok[k]) unit_store<T, V>(row, r.lo[k], r.hi[k], r.hi_ok[k], f);
       }
     }
@@ -424,7 +431,7 @@ __global__ void __launch_bounds__(kRotThreads, rot_blocks(V * U, false)) rotary_
 // weight and bias stay in the lanes' registers over all rows of a CTA and are added in a fixed
 // order at its end, so a CTA works for one tensor only.
 // ----------------------------------------------------------------------------------------
-template <typename T, int V, int U, bool HALF, int NB, bool GEN, int LL>
+template <typename T, int V, int U, bool HALF, int NB, bool GEN, int LL, bool PART>
 __global__ void __launch_bounds__(kRotThreads, rot_blocks(V * U, true)) rotary_bwd_kernel(const RotParams p) {
   extern __shared__ __align__(16) float sacc[];  // the tables; at the end [warps][2][dim]
   const RotTables tab = rot_tables<T, V, GEN>(p, sacc);
@@ -512,12 +519,9 @@ __global__ void __launch_bounds__(kRotThreads, rot_blocks(V * U, true)) rotary_b
 #pragma unroll
         for (int k = 0; k < U; ++k) {
           float2 x[V], g[V], w[V];
-          float cs[V], sn[V];
           unit_unpack<T, V>(px[n][k], x);
           unit_unpack<T, V>(pg[n][k], g);
-          table_take<V>(tab.c + r.at[k], cs);
-          table_take<V>(tab.s + r.at[k], sn);
-          unit_rotate<V, HALF, true>(g, cs, sn);
+          unit_turn<V, HALF, true>(g, tab, r.at[k], !PART || r.rot[k]);
           table_unit<V>(tab.w + which * tab.step, r.lo[k], r.hi[k], w);
 #pragma unroll
           for (int j = 0; j < V; ++j) {
@@ -550,12 +554,9 @@ __global__ void __launch_bounds__(kRotThreads, rot_blocks(V * U, true)) rotary_b
 #pragma unroll
       for (int k = 0; k < U; ++k) {
         float2 x[V], g[V], w[V];
-        float cs[V], sn[V];
         unit_unpack<T, V>(px[n][k], x);
         unit_unpack<T, V>(pg[n][k], g);
-        table_take<V>(tab.c + r.at[k], cs);
-        table_take<V>(tab.s + r.at[k], sn);
-        unit_rotate<V, HALF, true>(g, cs, sn);
+        unit_turn<V, HALF, true>(g, tab, r.at[k], !PART || r.rot[k]);
         table_unit<V>(tab.w + which * tab.step, r.lo[k], r.hi[k], w);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -626,24 +627,24 @@ struct RotPlan {
 template <typename T>
 int rotary_launch(const RotParams& p, const RotPlan& plan, bool backward, unsigned grid, cudaStream_t st);  // grid: of a backward
 
-template <typename T, int V, int U, bool HALF, bool GEN, int LL>
+template <typename T, int V, int U, bool HALF, bool GEN, int LL, bool PART>
 static int rotary_launch_one(const RotParams& p, bool backward, unsigned grid, cudaStream_t st) {
   // rows in flight per row group: 128 bytes of each tensor per lane where the registers allow it
   constexpr int W = 2 * V * U * (int)sizeof(T);
   constexpr int NBF = W <= 64 ? 2 : 1;
   constexpr int NBB = W <= 32 ? 2 : 1;
-  size_t smem = rot_tables_floats(p.units, V, p.dim, GEN) * sizeof(float);
+  size_t smem = rot_tables_floats(p.rot_units, V, p.dim, GEN) * sizeof(float);
   if (!backward) {
     // CTAs: those that are resident at once, fewer where there are not steps for all of their warps
     const int turn = (32 >> p.log2_l) * NBF;
     const int64_t total = (int64_t)p.tokens * ((p.t[0].heads + turn - 1) / turn + (p.t[1].heads + turn - 1) / turn);
     const int64_t all = (int64_t)sm_count() * rot_blocks(V * U, false), most = (total + kRotThreads / 32 - 1) / (kRotThreads / 32);
     grid = (unsigned)(most < all ? most : all);
-    rotary_fwd_kernel<T, V, U, HALF, NBF, GEN, LL><<<grid, kRotThreads, smem, st>>>(p);
+    rotary_fwd_kernel<T, V, U, HALF, NBF, GEN, LL, PART><<<grid, kRotThreads, smem, st>>>(p);
   } else {
     const size_t sums = (size_t)(kRotThreads / 32) * 2 * p.dim * sizeof(float);
     if (sums > smem) smem = sums;
-    rotary_bwd_kernel<T, V, U, HALF, NBB, GEN, LL><<<grid, kRotThreads, smem, st>>>(p);
+    rotary_bwd_kernel<T, V, U, HALF, NBB, GEN, LL, PART><<<grid, kRotThreads, smem, st>>>(p);
   }
   FLN_CHECK_LAUNCH();
   return FLN_OK;
@@ -653,12 +654,18 @@ static int rotary_launch_ll(const RotParams& p, bool backward, unsigned grid, cu
   // heads that fill the lanes with whole 16-byte vectors (64, 128 and 256 elements of 16 bits) have
   // their own kernels
   if constexpr (U == 1 && V * (int)sizeof(T) == 16) {
-    if (2 * p.units * V != p.dim || p.units != 1 << p.log2_l) return rotary_launch_one<T, V, U, HALF, GEN, -1>(p, backward, grid, st);
-    if (p.log2_l == 2) return rotary_launch_one<T, V, U, HALF, GEN, 2>(p, backward, grid, st);
-    if (p.log2_l == 3) return rotary_launch_one<T, V, U, HALF, GEN, 3>(p, backward, grid, st);
-    if (p.log2_l == 4) return rotary_launch_one<T, V, U, HALF, GEN, 4>(p, backward, grid, st);
+    if (2 * p.units * V == p.dim && p.units == 1 << p.log2_l) {
+#define FLN_ROT_LL(LL)                                                                                            \
+  if (p.log2_l == LL)                                                                                             \
+    return p.rot_units < p.units ? rotary_launch_one<T, V, U, HALF, GEN, LL, true>(p, backward, grid, st)         \
+                                 : rotary_launch_one<T, V, U, HALF, GEN, LL, false>(p, backward, grid, st);
+      FLN_ROT_LL(2)
+      FLN_ROT_LL(3)
+      FLN_ROT_LL(4)
+#undef FLN_ROT_LL
+    }
   }
-  return rotary_launch_one<T, V, U, HALF, GEN, -1>(p, backward, grid, st);
+  return rotary_launch_one<T, V, U, HALF, GEN, -1, true>(p, backward, grid, st);
 }
 template <typename T, int V, int U>
 static int rotary_launch_vu(const RotParams& p, bool half, bool backward, unsigned grid, cudaStream_t st) {

@@ -38,3 +38,35 @@ def test_infinite_inputs_in_the_gradient_of_a_shared_gate(shape, dtype, gate):
     assert int((~fin).sum()) == 2 and bool((want[~fin].abs() == math.inf).all())
     assert torch.equal(got[~fin].double(), want[~fin])
     R.check(got[fin], (want[fin], tol.expand(want.shape)[fin]), "dgate")
+
+
+@pytest.mark.parametrize("dim,pairs", [(128, 32), (80, 20), (72, 16), (50, 10), (51, 20), (64, 0), (256, 64), (510, 100)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_infinities_behind_the_rotated_part(dim, pairs, dtype, layout):
+    """Elements behind the rotated part pass without a norm as they are, in both directions: an
+    infinity or NaN among them stays where it is.  With a norm the row's other elements are zero
+    (rstd is 0), not NaN."""
+    rot = fl.RotaryAxes(dim, pairs, layout=layout, magnitude=1.25)
+    pos = torch.arange(9, device="cuda") * 37
+    g = torch.Generator().manual_seed(dim)
+    q, dq = (torch.randn(9, 3, dim, generator=g).to(dtype).cuda() for _ in range(2))
+    odd = {2 * pairs: float("inf"), dim - 1: float("nan"), 2 * pairs + (dim - 2 * pairs) // 2: float("-inf")}
+
+    def spoil(v):
+        v = v.clone()
+        for c, w in odd.items():
+            v[c % 9, 1, c] = w
+        return v
+
+    def run(q, dq):
+        leaf = q.clone().requires_grad_(True)
+        o, _ = fl.fused_qk_norm_rotary(leaf, None, pos, rot, norm=None)
+        return o.detach(), torch.autograd.grad(o, leaf, dq)[0]
+
+    for got, clean in zip(run(spoil(q), spoil(dq)), run(q, dq)):
+        assert torch.equal(torch.nan_to_num(got, nan=77.0), torch.nan_to_num(spoil(clean), nan=77.0))
+    one = q.clone()
+    one[4, 2, dim - 1] = float("inf")
+    o, _ = fl.fused_qk_norm_rotary(one, None, pos, rot)
+    assert bool(torch.isnan(o[4, 2, dim - 1])) and not bool(o[4, 2, :dim - 1].any())
