@@ -109,12 +109,16 @@ __device__ __forceinline__ void token_angles(const RotParams& p, const RotTables
     const int64_t at = at0 + (int64_t)__ldg(p.axis + i) * p.pos_axis;
     const long long pos = p.pos64 ? __ldg(reinterpret_cast<const long long*>(p.positions) + at)
                                   : (long long)__ldg(reinterpret_cast<const int*>(p.positions) + at);
-    const long long frac = (long long)((unsigned long long)pos * __ldg(p.turns + i));
-    // frac / 2^64 turns = frac / 2^63 half turns, in [-1, 1]
-    float sv, cv;
-    sincospif(__ll2float_rn(frac) * 1.0842021724855044e-19f, &sv, &cv);
-    t.c[i] = cv * p.mag;
-    t.s[i] = sv * p.mag;
+    // The fraction of a turn in 2^64ths.  Whole quarter turns are taken off while it is an integer:
+    // what goes into 32 bits is an eighth of a turn at most, so a cosine or sine keeps its own relative
+    // precision next to its zeros too (the whole fraction rounded: 1.1e-7 at most, so 5e-8).
+    const unsigned long long frac = (unsigned long long)pos * __ldg(p.turns + i);
+    const unsigned quarters = (unsigned)((frac + (1ull << 61)) >> 62);
+    float sv, cv;  // rest / 2^63 half turns, in [-1/4, 1/4]
+    sincospif(__ll2float_rn((long long)(frac - ((unsigned long long)quarters << 62))) * 1.0842021724855044e-19f, &sv, &cv);
+    const float c = quarters & 1 ? sv : cv, s = quarters & 1 ? cv : sv;
+    t.c[i] = ((quarters + 1) & 2 ? -c : c) * p.mag;
+    t.s[i] = (quarters & 2 ? -s : s) * p.mag;
   }
   __syncwarp();
 }

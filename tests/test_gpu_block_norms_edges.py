@@ -70,3 +70,33 @@ def test_infinities_behind_the_rotated_part(dim, pairs, dtype, layout):
     one[4, 2, dim - 1] = float("inf")
     o, _ = fl.fused_qk_norm_rotary(one, None, pos, rot)
     assert bool(torch.isnan(o[4, 2, dim - 1])) and not bool(o[4, 2, :dim - 1].any())
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_cosines_and_sines_keep_their_own_bits(layout):
+    """Every cosine and sine is good relative to itself, next to its zeros too.  The fraction of a turn
+    is an exact integer; what is left of it behind whole quarter turns is rounded to 24 bits, which
+    moves a sine or cosine by 2**-24 of itself at most (x cot x <= 1 and x tan x <= pi / 4 up to an
+    eighth of a turn), and sine and cosine are good to one unit in the last place, 2**-23."""
+    freq = [math.pi / 2, math.pi, math.pi / 4, 3 * math.pi / 2, 2 * math.pi / 3, 1.0, 1e-3, math.pi * (1 + 2.0 ** -30)]
+    n = len(freq)
+    rot = fl.RotaryAxes(2 * n, n, inv_freq=freq, layout=layout)
+    g = torch.Generator().manual_seed(0)
+    pos = torch.cat([torch.arange(-20, 20), torch.randint(-2 ** 40, 2 ** 40, (3000,), generator=g)]).cuda()
+    lo, hi = (slice(0, n), slice(n, 2 * n)) if layout == "half" else (slice(0, None, 2), slice(1, None, 2))
+    q = torch.zeros(len(pos), 1, 2 * n, device="cuda")
+    q[..., lo] = 1.0  # rotates to (cos, sin)
+    out = fl.fused_qk_norm_rotary(q, None, pos, rot, norm=None)[0][:, 0].cpu().double()
+    turns = [int(v) % 2 ** 64 for v in rot.turns.tolist()]
+    quarter, rest = [], []
+    for p in pos.tolist():
+        for t in turns:
+            f = p * t % 2 ** 64
+            quarter.append((f + 2 ** 61 >> 62) % 4)
+            rest.append(((f + 2 ** 61) % 2 ** 62 - 2 ** 61) / 2 ** 64)
+    k, a = torch.tensor(quarter).view(-1, n), torch.tensor(rest, dtype=torch.float64).view(-1, n) * (2 * math.pi)
+    c, s = torch.cos(a), torch.sin(a)
+    cos = torch.stack([c, -s, -c, s]).gather(0, k[None])[0]
+    sin = torch.stack([s, c, -s, -c]).gather(0, k[None])[0]
+    for got, want in ((out[:, lo], cos), (out[:, hi], sin)):
+        assert ((got - want).abs() <= 3.01 * 2.0 ** -24 * want.abs()).all(), ((got - want).abs() / want.abs()).max() * 2 ** 24
