@@ -100,3 +100,69 @@ def test_cosines_and_sines_keep_their_own_bits(layout):
     sin = torch.stack([s, c, -s, -c]).gather(0, k[None])[0]
     for got, want in ((out[:, lo], cos), (out[:, hi], sin)):
         assert ((got - want).abs() <= 3.01 * 2.0 ** -24 * want.abs()).all(), ((got - want).abs() / want.abs()).max() * 2 ** 24
+
+
+def behind(stream, fn, *bufs):
+    """Runs fn on `stream` behind a kernel that takes some 20 ms and a copy of the real inputs into
+    buffers of zeros: what is launched anywhere else finds the zeros."""
+    live = [torch.zeros_like(b) for b in bufs]
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(40_000_000)
+        for a, b in zip(live, bufs):
+            a.copy_(b)
+        out = fn(*live)
+    stream.synchronize()
+    return out
+
+
+def test_norm_gate_add_norm_follows_the_current_stream():
+    g = torch.Generator().manual_seed(1)
+    rn = lambda *s: torch.randn(*s, generator=g).to(BF16).cuda()
+    w1, w2, gate = rn(1024), rn(1024), rn(1024)
+
+    def step(x, r, dy):
+        leaves = [t.detach().requires_grad_(True) for t in (x, r, w1, w2, gate)]
+        y, s = fl.fused_norm_gate_add_norm(leaves[0], leaves[1], leaves[4], leaves[2], None, leaves[3])
+        return (y, s, *torch.autograd.grad(y, leaves, dy))
+
+    bufs = [rn(300, 1024) for _ in range(3)]
+    want = step(*bufs)
+    for a, b in zip(behind(torch.cuda.Stream(), step, *bufs), want):
+        assert torch.equal(a, b)
+
+
+def test_qk_norm_rotary_follows_the_current_stream():
+    g = torch.Generator().manual_seed(2)
+    rn = lambda *s: torch.randn(*s, generator=g).to(BF16).cuda()
+    w = rn(128)
+    rot = fl.RotaryAxes(128, (16, 24, 24))
+    pos = torch.arange(3 * 200, device="cuda").view(3, 200)
+
+    def step(q, k, dq, pos):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, w)]
+        o = fl.fused_qk_norm_rotary(leaves[0], leaves[1], pos, rot, leaves[2], leaves[2])
+        grads = torch.autograd.grad(o[0], leaves[::2], dq)
+        with torch.no_grad():
+            place = fl.fused_qk_norm_rotary_(q, k, pos, rot, w, w)
+        return (*o, *grads, *place)
+
+    bufs = [rn(200, 8, 128), rn(200, 2, 128), rn(200, 8, 128), pos]
+    want = step(*[b.clone() for b in bufs])
+    for a, b in zip(behind(torch.cuda.Stream(), step, *bufs), want):
+        assert torch.equal(a, b)
+
+
+def test_in_place_rotary_inside_a_compiled_function():
+    """The in-place form breaks the graph of torch.compile and runs between its parts."""
+    rot, pos = fl.RotaryAxes(64, 32), torch.arange(7, device="cuda")
+    qkv = torch.randn(7, 6, 64, device="cuda", generator=torch.Generator("cuda").manual_seed(0))
+
+    def fn(qkv):
+        qkv = qkv * 2.0
+        q, k = fl.fused_qk_norm_rotary_(qkv[:, :4], qkv[:, 4:5], pos, rot)
+        return q + 1.0, k, qkv
+
+    with torch.no_grad():
+        for a, b in zip(torch.compile(fn, backend="aot_eager")(qkv), fn(qkv)):
+            assert torch.equal(a, b)
