@@ -686,6 +686,53 @@ static bool all_aligned(std::initializer_list<const void*> ps) {
   return true;
 }
 
+// Byte ranges of a call: no output may share a byte with an input or with another output.
+struct NgaRanges {
+  struct Range {
+    uintptr_t from, to;
+  };
+  Range in[12], out[8];
+  int ins = 0, outs = 0;
+  static Range of(const void* p, size_t n) { return {reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + n}; }
+  void reads(const void* p, size_t n) {
+    if (p != nullptr) in[ins++] = of(p, n);
+  }
+  void writes(const void* p, size_t n) {
+    if (p != nullptr) out[outs++] = of(p, n);
+  }
+  bool apart() const {
+    auto meet = [](const Range& a, const Range& b) { return a.from < b.to && b.from < a.to; };
+    for (int o = 0; o < outs; ++o) {
+      for (int i = 0; i < ins; ++i)
+        if (meet(out[o], in[i])) return false;
+      for (int i = 0; i < o; ++i)
+        if (meet(out[o], out[i])) return false;
+    }
+    return true;
+  }
+};
+struct NgaSizes {
+  size_t all, vec, gate, affine, stat;
+  explicit NgaSizes(const fln_nga_args* a) {
+    const size_t es = a->dtype == FLN_F32 ? 4 : 2, groups = (size_t)(a->rows / a->group_rows);
+    vec = (size_t)a->cols * es;
+    all = (size_t)a->rows * vec;
+    gate = a->gate_mode == FLN_GATE_ELEMENT ? all : (a->gate_mode == FLN_GATE_GROUP ? groups * vec : vec);
+    affine = a->affine_grouped ? groups * vec : vec;
+    stat = (size_t)a->rows * sizeof(float);
+  }
+};
+static NgaRanges input_ranges(const fln_nga_args* a, const NgaSizes& n) {
+  NgaRanges r;
+  r.reads(a->x, n.all);
+  r.reads(a->residual, n.all);
+  r.reads(a->gate, n.gate);
+  r.reads(a->post_weight, n.vec);
+  r.reads(a->post_bias, n.vec);
+  r.reads(a->weight, n.affine);
+  return r;
+}
+
 // the column sums of parameters when there are no rows: zeros
 static int zero_grads(const fln_nga_args* a, const NgaGrads& g, cudaStream_t st) {
   const size_t n = (size_t)a->cols * (a->dtype == FLN_F32 ? 4 : 2);
@@ -710,9 +757,18 @@ extern "C" int fln_norm_gate_add_norm_forward(const fln_nga_args* a, void* y, vo
   if (a->rows == 0) return FLN_OK;
   if (a->x == nullptr || sum == nullptr) return FLN_ERR_NULL;
   if (a->kind != FLN_NO_NORM && y == nullptr) return FLN_ERR_NULL;
-  for (const void* q : {(const void*)y, (const void*)sum})
-    if (q != nullptr && (q == a->x || q == a->residual || q == a->gate)) return FLN_ERR_ARG;
-  if (y == sum) return FLN_ERR_ARG;
+  // (a statistic that the call has none of is not written)
+  if (a->post_kind != FLN_LAYERNORM) post_mean = nullptr;
+  if (a->post_kind == FLN_NO_NORM) post_rstd = nullptr;
+  if (a->kind != FLN_LAYERNORM) mean = nullptr;
+  if (a->kind == FLN_NO_NORM) y = nullptr, rstd = nullptr;
+  const NgaSizes n(a);
+  NgaRanges ranges = input_ranges(a, n);
+  ranges.reads(a->bias, n.affine);
+  ranges.writes(y, n.all);
+  ranges.writes(sum, n.all);
+  for (const float* q : {post_mean, post_rstd, mean, rstd}) ranges.writes(q, n.stat);
+  if (!ranges.apart()) return FLN_ERR_ARG;
   NgaParams p = base_params(a);
   p.y = y;
   p.sum = sum;
@@ -792,8 +848,6 @@ extern "C" int fln_norm_gate_add_norm_backward(const fln_nga_args* a, const floa
   if (a->x == nullptr) return FLN_ERR_NULL;
   if (dy != nullptr && (rstd == nullptr || (a->kind == FLN_LAYERNORM && mean == nullptr)))
     return FLN_ERR_NULL;
-  for (const void* q : {(const void*)dx, (const void*)dresidual, (const void*)dgate})
-    if (q != nullptr && (q == a->x || q == a->residual || q == a->gate || q == dy || q == dsum)) return FLN_ERR_ARG;
   if (a->post_kind != FLN_NO_NORM && (post_rstd == nullptr || (a->post_kind == FLN_LAYERNORM && post_mean == nullptr)))
     return FLN_ERR_NULL;
   NgaParams p = base_params(a);
@@ -811,12 +865,31 @@ extern "C" int fln_norm_gate_add_norm_backward(const fln_nga_args* a, const floa
   if (g.dw2 != nullptr) p.acc |= kAccU;
   if (g.db2 != nullptr) p.acc |= kAccV;
   p.nacc = __builtin_popcount((unsigned)p.acc);
+  size_t scratch = 0;
   if (p.acc != 0) {
-    if (workspace == nullptr || workspace_bytes < fln_norm_gate_add_norm_workspace_bytes(a)) return FLN_ERR_WORKSPACE;
+    scratch = fln_norm_gate_add_norm_workspace_bytes(a);
+    if (workspace == nullptr || workspace_bytes < scratch) return FLN_ERR_WORKSPACE;
     if (!is_aligned16(workspace)) return FLN_ERR_WORKSPACE;
     p.row_c = reinterpret_cast<float*>(workspace);
     p.partials = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + align256((size_t)p.rows * 8));
   }
+  const NgaSizes n(a);
+  NgaRanges ranges = input_ranges(a, n);
+  ranges.reads(dy, n.all);
+  ranges.reads(dsum, n.all);
+  if (a->post_kind == FLN_LAYERNORM) ranges.reads(post_mean, n.stat);
+  if (a->post_kind != FLN_NO_NORM) ranges.reads(post_rstd, n.stat);
+  if (dy != nullptr && a->kind == FLN_LAYERNORM) ranges.reads(mean, n.stat);
+  if (dy != nullptr) ranges.reads(rstd, n.stat);
+  ranges.writes(dx, n.all);
+  ranges.writes(dresidual, n.all);
+  ranges.writes(dgate, n.gate);
+  ranges.writes(dpost_weight, n.vec);
+  ranges.writes(dpost_bias, n.vec);
+  ranges.writes(dweight, n.affine);
+  ranges.writes(dbias, n.affine);
+  if (p.acc != 0) ranges.writes(workspace, scratch);
+  if (!ranges.apart()) return FLN_ERR_ARG;
   const bool aligned = all_aligned({a->x, a->residual, a->gate, a->post_weight, a->post_bias, a->weight, dy, dsum, dx,
                                     dresidual, dgate});
   switch (a->dtype) {

@@ -195,6 +195,12 @@ extern "C" int fln_qk_norm_rotary_forward(const fln_rotary_args* a, void* stream
   if (empty(a)) return FLN_OK;
   rc = check_pointers(a);
   if (rc != FLN_OK) return rc;
+  for (const fln_rotary_tensor& t : a->t) {  // in place: every row is read by the warp that writes it
+    if (t.heads > 0 && t.in == t.out &&
+        ((a->batch > 1 && t.in_batch != t.out_batch) || (a->seq > 1 && t.in_seq != t.out_seq) ||
+         (t.heads > 1 && t.in_head != t.out_head)))
+      return FLN_ERR_ARG;
+  }
   RotParams p = base_params(a);
   const RotPlan plan = make_rot_plan(a, nullptr, &p);
   return launch(a->dtype, p, plan, false, 0, reinterpret_cast<cudaStream_t>(stream));

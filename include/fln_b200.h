@@ -428,10 +428,10 @@ typedef struct {
   float branch_scale, residual_scale, weight_offset, post_eps, eps;
 } fln_nga_args;
 
-/* y may be NULL when kind is FLN_NO_NORM, and only then.  Outputs may not overlap inputs (a row can
- * be read again after it was written).  The statistics (fp32 [rows], each may
+/* y may be NULL when kind is FLN_NO_NORM, and only then.  The statistics (fp32 [rows], each may
  * be NULL) are what the backward reads: post_mean / mean of a LayerNorm, post_rstd / rstd of
- * either norm. */
+ * either norm.  An output that shares a byte with an input or with another output is refused
+ * (FLN_ERR_ARG): a row can be read again after it was written. */
 int fln_norm_gate_add_norm_forward(const fln_nga_args* a, void* y, void* sum, float* post_mean, float* post_rstd,
                                    float* mean, float* rstd, void* stream);
 
@@ -442,7 +442,8 @@ size_t fln_norm_gate_add_norm_workspace_bytes(const fln_nga_args* a);
 /* Gradients from dy (of y; may be NULL) and dsum (of sum; may be NULL, but not both) and the
  * forward's inputs: the 32-bit sum is made again from x and residual.  Every gradient may be
  * NULL (not computed); each has the shape and type of its tensor.  Sums over
- * rows are made in 32 bits in a fixed order: repeated calls agree bit for bit. */
+ * rows are made in 32 bits in a fixed order: repeated calls agree bit for bit.  Gradients and
+ * workspace may not share a byte with an input or with each other (FLN_ERR_ARG). */
 int fln_norm_gate_add_norm_backward(const fln_nga_args* a, const float* post_mean,
                                     const float* post_rstd, const float* mean, const float* rstd, const void* dy,
                                     const void* dsum, void* dx, void* dresidual, void* dgate, void* dpost_weight,
@@ -464,7 +465,10 @@ typedef enum { FLN_ROTARY_HALF = 0, FLN_ROTARY_INTERLEAVED = 1 } fln_rotary_layo
 
 typedef struct {
   const void* in; /* [batch, seq, heads, head_dim] with these strides */
-  void* out;      /* may be `in` with the same strides: every row is read before it is written */
+  /* may be `in`, with the same strides (else FLN_ERR_ARG): every row is read before it is written.
+   * Beyond that nothing is checked: strided views share their ranges, so it is for the caller that
+   * no element of an output is an element of any other tensor of the call. */
+  void* out;
   int64_t in_batch, in_seq, in_head;
   int64_t out_batch, out_seq, out_head;
   const void* weight; /* [head_dim] or NULL */
@@ -494,7 +498,7 @@ size_t fln_qk_norm_rotary_workspace_bytes(const fln_rotary_args* a);
 
 /* a->t[].in are the forward's inputs and a->t[].out the gradients of its outputs (read; with
  * the out strides).  dx[i]: gradient of t[i].in, contiguous [batch, seq, heads, head_dim], may
- * be NULL.  dweight / dbias: [head_dim], may be NULL.  Fixed order of summation. */
+ * be NULL, overlaps nothing (not checked).  dweight / dbias: [head_dim], may be NULL.  Fixed order of summation. */
 int fln_qk_norm_rotary_backward(const fln_rotary_args* a, void* const dx[2], void* const dweight[2],
                                 void* const dbias[2], void* workspace, size_t workspace_bytes, void* stream);
 
