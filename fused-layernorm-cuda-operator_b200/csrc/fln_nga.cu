@@ -534,10 +534,17 @@ static int plan_forward(NgaParams* pp, int es, NgaGeom* g) {
   return K;
 }
 
+// What a backward plan reads of the library's settings.  A call reads them once: the workspace that it asks
+// for and the slots that it fills come from the same numbers, also while another thread changes them.
+struct NgaSettings {
+  int sms = usable_sms(), K = 0, tpr = 0;
+  NgaSettings() { plan_override(&K, &tpr); }
+};
+
 // The backward's plan: threads and shared memory so that an SM holds as many threads as the
 // kernels' registers allow (640 with 8 elements per thread, 512 with 16), at least two rows on
 // their way per row group.  Fills p's slots.  K = 0: not for the row kernels.
-static int plan_backward(NgaParams* p, int es, NgaGeom* g) {
+static int plan_backward(NgaParams* p, int es, const NgaSettings& settings, NgaGeom* g) {
   if (!row_vectors(p, es)) return 0;
   const int vec = 16 / es;
   g->nv = row_vector_count(*p, es);
@@ -546,9 +553,7 @@ static int plan_backward(NgaParams* p, int es, NgaGeom* g) {
   // one CTA of either: 8192 x 4096, 145 us with 512 threads, 165 with 256)
   const bool eight = nga_general(*p) || es == 4;
   int E = eight ? 8 : 16;
-  int fK = 0, ftpr = 0;
-  plan_override(&fK, &ftpr);
-  if (fK == 1 || fK == 2) E = 8 * fK;
+  if (settings.K == 1 || settings.K == 2) E = 8 * settings.K;
   if (threads_per_row(g->nv, E / vec) > most(E)) E = 16;
   const int K = E / vec;
   g->tpr = threads_per_row(g->nv, K);
@@ -595,7 +600,7 @@ static int plan_backward(NgaParams* p, int es, NgaGeom* g) {
   // cost (its partial rows) counts as one more step.
   const int64_t groups = p->rows / p->group_rows, T = p->group_rows;
   const int64_t slots_max = (T + g->R - 1) / g->R;
-  const int64_t cta = g->pair ? usable_sms() / 2 : (int64_t)usable_sms() * ctas;  // (or pairs of them)
+  const int64_t cta = g->pair ? settings.sms / 2 : (int64_t)settings.sms * ctas;  // (or pairs of them)
   if (cta < 1) return 0;
   if (p->period > 1) {
     const int64_t n = (T + p->period - 1) / p->period, per = groups * p->classes;
@@ -655,11 +660,11 @@ static int finalize(NgaParams p, const NgaGrads& g, cudaStream_t st) {
 }
 
 template <typename T>
-static int run_backward(NgaParams p, const NgaGrads& g, bool aligned, cudaStream_t st) {
+static int run_backward(NgaParams p, const NgaGrads& g, bool aligned, const NgaSettings& settings, cudaStream_t st) {
   if (aligned) {
     NgaParams q = p;
     NgaGeom geom = {};
-    const int K = plan_backward(&q, (int)sizeof(T), &geom);
+    const int K = plan_backward(&q, (int)sizeof(T), settings, &geom);
     if (K != 0) {
       q.partials = p.row_c;  // the whole workspace: the row scalars are not kept
       const int rc = nga_bwd_rows<T>(q, geom, K, st);
@@ -678,6 +683,28 @@ static int run_backward(NgaParams p, const NgaGrads& g, bool aligned, cudaStream
     return finalize<T>(p, g, st);
   }
   return FLN_OK;
+}
+
+static size_t workspace_bytes_of(const fln_nga_args* a, const NgaSettings& settings) {
+  // the most that any of the plans takes: which one it is depends on the gradients asked for and
+  // on the alignment of all tensors
+  NgaParams p = base_params(a);
+  const size_t row = 4 * (size_t)p.cols * 4;
+  plan_slots(&p);
+  size_t most = align256((size_t)p.rows * 8) + (size_t)p.slots * row;
+  for (int acc = kAccP | kAccU; acc <= 15; acc += kAccQ | kAccV) {
+    for (int grads = 1; grads <= 3; ++grads) {  // dy, dsum, both
+      NgaParams q = base_params(a);
+      NgaGeom g = {};
+      q.acc = acc;
+      q.dy = (grads & 1) != 0 && a->kind != FLN_NO_NORM ? a->x : nullptr;
+      q.ds = (grads & 2) != 0 ? a->x : nullptr;
+      if (plan_backward(&q, a->dtype == FLN_F32 ? 4 : 2, settings, &g) == 0) continue;
+      const size_t n = (size_t)q.slots * row;
+      if (n > most) most = n;
+    }
+  }
+  return most;
 }
 
 static bool all_aligned(std::initializer_list<const void*> ps) {
@@ -803,26 +830,7 @@ extern "C" int fln_norm_gate_add_norm_forward(const fln_nga_args* a, void* y, vo
 }
 
 extern "C" size_t fln_norm_gate_add_norm_workspace_bytes(const fln_nga_args* a) {
-  if (check_args(a) != FLN_OK || a->rows == 0) return 0;
-  // the most that any of the plans takes: which one it is depends on the gradients asked for and
-  // on the alignment of all tensors
-  NgaParams p = base_params(a);
-  const size_t row = 4 * (size_t)p.cols * 4;
-  plan_slots(&p);
-  size_t most = align256((size_t)p.rows * 8) + (size_t)p.slots * row;
-  for (int acc = kAccP | kAccU; acc <= 15; acc += kAccQ | kAccV) {
-    for (int grads = 1; grads <= 3; ++grads) {  // dy, dsum, both
-      NgaParams q = base_params(a);
-      NgaGeom g = {};
-      q.acc = acc;
-      q.dy = (grads & 1) != 0 && a->kind != FLN_NO_NORM ? a->x : nullptr;
-      q.ds = (grads & 2) != 0 ? a->x : nullptr;
-      if (plan_backward(&q, a->dtype == FLN_F32 ? 4 : 2, &g) == 0) continue;
-      const size_t n = (size_t)q.slots * row;
-      if (n > most) most = n;
-    }
-  }
-  return most;
+  return check_args(a) != FLN_OK || a->rows == 0 ? 0 : workspace_bytes_of(a, NgaSettings());
 }
 
 extern "C" int fln_norm_gate_add_norm_backward(const fln_nga_args* a, const float* post_mean,
@@ -865,9 +873,10 @@ extern "C" int fln_norm_gate_add_norm_backward(const fln_nga_args* a, const floa
   if (g.dw2 != nullptr) p.acc |= kAccU;
   if (g.db2 != nullptr) p.acc |= kAccV;
   p.nacc = __builtin_popcount((unsigned)p.acc);
+  const NgaSettings settings;
   size_t scratch = 0;
   if (p.acc != 0) {
-    scratch = fln_norm_gate_add_norm_workspace_bytes(a);
+    scratch = workspace_bytes_of(a, settings);
     if (workspace == nullptr || workspace_bytes < scratch) return FLN_ERR_WORKSPACE;
     if (!is_aligned16(workspace)) return FLN_ERR_WORKSPACE;
     p.row_c = reinterpret_cast<float*>(workspace);
@@ -894,10 +903,10 @@ extern "C" int fln_norm_gate_add_norm_backward(const fln_nga_args* a, const floa
                                     dresidual, dgate});
   switch (a->dtype) {
     case FLN_F32:
-      return run_backward<float>(p, g, aligned, st);
+      return run_backward<float>(p, g, aligned, settings, st);
     case FLN_BF16:
-      return run_backward<__nv_bfloat16>(p, g, aligned, st);
+      return run_backward<__nv_bfloat16>(p, g, aligned, settings, st);
     default:
-      return run_backward<__half>(p, g, aligned, st);
+      return run_backward<__half>(p, g, aligned, settings, st);
   }
 }

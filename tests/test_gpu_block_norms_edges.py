@@ -166,3 +166,43 @@ def test_in_place_rotary_inside_a_compiled_function():
     with torch.no_grad():
         for a, b in zip(torch.compile(fn, backend="aot_eager")(qkv), fn(qkv)):
             assert torch.equal(a, b)
+
+
+def test_backward_while_another_thread_changes_the_sm_reserve():
+    """A backward plans with the settings of one moment: beside a thread that moves the reserve it is
+    right, or refused for the workspace that was asked for at another moment."""
+    import threading
+    from fused_layernorm import _capi as capi
+    g = torch.Generator().manual_seed(4)
+    rn = lambda *s: torch.randn(*s, generator=g).to(BF16).cuda()
+    t = dict.fromkeys(R.NAMES)
+    t.update(input=rn(900, 512), residual=rn(900, 512), post_weight=rn(512), weight=rn(512))
+    dy = rn(900, 512)
+    leaves = {k: v.requires_grad_(True) for k, v in t.items() if v is not None}
+    want = R.nga_bounds({k: None if v is None else v.detach().double() for k, v in t.items()}, dy.double(), None, BF16, "rmsnorm",
+                        "rmsnorm", "none", 1.0, 1.0, 0.0)["grads"]
+    lib, stop = capi.lib(), threading.Event()
+
+    def move():
+        while not stop.is_set():
+            for n in (0, 100, 40, 140):
+                lib.fln_set_sm_reserve(n)
+
+    mover, right = threading.Thread(target=move), 0
+    mover.start()
+    try:
+        for _ in range(200):
+            y, s = fl.fused_norm_gate_add_norm(t["input"], t["residual"], None, t["post_weight"], None, t["weight"], None,
+                                               post_eps=R.EPS1, eps=R.EPS2)
+            try:
+                got = torch.autograd.grad(y, list(leaves.values()), dy)
+            except RuntimeError as e:
+                assert "workspace" in str(e)
+                continue
+            right += 1
+            for k, v in zip(leaves, got):
+                R.check(v, want[k], k)
+    finally:
+        stop.set(), mover.join()
+        lib.fln_set_sm_reserve(0)
+    assert right > 0
