@@ -358,7 +358,8 @@ __device__ __forceinline__ void coef1(const NgaParams& p, int col, int64_t goff,
     b[e] = f2mul(b[e], a[e]);
   }
 }
-template <typename T, bool SHIFT>
+// (BIAS: the backward has no use for B2)
+template <typename T, bool SHIFT, bool BIAS>
 __device__ __forceinline__ void coef2(const NgaParams& p, int col, int64_t aoff, float2 (&c)[8 / sizeof(T)], float2 (&b)[8 / sizeof(T)]) {
   constexpr int V2 = 8 / (int)sizeof(T);
 #pragma unroll
@@ -371,7 +372,7 @@ __device__ __forceinline__ void coef2(const NgaParams& p, int col, int64_t aoff,
 #pragma unroll
     for (int e = 0; e < V2; ++e) c[e] = f2add(c[e], f2(p.woff));
   }
-  if (p.b2 != nullptr) param2<T, SHIFT>(p.b2, aoff, col, p.cols, b);
+  if (BIAS && p.b2 != nullptr) param2<T, SHIFT>(p.b2, aoff, col, p.cols, b);
 }
 
 // ----------------------------------------------------------------------------------------
@@ -463,7 +464,7 @@ __global__ void __launch_bounds__(TPR == 320 ? 320 : 512, TPR == 320 && sizeof(T
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       coef1<T, GATE, SHIFT>(p, w.at[k], goff, c1[HOLD ? k : 0], b1[HOLD && GEN ? k : 0]);
-      coef2<T, SHIFT>(p, w.at[k], aoff, c2[HOLD ? k : 0], b2[HOLD && GEN ? k : 0]);
+      coef2<T, SHIFT, true>(p, w.at[k], aoff, c2[HOLD ? k : 0], b2[HOLD && GEN ? k : 0]);
     }
   }
   const float2 ra = f2(p.ra);
@@ -529,7 +530,7 @@ __global__ void __launch_bounds__(TPR == 320 ? 320 : 512, TPR == 320 && sizeof(T
       for (int k = 0; k < K; ++k) {
         {
           float2 tc[V2], tb[V2];
-          if (!HOLD) coef2<T, SHIFT>(p, w.at[k], aoff, tc, tb);
+          if (!HOLD) coef2<T, SHIFT, true>(p, w.at[k], aoff, tc, tb);
 #pragma unroll
           for (int e = 0; e < V2; ++e) {
             if (GEN) s[k][e] = f2add(s[k][e], f2(-mean2));
@@ -776,7 +777,7 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
               if (GEN) put(l.b1, b);
             }
             if (has_dy && (first || p.affine_grouped)) {
-              coef2<T, SHIFT>(p, w.at[k], aoff, c, b);
+              coef2<T, SHIFT, false>(p, w.at[k], aoff, c, b);
               put(l.c2, c);
             }
           }
@@ -842,7 +843,7 @@ __global__ void __launch_bounds__(K * 16 / (int)sizeof(T) <= 8 ? 640 : 512) nga_
             for (int e = 0; e < V2; ++e) g2[k][e] = f2only(live && w.ok[k], g2[k][e]);
           }
           if (CSM) coef(l.c2, k, c);
-          else coef2<T, SHIFT>(p, w.at[k], aoff, c, b);
+          else coef2<T, SHIFT, false>(p, w.at[k], aoff, c, b);
 #pragma unroll
           for (int e = 0; e < V2; ++e) {
             if (GEN) sh[k][e] = f2add(sh[k][e], f2(-sc.mean2));

@@ -206,3 +206,27 @@ def test_backward_while_another_thread_changes_the_sm_reserve():
         stop.set(), mover.join()
         lib.fln_set_sm_reserve(0)
     assert right > 0
+
+
+@pytest.mark.parametrize("post", [None, "layernorm"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_unaligned_bias_beside_aligned_tensors(dtype, post):
+    """The backward has no use for the second norm's bias: one that lies off a vector boundary, alone,
+    leaves the backward with the kernels for aligned tensors."""
+    g = torch.Generator().manual_seed(6)
+    rn = lambda *s: torch.randn(*s, generator=g).to(dtype).cuda()
+    t = dict.fromkeys(R.NAMES)
+    t.update(input=rn(70, 640), residual=rn(70, 640), weight=rn(640), bias=rn(641)[1:])
+    if post:
+        t.update(post_weight=rn(640), post_bias=rn(640))
+    dy, ds = rn(70, 640), rn(70, 640)
+    leaves = {k: v.detach().requires_grad_(True) for k, v in t.items() if v is not None}
+    assert leaves["bias"].data_ptr() % 16
+    want = R.nga_bounds({k: None if v is None else v.double() for k, v in t.items()}, dy.double(), ds.double(), dtype, post or "none",
+                        "layernorm", "none", 1.0, 1.0, 0.0)
+    y, s = fl.fused_norm_gate_add_norm(leaves["input"], leaves["residual"], None, leaves.get("post_weight"), leaves.get("post_bias"),
+                                       leaves["weight"], leaves["bias"], post_norm=post, norm="layernorm", post_eps=R.EPS1,
+                                       eps=R.EPS2)
+    R.check(y.detach(), want["y"], "y"), R.check(s.detach(), want["sum"], "sum")
+    for k, v in zip(leaves, torch.autograd.grad([y, s], list(leaves.values()), [dy, ds])):
+        R.check(v, want["grads"][k], k)
