@@ -499,7 +499,10 @@ static int plan_forward(NgaParams* pp, int es, NgaGeom* g) {
   if (threads_per_row(nv, E / vec) > 512) return 0;
   const int K = E / vec;
   g->tpr = threads_per_row(nv, K);
-  if (p.period == 1 && E == 16 && K * g->tpr != nv && nga_ragged_tpr(g->tpr) != 0) g->tpr = nga_ragged_tpr(g->tpr);
+  if (p.period == 1 && E == 16) {
+    const int fixed = fixed_tpr(g->tpr, K * g->tpr == nv, 512);
+    if (fixed != 0) g->tpr = fixed;
+  }
   rows_per_cta(g);
   const int tensors = 1 + (p.res != nullptr) + (p.gate_mode == FLN_GATE_ELEMENT);
   g->stages = 3;
@@ -563,37 +566,44 @@ static int plan_backward(NgaParams* p, int es, const NgaSettings& settings, NgaG
     if (g->tpr > 512) return 0;
   }
   const int set = p->period == 1 && !g->pair ? nga_set_of(*p) : 0;  // (0: dsum never past the ring)
-  if (set == 1 && E == (eight ? 8 : 16) && K * g->tpr != g->nv && nga_ragged_tpr(g->tpr) != 0 && g->tpr > 96)
-    g->tpr = nga_ragged_tpr(g->tpr);
-  rows_per_cta(g);
-  g->rep = g->tpr < 32 ? g->threads / 32 : g->R;
-  const size_t unit = (size_t)K * g->threads * 16;
-  int ctas = most(E) / g->threads;
-  if (ctas < 1) ctas = 1;
-  // as many CTAs as the registers allow if two rows each fit, else fewer; then dsum past the ring,
-  // then the coefficients out of it, and a ring of one row last
-  bool fits = false;
-  auto fit = [&](int ctas, int csm, int direct, int rows) {
-    const size_t per = (size_t)227 * 1024 / ctas - 1024;  // the runtime keeps 1 KB of every CTA
-    const NgaBwdLayout l = nga_bwd_layout(*p, es, csm != 0, nga_general(*p), direct != 0);
-    const size_t joint = g->rep > 1 ? (size_t)g->rep * g->tpr * vec * 4 : 0;
-    const size_t fixed = kNgaBwdHeader + (size_t)l.coefs * unit + joint, stage = (size_t)l.tensors * unit;
-    if (fixed + rows * stage > per) return false;
-    int s = (int)((per - fixed) / stage);
-    if (s > 3) s = 3;
-    g->csm = csm;
-    g->direct = direct;
-    g->stages = s;
-    g->smem = fixed + (size_t)s * stage;
-    return true;
-  };
-  for (; ctas >= 1 && !fits; --ctas) {
-    fits = fit(ctas, 1, 0, 2);
-    if (fits) break;
-  }
-  if (!fits) {
+  int ctas = 1;
+  // Lays out a CTA for rows of `tpr` threads: as many CTAs as the registers allow if two rows each fit, else
+  // fewer; then dsum past the ring, then the coefficients out of it, and a ring of one row last.
+  auto lay_out = [&](int tpr) {
+    g->tpr = tpr;
+    rows_per_cta(g);
+    g->rep = g->tpr < 32 ? g->threads / 32 : g->R;
+    const size_t unit = (size_t)K * g->threads * 16;
+    auto fit = [&](int ctas, int csm, int direct, int rows) {
+      const size_t per = (size_t)227 * 1024 / ctas - 1024;  // the runtime keeps 1 KB of every CTA
+      const NgaBwdLayout l = nga_bwd_layout(*p, es, csm != 0, nga_general(*p), direct != 0);
+      const size_t joint = g->rep > 1 ? (size_t)g->rep * g->tpr * vec * 4 : 0;
+      const size_t fixed = kNgaBwdHeader + (size_t)l.coefs * unit + joint, stage = (size_t)l.tensors * unit;
+      if (fixed + rows * stage > per) return false;
+      int s = (int)((per - fixed) / stage);
+      if (s > 3) s = 3;
+      g->csm = csm;
+      g->direct = direct;
+      g->stages = s;
+      g->smem = fixed + (size_t)s * stage;
+      return true;
+    };
+    ctas = most(E) / g->threads;
+    if (ctas < 1) ctas = 1;
+    for (; ctas >= 1; --ctas)
+      if (fit(ctas, 1, 0, 2)) return true;
     ctas = 1;
-    fits = (set == 1 && fit(1, 1, 1, 2)) || fit(1, 0, 0, 2) || (set == 1 && fit(1, 0, 1, 2)) || fit(1, 1, 0, 1) || fit(1, 0, 0, 1);
+    return (set == 1 && fit(1, 1, 1, 2)) || fit(1, 0, 0, 2) || (set == 1 && fit(1, 0, 1, 2)) || fit(1, 1, 0, 1) || fit(1, 0, 0, 1);
+  };
+  // A compile-time number of threads, unless only its idle ones put dsum past the ring or the coefficients
+  // out of it, or dsum is past it and there is no such kernel (not the general form).
+  auto grade = [&](bool fits) { return !fits ? 0 : (!g->csm ? 1 : (g->direct ? 2 : 3)); };
+  const int tpr = g->tpr, fixed = set == 1 && E == (eight ? 8 : 16) ? fixed_tpr(tpr, K * tpr == g->nv, most(E)) : 0;
+  bool fits = lay_out(fixed != 0 ? fixed : tpr);
+  if (fixed != 0 && fixed != tpr && grade(fits) < 3) {
+    const int with_fixed = grade(fits);
+    fits = lay_out(tpr);
+    if (grade(fits) < with_fixed || (grade(fits) == with_fixed && nga_general(*p))) fits = lay_out(fixed);
   }
   if (!fits) return 0;
   // Slots: as many per group as give every CTA the same number of row steps, nearly; a slot's own

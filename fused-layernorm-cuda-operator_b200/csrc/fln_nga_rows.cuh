@@ -63,6 +63,27 @@ struct NgaGeom {
 // 4096 columns, 51 -> 28 of the backward.  Rows per CTA of these:
 __host__ __device__ constexpr int fixed_rows(int tpr) { return tpr >= 128 ? 1 : (tpr > 32 ? 2 : 256 / tpr); }
 
+// Numbers of threads per row that are known at compile time: 4 to 64 for short rows that are whole (heads
+// of 32 to 512 elements: 524288 x 64 bf16 with a gate per element, backward 116 us at run time, 71 so),
+// and for longer ones the next of this list where that leaves few of them idle (8192 x 5064 bf16, two
+// LayerNorms with biases, backward 193 us at run time, 151 so).  Whole rows of a number of their own
+// keep it where the next one would idle more than an eighth of the threads (288 -> 320 threads, 8192 x
+// 4608 bf16: forward 147 -> 102 us; 160 -> 192, 16384 x 2560: backward 101 -> 116).  0: everything is
+// found out at run time.  All but 192, 384 and (dsum past the ring) 640 have a kernel for rows that fill
+// their threads besides the one for rows that do not: there it gained nothing (16384 x 6144 bf16: 212
+// and 208 us backward, 16384 x 1536 general: 91 and 95).
+constexpr int kFixedTpr[] = {128, 192, 256, 320, 384, 512, 640};
+inline int fixed_tpr(int tpr, bool whole, int most) {
+  for (int t : kFixedTpr)
+    if (t >= tpr && t <= most && (t - tpr) * (whole ? 8 : 6) <= t) return t;
+  return 0;
+}
+// Forward: what fits once on an SM may have all of its registers; two CTAs where that leaves 96 for a
+// thread and the ring of 16-bit rows leaves the shared memory (16384 x 5120 bf16 with a gate per element
+// and two LayerNorms: 300 -> 207 us; up to 256 threads the bound of 128 registers does it by itself).
+__host__ __device__ constexpr int fwd_threads(int tpr) { return tpr > 256 ? tpr : 512; }
+__host__ __device__ constexpr int fwd_ctas(int es, int tpr) { return es == 2 && tpr > 256 && 2 * 96 * tpr <= 65536 ? 2 : 1; }
+
 // ----------------------------------------------------------------------------------------
 // sums over the threads of a row
 // ----------------------------------------------------------------------------------------
@@ -383,10 +404,8 @@ __device__ __forceinline__ void coef2(const NgaParams& p, int col, int64_t aoff,
 // GATE 0: none, 1: shared by rows, 2: an element each.  HOLD: the coefficients stay in registers
 // over the chunk, else they are made again for every row (rows too long for that).
 // ----------------------------------------------------------------------------------------
-// (320 threads of a 16-bit type: registers for two CTAs on an SM; 16384 x 5120 bf16 with a gate per
-// element and two LayerNorms 300 -> 207 us)
 template <typename T, int K, int GATE, bool GEN, bool HOLD, int TPR, bool RAG, bool SHIFT>
-__global__ void __launch_bounds__(TPR == 320 ? 320 : 512, TPR == 320 && sizeof(T) == 2 ? 2 : 1) nga_fwd_rows_kernel(const NgaParams p, const NgaGeom g) {
+__global__ void __launch_bounds__(fwd_threads(TPR), fwd_ctas((int)sizeof(T), TPR)) nga_fwd_rows_kernel(const NgaParams p, const NgaGeom g) {
   constexpr bool EXACT = sizeof(T) == 4;
   constexpr int VEC = 16 / (int)sizeof(T), V2 = VEC / 2;
   extern __shared__ __align__(128) unsigned char smem[];
@@ -1067,14 +1086,6 @@ static int nga_launch(const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
   FLN_CHECK_LAUNCH();
   return FLN_OK;
 }
-// Threads per row of the compile-time kernels for rows that are not whole: the next of these where
-// that leaves at most a sixth of the threads idle, else 0 (everything found out at run time).
-inline int nga_ragged_tpr(int tpr) {
-  const int list[] = {128, 192, 256, 320, 384, 512};
-  for (int t : list)
-    if (t >= tpr && (t - tpr) * 6 <= t) return t;
-  return 0;
-}
 template <typename T, int K, int GATE, int TPR, bool RAG, bool SHIFT = false>
 static int nga_fwd_rows_t(const NgaParams& p, const NgaGeom& g, cudaStream_t st) {
   constexpr bool HOLD = K * 16 / (int)sizeof(T) <= 16;
@@ -1086,36 +1097,33 @@ static int nga_fwd_rows_k(const NgaParams& p, const NgaGeom& g, cudaStream_t st)
   if (p.period > 1) return nga_fwd_rows_t<T, K, GATE, 0, false, true>(p, g, st);
   // compile-time rows: 16 elements per thread
   if constexpr (K * 16 / (int)sizeof(T) == 16) {
-    if (g.nv == K * g.tpr) {
-      switch (g.tpr) {
-        case 8:
-          return nga_fwd_rows_t<T, K, GATE, 8, false>(p, g, st);
-        case 64:
-          return nga_fwd_rows_t<T, K, GATE, 64, false>(p, g, st);
-        case 128:
-          return nga_fwd_rows_t<T, K, GATE, 128, false>(p, g, st);
-        case 256:
-          return nga_fwd_rows_t<T, K, GATE, 256, false>(p, g, st);
-        case 320:
-          return nga_fwd_rows_t<T, K, GATE, 320, false>(p, g, st);
-        case 512:
-          return nga_fwd_rows_t<T, K, GATE, 512, false>(p, g, st);
-      }
-    }
+    const bool whole = g.nv == K * g.tpr;
+#define FLN_NGA_SHORT(TPR) \
+  case TPR:                \
+    if (whole) return nga_fwd_rows_t<T, K, GATE, TPR, false>(p, g, st); \
+    break;
+#define FLN_NGA_RAG(TPR) \
+  case TPR:              \
+    return nga_fwd_rows_t<T, K, GATE, TPR, true>(p, g, st);
+#define FLN_NGA_LONG(TPR) \
+  case TPR:               \
+    return whole ? nga_fwd_rows_t<T, K, GATE, TPR, false>(p, g, st) : nga_fwd_rows_t<T, K, GATE, TPR, true>(p, g, st);
     switch (g.tpr) {
-      case 128:
-        return nga_fwd_rows_t<T, K, GATE, 128, true>(p, g, st);
-      case 192:
-        return nga_fwd_rows_t<T, K, GATE, 192, true>(p, g, st);
-      case 256:
-        return nga_fwd_rows_t<T, K, GATE, 256, true>(p, g, st);
-      case 320:
-        return nga_fwd_rows_t<T, K, GATE, 320, true>(p, g, st);
-      case 384:
-        return nga_fwd_rows_t<T, K, GATE, 384, true>(p, g, st);
-      case 512:
-        return nga_fwd_rows_t<T, K, GATE, 512, true>(p, g, st);
+      FLN_NGA_SHORT(4)
+      FLN_NGA_SHORT(8)
+      FLN_NGA_SHORT(16)
+      FLN_NGA_SHORT(32)
+      FLN_NGA_SHORT(64)
+      FLN_NGA_LONG(128)
+      FLN_NGA_RAG(192)
+      FLN_NGA_LONG(256)
+      FLN_NGA_LONG(320)
+      FLN_NGA_RAG(384)
+      FLN_NGA_LONG(512)
     }
+#undef FLN_NGA_RAG
+#undef FLN_NGA_SHORT
+#undef FLN_NGA_LONG
   }
   return nga_fwd_rows_t<T, K, GATE, 0, false>(p, g, st);
 }
@@ -1136,10 +1144,13 @@ static int nga_bwd_rows_g(const NgaParams& p, const NgaGeom& g, cudaStream_t st)
     return nga_set_of(p) == 1 ? nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 1, true>>(p, g, st)
                               : nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 0, true>>(p, g, st);
   }
+  const bool whole = g.nv == K * g.tpr;
   if (g.direct) {
-    // (fp32 rows of 5120, general form: 84 us at 2047 rows with the threads per row found out at run time, 67 so)
-    if constexpr (sizeof(T) == 4 && K * 16 / (int)sizeof(T) == 8) {
-      if (g.csm && g.nv == K * g.tpr && g.tpr == 640) return nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, true, 640, false, 3, false>>(p, g, st);
+    // (640 threads come here in fp32 with a gate per element.  General form, 2047 rows of 4864 / 5056: 101 /
+    // 103 us with the threads found out at run time, 87 / 87 so; without means and biases 4096 rows of 4864
+    // take 118 us at run time, 134 so)
+    if constexpr (sizeof(T) == 4 && K * 16 / (int)sizeof(T) == 8 && GATE == 2 && GEN) {
+      if (g.csm && g.tpr == 640) return nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, true, 640, true, 3, false>>(p, g, st);
     }
     return g.csm ? nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 3, false>>(p, g, st)
                  : nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, false, 0, false, 3, false>>(p, g, st);
@@ -1148,39 +1159,43 @@ static int nga_bwd_rows_g(const NgaParams& p, const NgaGeom& g, cudaStream_t st)
   const int set = nga_set_of(p);
   // compile-time rows where the registers allow: 16 elements per thread, 8 of the general form and of fp32
   if constexpr (K * 16 / (int)sizeof(T) == (GEN || sizeof(T) == 4 ? 8 : 16)) {
-#define FLN_NGA_BWD(TPR, RAG, SET) \
-  case TPR:                        \
-    return nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, true, TPR, RAG, SET, false>>(p, g, st);
-    if (g.nv == K * g.tpr && set == 1) {
-      switch (g.tpr) {
-        FLN_NGA_BWD(64, false, 1)
-        FLN_NGA_BWD(128, false, 1)
-        FLN_NGA_BWD(256, false, 1)
-        FLN_NGA_BWD(320, false, 1)
-        FLN_NGA_BWD(512, false, 1)
-        default:
-          if constexpr (K * 16 / (int)sizeof(T) == 8) {  // (what 640 threads have the registers for)
-            if (g.tpr == 640) return nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, true, 640, false, 1, false>>(p, g, st);
-          }
-      }
-    }
-    if (g.nv == K * g.tpr && set == 2) {
-      switch (g.tpr) {
-        FLN_NGA_BWD(8, false, 2)
-        FLN_NGA_BWD(16, false, 2)
-      }
-    }
+#define FLN_NGA_SHORT(TPR, SET) \
+  case TPR:                     \
+    if (whole) return nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, true, TPR, false, SET, false>>(p, g, st); \
+    break;
+#define FLN_NGA_RAG(TPR) \
+  case TPR:              \
+    return nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, true, TPR, true, 1, false>>(p, g, st);
+#define FLN_NGA_LONG(TPR)                                                                                          \
+  case TPR:                                                                                                        \
+    return whole ? nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, true, TPR, false, 1, false>>(p, g, st)          \
+                 : nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, true, TPR, true, 1, false>>(p, g, st);
     if (set == 1) {
       switch (g.tpr) {
-        FLN_NGA_BWD(128, true, 1)
-        FLN_NGA_BWD(192, true, 1)
-        FLN_NGA_BWD(256, true, 1)
-        FLN_NGA_BWD(320, true, 1)
-        FLN_NGA_BWD(384, true, 1)
-        FLN_NGA_BWD(512, true, 1)
+        FLN_NGA_SHORT(64, 1)
+        FLN_NGA_LONG(128)
+        FLN_NGA_RAG(192)
+        FLN_NGA_LONG(256)
+        FLN_NGA_LONG(320)
+        FLN_NGA_RAG(384)
+        FLN_NGA_LONG(512)
+      }
+      if constexpr (K * 16 / (int)sizeof(T) == 8) {  // (what 640 threads have the registers for)
+        switch (g.tpr) { FLN_NGA_LONG(640) }
       }
     }
-#undef FLN_NGA_BWD
+    if (set == 2) {
+      switch (g.tpr) {
+        FLN_NGA_SHORT(4, 2)
+        FLN_NGA_SHORT(8, 2)
+        FLN_NGA_SHORT(16, 2)
+        FLN_NGA_SHORT(32, 2)
+        FLN_NGA_SHORT(64, 2)
+      }
+    }
+#undef FLN_NGA_RAG
+#undef FLN_NGA_SHORT
+#undef FLN_NGA_LONG
   }
   if (set == 1) return nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 1, false>>(p, g, st);
   return nga_launch<nga_bwd_rows_kernel<T, K, GATE, GEN, true, 0, false, 0, false>>(p, g, st);

@@ -230,3 +230,49 @@ def test_unaligned_bias_beside_aligned_tensors(dtype, post):
     R.check(y.detach(), want["y"], "y"), R.check(s.detach(), want["sum"], "sum")
     for k, v in zip(leaves, torch.autograd.grad([y, s], list(leaves.values()), [dy, ds])):
         R.check(v, want["grads"][k], k)
+
+
+WIDTHS = [(F32, 4356), (F32, 4608), (F32, 4864), (F32, 5056), (F32, 5120), (BF16, 5064), (F16, 4888), (BF16, 3584), (F16, 7168),
+          (BF16, 6144), (F32, 1536), (BF16, 1528)]
+
+
+@pytest.mark.parametrize("dtype,h", WIDTHS, ids=str)
+@pytest.mark.parametrize("gate", ["none", "element"])
+@pytest.mark.parametrize("norm", ["rmsnorm", "layernorm"])
+def test_row_lengths_between_the_common_ones(dtype, h, gate, norm):
+    """Row lengths around those at which the number of threads per row, or what stays in shared memory,
+    changes, whole and not; with the residual and both gradients."""
+    check(dtype, (2, 33, h), gate, norm, norm, residual=True)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
+@pytest.mark.parametrize("h", [32, 64, 128, 256, 512, 120, 72])
+@pytest.mark.parametrize("gate", ["none", "vector", "element"])
+@pytest.mark.parametrize("post", ["rmsnorm", "layernorm"])
+def test_heads_without_a_second_norm(dtype, h, gate, post):
+    """The norm of a head and its gate, forward and backward, over rows that leave row groups empty."""
+    for rows in (1, 31, 700):
+        check(dtype, (1, rows, h), gate, post, "none", residual=False)
+
+
+def check(dtype, shape, gate, post, norm, residual):
+    g = torch.Generator().manual_seed(shape[-1] + shape[-2])
+    rn = lambda *s: torch.randn(*s, generator=g).to(dtype).cuda()
+    h, bias, act = shape[-1], post == "layernorm", "none" if gate == "none" else "silu"
+    t = dict.fromkeys(R.NAMES)
+    t.update(input=rn(*shape), residual=rn(*shape) if residual else None, post_weight=rn(h), post_bias=rn(h) if bias else None,
+             gate=None if gate == "none" else rn(*(shape if gate == "element" else (h,))))
+    if norm != "none":
+        t.update(weight=rn(h), bias=rn(h) if bias else None)
+    dy, ds = rn(*shape) if norm != "none" else None, rn(*shape)
+    d = lambda v: None if v is None else v.double()
+    want = R.nga_bounds({k: d(v) for k, v in t.items()}, d(dy), d(ds), dtype, post, norm, act, 0.7, 1.0, 0.0)
+    leaves = {k: v.detach().requires_grad_(True) for k, v in t.items() if v is not None}
+    y, s = fl.fused_norm_gate_add_norm(*[leaves.get(n) for n in R.NAMES], post_norm=post, norm=norm, gate_activation=act,
+                                       branch_scale=0.7, post_eps=R.EPS1, eps=R.EPS2)
+    R.check(s.detach(), want["sum"], "sum")
+    if y is not None:
+        R.check(y.detach(), want["y"], "y")
+    outs, gs = ([s], [ds]) if y is None else ([y, s], [dy, ds])
+    for k, v in zip(leaves, torch.autograd.grad(outs, list(leaves.values()), gs)):
+        R.check(v, want["grads"][k], k)
