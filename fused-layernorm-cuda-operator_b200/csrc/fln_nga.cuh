@@ -74,8 +74,11 @@ struct NgaParams {
 };
 constexpr int kAccP = 1, kAccQ = 2, kAccU = 4, kAccV = 8;
 
-// act(v) and act'(v).  32-bit types: the full-precision functions.  16-bit types: the hardware
-// exponential and reciprocal, relative error about 2^-21, far below the type's 2^-9.
+// act(v) and act'(v).  32-bit types: the full-precision exponential and tanh; the reciprocal is the
+// hardware's, good to one unit in the last place, where a correctly rounded one costs some eight
+// instructions.  16-bit types: the hardware exponential too.  Its argument v log2(e) is rounded to 24
+// bits, so a sigmoid is good to 2^-22 + |v| 2^-24 of itself: 2^-18 at v = -40, below the half step of
+// 2^-12 that fp16 has and the 2^-9 of bf16.
 template <bool EXACT>
 __device__ __forceinline__ float sigmoid_of(float v) {
   if (EXACT) return rcp_approx(1.0f + expf(-v));  // (the reciprocal is good to one unit in the last place)

@@ -17,8 +17,9 @@
 //     C2 = w2, B2 = b2            y  = sh * C2 + B2,                    g2 = dy * C2
 // The column sums P and Q are kept of ds (times a) and multiplied by ba when they are left.
 // The unfolded form on single floats took 48 (forward) and 84 (backward) instructions per element
-// at 16384 x 4096 bf16: 127 and 248 us.  As it is: 22 and 28, 90 and 147 us; 16384 x 8192: 170 us (6.3
-// TB/s of the 8 bytes per element) and 262 us (6.1 TB/s of 12), where HBM is the bound.
+// at 16384 x 4096 bf16: 127 and 248 us.  As it is: 20 and 28, 90 and 146 us (with the sums of its partial
+// rows); 16384 x 8192: 180 us (6.0 TB/s of the 8 bytes per element) and 261 us (6.2 TB/s of 12), where
+// HBM is the bound.
 //
 // SHIFT: rows that are not whole 16-byte vectors (tensors that start on a 16-byte boundary, row length
 // not a multiple of a vector).  Such a row starts at one of 2, 4 or 8 places of a vector, by its
@@ -26,7 +27,9 @@
 // the same place of the same thread's vectors.  So all that is above holds: the row is staged as
 // the vectors that cover it, what belongs to the neighbouring rows in its first and last vector is
 // set to zero, and only those two are stored element by element.  (Rows held element by element
-// instead: 16384 x 2777 bf16 at 190 us forward and 546 us backward; this way 123 and 205.)
+// instead: 16384 x 2777 bf16 at 190 us forward and 546 us backward; this way 123 and 203.  The general
+// form with a gate per element takes 246 and 498 there: its limits per vector and four column sums do
+// not fit the registers.)
 //
 // PAIR (backward): a row is shared by the two CTAs of a cluster, half of its vectors each, where one
 // CTA's registers do not hold it.  The row sums go through the shared memory of both and the
@@ -34,7 +37,10 @@
 // 4096 x 12288 bf16, 12 bytes per element: 235 us, 1590 with the looping kernels.
 //
 // GEN = false: both norms RMSNorm or none and no bias, which is what most blocks have; no means, no
-// Q and V.  GEN = true: everything.
+// Q and V.  GEN = true: everything, in more registers: 16384 x 4096 bf16, two LayerNorms with biases 135
+// and 208 us, with a sigmoid gate per element too 162 and 318 (1.6 to 2 times its bytes).  Backward rows
+// of 5121 to 8192 elements of 16 bits (fp32: past 5120) take 16 elements per thread, and there the
+// general form spills: 16384 x 8192 in 826 us, 3.4 times its bytes.
 #pragma once
 
 #include "fln_nga.cuh"

@@ -8,10 +8,11 @@ rmsnorm.py.
                              with one or several axes (time, height, width)
 
 Both take fp32, bf16 and fp16 CUDA tensors, keep everything between their inputs and outputs in
-32 bits, are differentiable (one C++ autograd node each; no second derivatives), launch on the
-current stream, can be captured into a CUDA graph, and trace under torch.compile.  As with every
-autograd function, capturing a backward pass needs leaves whose gradients no eager graph still
-refers to.
+32 bits, are differentiable (one C++ autograd node each; second and forward-mode derivatives are
+refused), launch on the current stream, can be captured into a CUDA graph, and trace under
+torch.compile, apart from fused_qk_norm_rotary_, which breaks the graph there and runs between its
+parts.  As with every autograd function, capturing a backward pass needs leaves whose gradients no
+eager graph still refers to.
 """
 from __future__ import annotations
 
@@ -59,7 +60,8 @@ def fused_norm_gate_add_norm(input: torch.Tensor, residual: Optional[torch.Tenso
     gate is [hidden], one vector for each entry of the first dimension
     ([input.shape[0], hidden], also with dimensions of size one in between), or of the shape of
     input; weight and bias are [hidden] or one vector for each entry of the first dimension (with
-    weight_offset=1 that is adaptive modulation, (1 + scale) and shift per sample).
+    weight_offset=1 that is adaptive modulation, (1 + scale) and shift per sample; the offset is
+    that of both norms).
 
     The sum stays in 32 bits for N2 and is rounded only where it is returned, so y may differ in
     its last bit from a norm taken of the returned sum.  Differentiable in all seven tensors; the
@@ -151,7 +153,8 @@ class RotaryAxes:
     "interleaved" pairs 2i with 2i + 1.  magnitude multiplies the rotated elements.
 
     Positions are whole numbers; the angle position * inv_freq is reduced exactly (to
-    |position| * 2**-65 turns), so far positions lose nothing."""
+    |position| * 2**-65 turns) and rounded to 32 bits only behind its whole quarter turns, so far
+    positions lose nothing and a cosine or sine is good to some 2**-22 of itself."""
 
     def __init__(self, head_dim: int, sections: Union[int, Sequence[int]], base: float = 10000.0, *,
                  per_axis: bool = False, layout: str = "half", inv_freq: Optional[Sequence[float]] = None,
@@ -252,8 +255,8 @@ def fused_qk_norm_rotary_(q: torch.Tensor, k: Optional[torch.Tensor], positions:
                           norm: Optional[str] = "rmsnorm", eps: float = 1e-6,
                           weight_offset: float = 0.0) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """fused_qk_norm_rotary written over q and k (returned): for serving, where the heads stay
-    inside the packed projection.  Records no gradient (call it under torch.no_grad() when q or k
-    require one) and needs strides that it can take as they are; q and k must not overlap."""
+    inside the packed projection.  Records no gradient (call it under torch.no_grad() when q, k or a
+    parameter requires one) and needs strides that it can take as they are; q and k must not overlap."""
     return _rotary_call(q, k, positions, rotary, q_weight, k_weight, q_bias, k_bias, norm, eps, weight_offset, True)
 
 
